@@ -24,6 +24,11 @@ QUANT_NAMES = {v: k for k, v in QUANT_IDS.items()}
 
 FRC_GEMV_ACCUMULATE = 1  # frc_gemv_ex flag
 
+# element types of the serving operators (GGML type ids)
+FRC_F32 = 0
+FRC_F16 = 1
+FRC_BF16 = 30
+
 # frc_set_option ids (include/frcuda.h FRC_OPT_*)
 OPTIONS = {"batch1_int16": 1, "batched_fp32": 2, "prefill_tc": 3, "prefill_splits": 4, "inject_oom": 5,
            "batch1_tc": 6}
@@ -60,6 +65,16 @@ SIGNATURES: dict[str, list] = {
     "frc_argmax": [_p, _i64, _p, _p, _p],
     "frc_embed_row": [_i, _p, _i64, _p, _p, _p],
     "frc_pos_advance": [_p, _p],
+    "frc_qk_norm_rope": [_i, _i, _p, _i64, _i64, _i, _i, _i, _p, _p, _p, ctypes.c_float, _p, _p, _i64, _i, _i, _p,
+                         _p, _i64, _p, _i64, _p, _i64, _p],
+    "frc_kv_q4_bytes": [_i64, _i, _i, _i, ctypes.POINTER(_sz)],
+    "frc_kv_append_q4": [_i, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i, _i, _i64, _i, _p, _p],
+    "frc_kv_read_q4": [_i, _p, _p, _i64, _i, _i, _i64, _i, _p, _i64, _i64, _p, _i64, _i64, _p],
+    "frc_attention_decode_q4_workspace": [_i, _i, _i, _i, ctypes.POINTER(_sz)],
+    "frc_attention_decode_q4": [_i, _p, _i64, _i64, _p, _i64, _i, _p, _i64, _i, _p, _i, _i, _i, _i, ctypes.c_float,
+                                _p, _sz, _p, _i64, _i64, _p],
+    "frc_attention_prefill": [_i, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i, _i64, _i64, _i, _i, _i,
+                              ctypes.c_float, _i, _p, _i64, _i64, _p],
     "frc_gemv": [_i, _p, _sz, _i64, _i64, _p, _i64, _p, _p],
     "frc_gemv_noalloc": [_i, _p, _sz, _i64, _i64, _p, _i64, _p, _p],
     "frc_ipc_alloc": [_sz, ctypes.POINTER(_p), _p],

@@ -1,0 +1,340 @@
+"""Serving operators around a 4-bit paged key/value cache, on torch tensors.
+
+What a prompt and the decode tokens of a batch of sequences need besides the
+projections (the C ABI's serving operators, include/frcuda.h; no reference
+counterpart: the reference forwarder keeps one sequence's fp32 cache in NumPy,
+flatrun/model/qwen2.py:1527-1614):
+
+  qk_norm_rope          bias, norms of query and key heads, position rotation
+  rope_tables_scaled    the rotation's tables, also for long contexts
+  kv_cache_q4           an empty 4-bit paged cache
+  kv_append_q4          keys and values of tokens into it
+  kv_read_q4            and back
+  attention_decode_q4   one query token a sequence over its cached tokens
+  attention_prefill     causal attention of whole packed prompts
+
+A step of a batch: ``qk_norm_rope``, then ``kv_append_q4`` of the new tokens,
+then ``attention_decode_q4`` with lengths that count them; a prompt attends
+through ``attention_prefill`` and is appended for the tokens that follow.
+
+Every call is enqueued on the current stream of its tensors' device and
+returns without waiting; positions, slots, tables and lengths are read on the
+device, so calls can be captured in a CUDA graph and replayed with new ones
+(pass ``out=`` to keep the results in place).  Arguments that do not fit raise
+ValueError before anything is launched.  Inference only: tensors that require
+gradients are refused while gradients are recorded.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import numpy as np
+import torch
+
+from . import _lib
+
+_TYPE = {torch.float32: _lib.FRC_F32, torch.float16: _lib.FRC_F16, torch.bfloat16: _lib.FRC_BF16}
+_BLOCK = 16  # tokens of a cache block
+
+
+def _need(cond: bool, what: str) -> None:
+    if not cond:
+        raise ValueError(what)
+
+
+def _launch(device: torch.device, fn, *args) -> None:
+    """fn(*args, stream) with `device` current, on its current stream."""
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc:
+        _lib.check(rc)
+
+
+def _same_cuda_device(tensors) -> torch.device:
+    device = tensors[0].device
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t.device != device:
+            raise ValueError(f"tensors on different devices: {device} and {t.device}")
+        if grad and t.requires_grad:
+            raise ValueError("the operator has no backward pass: call it under torch.no_grad()")
+    _need(device.type == "cuda", f"tensors must be on a CUDA device, not {device}")
+    return device
+
+
+def _index(t: torch.Tensor, name: str, dtype: torch.dtype, shape) -> None:
+    _need(t.dtype == dtype and tuple(t.shape) == tuple(shape) and t.is_contiguous(),
+          f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}")
+
+
+def _rows(t: torch.Tensor, name: str, shape, dtype: torch.dtype) -> None:
+    """A (rows, heads, head_dim) tensor with contiguous channels."""
+    _need(tuple(t.shape) == tuple(shape) and t.dtype == dtype,
+          f"{name} must be a {dtype} tensor of shape {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
+    _need(t.stride(-1) == 1 or t.shape[-1] == 1 or t.numel() == 0, f"the channels of {name} must be contiguous")
+
+
+# ---- position rotation ----------------------------------------------------------------
+def rope_tables_scaled(rot: int, theta: float, max_pos: int, scaling: dict | None = None):
+    """cos and sin tables [max_pos][rot / 2] in fp32 of the rotation by
+    position * theta^(-2 i / rot), with the angles in 64 bits, so that far
+    positions keep their phase.  `scaling` stretches them for long contexts:
+
+    * ``{"type": "linear", "factor": s}``: positions / s;
+    * ``{"type": "ntk", "factor": s}``: theta * s^(rot / (rot - 2)), which
+      stretches the slowest pair by s and leaves the fastest;
+    * ``{"type": "yarn", "factor": s, "original_max_position": n}``
+      (``beta_fast`` 32, ``beta_slow`` 1, ``attention_factor`` 0.1 ln s + 1):
+      pairs that turn more than beta_fast times in n positions stay, those below
+      beta_slow turns are divided by s, a linear ramp between; cos and sin
+      times the attention factor (Peng et al. 2023, arXiv 2309.00071);
+    * ``{"type": "llama3", "factor": s, "original_max_position": n}``
+      (``low_freq_factor`` 1, ``high_freq_factor`` 4): the same with the ramp
+      linear in the number of turns.
+    """
+    _need(rot > 0 and rot % 2 == 0 and max_pos > 0 and theta > 0, "rot must be even and max_pos and theta positive")
+    inv = float(theta) ** (-np.arange(0, rot, 2, dtype=np.float64) / rot)
+    magnitude = 1.0
+    if scaling is not None:
+        kind, s = scaling.get("type"), float(scaling.get("factor", 0.0))
+        _need(kind in ("linear", "ntk", "yarn", "llama3"), f"unknown rope scaling {kind!r}")
+        _need(s >= 1.0, "rope scaling needs a factor of at least 1")
+        if kind == "linear":
+            inv = inv / s
+        elif kind == "ntk":
+            _need(rot > 2, "ntk scaling needs more than one pair")
+            inv = (theta * s ** (rot / (rot - 2))) ** (-np.arange(0, rot, 2, dtype=np.float64) / rot)
+        else:
+            n = float(scaling.get("original_max_position", 0))
+            _need(n > 0, f"{kind} scaling needs original_max_position")
+            turns = n * inv / (2 * math.pi)
+            if kind == "yarn":
+                fast, slow = float(scaling.get("beta_fast", 32)), float(scaling.get("beta_slow", 1))
+                _need(fast > slow > 0, "yarn scaling needs beta_fast > beta_slow > 0")
+
+                def pair(r):  # the (fractional) pair that turns r times in n positions
+                    return rot * math.log(n / (r * 2 * math.pi)) / (2 * math.log(theta))
+
+                low = max(math.floor(pair(fast)), 0)
+                high = min(math.ceil(pair(slow)), rot - 1)
+                ramp = np.clip((np.arange(rot // 2) - low) / max(high - low, 1e-3), 0.0, 1.0)
+                inv = inv * (1 - ramp) + inv / s * ramp
+                magnitude = float(scaling.get("attention_factor", 0.1 * math.log(s) + 1.0))
+            else:
+                lo, hi = float(scaling.get("low_freq_factor", 1)), float(scaling.get("high_freq_factor", 4))
+                _need(hi > lo > 0, "llama3 scaling needs high_freq_factor > low_freq_factor > 0")
+                keep = np.clip((turns - lo) / (hi - lo), 0.0, 1.0)
+                inv = inv * keep + inv / s * (1 - keep)
+    angle = np.arange(max_pos, dtype=np.float64)[:, None] * inv
+    return (np.cos(angle) * magnitude).astype(np.float32), (np.sin(angle) * magnitude).astype(np.float32)
+
+
+def qk_norm_rope(qkv, heads: int, kv_heads: int, cos, sin, positions, *, bias=None, q_norm=None, k_norm=None,
+                 eps: float = 1e-6, interleaved: bool = False, out_dtype=None, out=None):
+    """Queries, keys and values of tokens, ready for attention, in one pass.
+
+    `qkv` (tokens, (heads + 2 kv_heads) * head_dim): rows [q | k | v], which
+    get `bias`, norms of each query and key head (weights `q_norm`, `k_norm` of
+    head_dim, RMS with `eps`) and the rotation at `positions` (int32) by
+    `cos` and `sin` (max_pos, rot / 2), fp32; rot may be less than head_dim.
+    Pairs are (i, i + rot / 2), or (2 i, 2 i + 1) if `interleaved`.  Rows whose
+    position is outside the tables are padding: their outputs are left as they
+    are (zeros where this call makes the outputs).
+
+    Returns q (tokens, heads, head_dim), k and v (tokens, kv_heads, head_dim)
+    in `out_dtype` (default: qkv's); `out` = (q, k, v) to write to, which may
+    be views of qkv itself.
+    """
+    _need(qkv.dim() == 2 and qkv.dtype in _TYPE, "qkv must be a 2-D fp32, fp16 or bf16 tensor")
+    _need(heads > 0 and kv_heads > 0, "heads and kv_heads must be positive")
+    tokens, n = qkv.shape
+    _need(n % (heads + 2 * kv_heads) == 0, f"rows of {n} do not hold {heads} + 2 * {kv_heads} heads")
+    hd = n // (heads + 2 * kv_heads)
+    _need(hd > 0 and hd % 2 == 0 and hd <= 256, f"head_dim must be even and at most 256, not {hd}")
+    _need(qkv.stride(1) == 1, "the rows of qkv must be contiguous")
+    _need(cos.dim() == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype == torch.float32 and
+          cos.is_contiguous() and sin.is_contiguous() and cos.shape[0] > 0,
+          "cos and sin must be contiguous fp32 tensors of one shape (max_pos, rot / 2)")
+    rot = 2 * cos.shape[1]
+    _need(rot <= hd, f"the tables rotate {rot} of {hd} channels")
+    _index(positions, "positions", torch.int32, (tokens,))
+    used = [qkv, cos, sin, positions]
+    for t, name, size in ((bias, "bias", n), (q_norm, "q_norm", hd), (k_norm, "k_norm", hd)):
+        if t is not None:
+            _index(t, name, torch.float32, (size,))
+            used.append(t)
+    if out is None:
+        dtype = out_dtype or qkv.dtype
+        _need(dtype in _TYPE, f"out_dtype must be fp32, fp16 or bf16, not {dtype}")
+        out = tuple(torch.zeros((tokens, h, hd), dtype=dtype, device=qkv.device) for h in (heads, kv_heads, kv_heads))
+    else:
+        _need(len(out) == 3, "out must be (q, k, v)")
+        dtype = out[0].dtype
+        _need(dtype in _TYPE and out_dtype in (None, dtype), "out has another type than out_dtype, or not fp32/fp16/bf16")
+        for t, name, h in zip(out, ("q", "k", "v"), (heads, kv_heads, kv_heads)):
+            _rows(t, f"out {name}", (tokens, h, hd), dtype)
+            _need(t.stride(1) == hd or h == 1 or tokens == 0, f"the heads of out {name} must be contiguous")
+    device = _same_cuda_device([*used, *out])
+    q, k, v = out
+    _launch(device, _lib.load().frc_qk_norm_rope, _TYPE[qkv.dtype], _TYPE[dtype], qkv.data_ptr(),
+            qkv.stride(0) if tokens > 1 else n, tokens, heads, kv_heads, hd,
+            bias.data_ptr() if bias is not None else None, q_norm.data_ptr() if q_norm is not None else None,
+            k_norm.data_ptr() if k_norm is not None else None, eps, cos.data_ptr(), sin.data_ptr(), cos.shape[0], rot,
+            1 if interleaved else 0, positions.data_ptr(), q.data_ptr(), q.stride(0) if tokens > 1 else heads * hd,
+            k.data_ptr(), k.stride(0) if tokens > 1 else kv_heads * hd, v.data_ptr(),
+            v.stride(0) if tokens > 1 else kv_heads * hd)
+    return out
+
+
+# ---- the cache ------------------------------------------------------------------------
+def kv_cache_q4(pages: int, page_size: int, kv_heads: int, head_dim: int, device="cuda") -> torch.Tensor:
+    """A 4-bit cache of `pages` pages of `page_size` tokens (a multiple of 16):
+    a uint8 tensor (pages, kv_heads, page_size / 16, 20 * head_dim), zeroed
+    (zeros stand for zeros).  head_dim is 64 or 128."""
+    _need(pages > 0 and kv_heads > 0, "pages and kv_heads must be positive")
+    _need(page_size > 0 and page_size % _BLOCK == 0, f"page_size must be a multiple of {_BLOCK}, not {page_size}")
+    _need(head_dim in (64, 128), f"head_dim must be 64 or 128, not {head_dim}")
+    return torch.zeros((pages, kv_heads, page_size // _BLOCK, 20 * head_dim), dtype=torch.uint8, device=device)
+
+
+def _cache(cache) -> tuple[int, int, int, int]:
+    _need(cache.dim() == 4 and cache.dtype == torch.uint8 and cache.is_contiguous() and cache.numel() > 0 and
+          cache.shape[3] in (20 * 64, 20 * 128),
+          "the cache must be a contiguous uint8 tensor (pages, kv_heads, page_size / 16, 20 * head_dim), "
+          "head_dim 64 or 128")
+    pages, kv_heads, blocks, nbytes = cache.shape
+    return pages, kv_heads, blocks * _BLOCK, nbytes // 20
+
+
+def kv_append_q4(cache, k, v, slots) -> None:
+    """Quantise keys and values (tokens, kv_heads, head_dim) into `slots`
+    (int64, page * page_size + offset) of the cache.  Slots outside the cache
+    are skipped (use -1 for padding rows); the others of one call must differ."""
+    pages, nkv, page, hd = _cache(cache)
+    _need(k.dtype in _TYPE, f"keys must be fp32, fp16 or bf16, not {k.dtype}")
+    tokens = k.shape[0] if k.dim() else 0
+    _rows(k, "k", (tokens, nkv, hd), k.dtype)
+    _rows(v, "v", (tokens, nkv, hd), k.dtype)
+    _index(slots, "slots", torch.int64, (tokens,))
+    device = _same_cuda_device((cache, k, v, slots))
+    _launch(device, _lib.load().frc_kv_append_q4, _TYPE[k.dtype], k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+            v.stride(0), v.stride(1), tokens, slots.data_ptr(), nkv, hd, pages, page, cache.data_ptr())
+
+
+def kv_read_q4(cache, slots, *, dtype=None, out=None):
+    """Keys and values (tokens, kv_heads, head_dim) that the cache holds in
+    `slots`, in `dtype` (default fp32) or into `out` = (k, v).  Rows whose slot
+    is outside the cache are left as they are (zeros where this call makes
+    the outputs)."""
+    pages, nkv, page, hd = _cache(cache)
+    _need(slots.dim() == 1, "slots must have one dimension")
+    tokens = slots.shape[0]
+    _index(slots, "slots", torch.int64, (tokens,))
+    if out is None:
+        dtype = dtype or torch.float32
+        _need(dtype in _TYPE, f"dtype must be fp32, fp16 or bf16, not {dtype}")
+        out = tuple(torch.zeros((tokens, nkv, hd), dtype=dtype, device=cache.device) for _ in range(2))
+    _need(len(out) == 2 and out[0].dtype in _TYPE and dtype in (None, out[0].dtype),
+          "out must be (k, v) in fp32, fp16 or bf16, of the type asked for")
+    k, v = out
+    _rows(k, "out k", (tokens, nkv, hd), k.dtype)
+    _rows(v, "out v", (tokens, nkv, hd), k.dtype)
+    device = _same_cuda_device((cache, slots, k, v))
+    _launch(device, _lib.load().frc_kv_read_q4, _TYPE[k.dtype], cache.data_ptr(), slots.data_ptr(), tokens, nkv, hd,
+            pages, page, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1))
+    return out
+
+
+# ---- attention ----------------------------------------------------------------------------
+_workspace_bytes: dict = {}
+
+
+def _decode_q4_workspace(batch: int, nh: int, nkv: int, hd: int) -> int:
+    key = (batch, nh, nkv, hd)
+    if key not in _workspace_bytes:
+        ws = ctypes.c_size_t()
+        _lib.check(_lib.load().frc_attention_decode_q4_workspace(batch, nh, nkv, hd, ctypes.byref(ws)))
+        _workspace_bytes[key] = int(ws.value)
+    return _workspace_bytes[key]
+
+
+def attention_decode_q4(q, cache, block_table, lengths, *, scale: float | None = None, out=None):
+    """Attention of one query token a sequence over the 4-bit cache.
+
+    `q` (batch, heads, head_dim), fp32, fp16 or bf16, heads a multiple of the
+    cache's; sequence b's tokens 0 .. lengths[b] - 1 lie in pages
+    block_table[b] (int32, (batch, max_pages)), the t-th in entry
+    t // page_size.  `scale` defaults to head_dim^-1/2.  Page numbers outside
+    the cache hide their tokens, lengths are held to what the table covers, and
+    a sequence without tokens gives zeros.  Returns (batch, heads, head_dim) in
+    q's type, into `out` where given.
+    """
+    pages, nkv, page, hd = _cache(cache)
+    _need(q.dim() == 3 and q.dtype in _TYPE, "q must be (batch, heads, head_dim) in fp32, fp16 or bf16")
+    batch, nh = q.shape[0], q.shape[1]
+    _rows(q, "q", (batch, nh, hd), q.dtype)
+    _need(nh > 0 and nh % nkv == 0, f"{nh} query heads are not a multiple of the cache's {nkv}")
+    _need(block_table.dim() == 2, "block_table must be (batch, max_pages)")
+    _index(block_table, "block_table", torch.int32, (batch, block_table.shape[1]))
+    _index(lengths, "lengths", torch.int32, (batch,))
+    if out is None:
+        out = torch.empty((batch, nh, hd), dtype=q.dtype, device=q.device)
+    else:
+        _rows(out, "out", (batch, nh, hd), q.dtype)
+    device = _same_cuda_device((q, cache, block_table, lengths, out))
+    ws = torch.empty(_decode_q4_workspace(batch, nh, nkv, hd), dtype=torch.uint8, device=device)
+    _launch(device, _lib.load().frc_attention_decode_q4, _TYPE[q.dtype], q.data_ptr(), q.stride(0), q.stride(1),
+            cache.data_ptr(), pages, page, block_table.data_ptr(), block_table.shape[1], block_table.shape[1],
+            lengths.data_ptr(), batch, nh, nkv, hd, hd ** -0.5 if scale is None else scale, ws.data_ptr(), ws.numel(),
+            out.data_ptr(), out.stride(0), out.stride(1))
+    return out
+
+
+def attention_prefill(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: float | None = None, out=None):
+    """Attention of whole prompts, packed one after the other.
+
+    `q` (tokens, heads, head_dim), `k` and `v` (key tokens, kv_heads,
+    head_dim), fp16 or bf16, head_dim 64 or 128, heads a multiple of kv_heads;
+    sequence b is rows cu_q[b] .. cu_q[b + 1] of q and cu_k[b] .. cu_k[b + 1] of
+    k and v (int32, batch + 1 ends that do not fall; `cu_k` defaults to `cu_q`).
+    Causal: the last query of a sequence sees all its keys, each earlier one a
+    key less, so a prompt may go on behind tokens that came before.  A query that
+    sees no key gives zeros; rows of no sequence are left as they are (zeros
+    where this call makes the output).  `scale` defaults to head_dim^-1/2.
+    """
+    _need(q.dim() == 3 and q.dtype in (torch.float16, torch.bfloat16), "q must be (tokens, heads, head_dim), fp16 or bf16")
+    _need(k.dim() == 3, "k must be (tokens, kv_heads, head_dim)")
+    tokens, nh, hd = q.shape
+    tokens_k, nkv = k.shape[0], k.shape[1]
+    _need(hd in (64, 128), f"head_dim must be 64 or 128, not {hd}")
+    _rows(q, "q", (tokens, nh, hd), q.dtype)
+    _rows(k, "k", (tokens_k, nkv, hd), q.dtype)
+    _rows(v, "v", (tokens_k, nkv, hd), q.dtype)
+    _need(nkv > 0 and nh > 0 and nh % nkv == 0, f"{nh} query heads are not a multiple of {nkv} key heads")
+    if cu_k is None:
+        cu_k = cu_q
+    _need(cu_q.dim() == 1 and cu_q.shape[0] >= 1, "cu_q must hold batch + 1 ends")
+    _index(cu_q, "cu_q", torch.int32, cu_q.shape)
+    _index(cu_k, "cu_k", torch.int32, cu_q.shape)
+    if out is None:
+        out = torch.zeros((tokens, nh, hd), dtype=q.dtype, device=q.device)
+    else:
+        _rows(out, "out", (tokens, nh, hd), q.dtype)
+    for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
+        _need(t.numel() == 0 or (t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0),
+              f"{name} must be 16-byte aligned, with row and head strides that are multiples of 8")
+    device = _same_cuda_device((q, k, v, cu_q, cu_k, out))
+    _launch(device, _lib.load().frc_attention_prefill, _TYPE[q.dtype], q.data_ptr(), q.stride(0), q.stride(1),
+            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), cu_q.data_ptr(),
+            cu_k.data_ptr(), cu_q.shape[0] - 1, tokens, tokens_k, nh, nkv, hd, hd ** -0.5 if scale is None else scale,
+            1 if causal else 0, out.data_ptr(), out.stride(0), out.stride(1))
+    return out
+
+
+__all__ = ["qk_norm_rope", "rope_tables_scaled", "kv_cache_q4", "kv_append_q4", "kv_read_q4", "attention_decode_q4",
+           "attention_prefill"]

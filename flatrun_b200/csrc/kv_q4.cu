@@ -1,0 +1,252 @@
+// Writing keys and values into the 4-bit paged cache, and reading them back.
+//
+// Of the 32 values x of a group, in exact arithmetic:
+//   m = fp16(min x), held within +-65504
+//   d = fp16((max x - m) / 15), held within 0 .. 65504
+//   n = round((x - m) / d) to the nearest integer, ties to even, held within
+//       0 .. 15 (0 where d = 0)
+// and a group with a value that is not finite gets m = NaN, so that it reads
+// back as NaN.  The quotients are formed in fp32; where one lies so near a
+// border between two results that fp32 could fall on the wrong side, that
+// lane forms it in fp64 (exact for these operands: an fp32 difference and a
+// quotient by at most 11 bits that is nowhere within 2^-53 of a border without
+// being on it), so the cache's bits follow from the definition alone.
+//
+// Bound by HBM: 2 or 4 bytes a value in, 5/8 of a byte out (append), and the
+// reverse (read).  A warp takes eight tokens of one head, four lanes a token
+// and eight channels a lane, one group at a time: a group's minimum and maximum
+// are two shuffles, a lane's eight nibbles are one word, a token's K words one
+// 4 NG byte store, and the V words of eight consecutive tokens a full 32-byte
+// sector.
+#include <cuda_runtime.h>
+
+#include <cstdio>
+
+#include "../../include/frcuda.h"
+#include "kv_q4.cuh"
+
+namespace frc {
+
+struct KvQ4Params {
+  uint8_t* cache;
+  int64_t pages;
+  int nkv, blocks_per_page;
+  const int64_t* slots;
+  int64_t tokens;
+  const void *k, *v;     // append: inputs; read: outputs
+  int64_t k_tok, k_head, v_tok, v_head;  // strides in elements
+};
+
+constexpr int kQ4Threads = 256;
+
+// fp16 of v / 15, v >= 0, rounded once.  The fp32 quotient is within 3 ulp
+// (three roundings); 13 of its bits are dropped, so only within 4 ulp of their
+// middle can the rounding fall on the wrong side (below fp16's normal range
+// more bits are dropped: there the quotient is formed in fp64).
+FRC_DEVICE_INLINE __half half_fifteenth(double v) {
+  const float f = static_cast<float>(v) * (1.0f / 15.0f);
+  const uint32_t low = __float_as_uint(f) & 0x1fffu;
+  if (f < 6.2e-5f || (low >= 0x1000u - 4u && low <= 0x1000u + 4u)) return __double2half(v / 15.0);
+  return __float2half_rn(f);
+}
+
+// The lane's eight values of a group shared by the four lanes of its quad:
+// its nibbles as one word, and the group's step and offset.
+FRC_DEVICE_INLINE uint32_t quantise8(const float (&x)[8], __half& step, __half& offset) {
+  float lo = x[0], hi = x[0];
+  bool finite = true;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    lo = fminf(lo, x[i]);
+    hi = fmaxf(hi, x[i]);
+    finite = finite && fabsf(x[i]) <= 3.402823466e38f;  // false for NaN too
+  }
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    finite = __shfl_xor_sync(0xffffffffu, finite ? 1 : 0, o) && finite;
+  }
+  offset = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f));
+  const float m = __half2float(offset);
+  const double range = static_cast<double>(hi) - static_cast<double>(m);
+  step = range >= 15.0 * 65504.0 ? __ushort_as_half(0x7bff) : half_fifteenth(range > 0.0 ? range : 0.0);
+  const float d = __half2float(step);
+  if (!finite) {
+    offset = __ushort_as_half(0x7fff);
+    step = __ushort_as_half(0);
+    return 0u;
+  }
+  if (d == 0.f) return 0u;
+  const float inv = 1.0f / d;
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    // relative error of t: 2^-24 each of the difference, the reciprocal and
+    // the product: below 3e-6 at 15.5
+    const float t = fminf(fmaxf((x[i] - m) * inv, 0.f), 15.f);
+    float r = rintf(t);
+    if (fabsf(fabsf(t - r) - 0.5f) < 4e-6f)
+      r = static_cast<float>(fmin(fmax(rint((static_cast<double>(x[i]) - static_cast<double>(m)) /
+                                            static_cast<double>(d)), 0.0), 15.0));
+    w |= static_cast<uint32_t>(r) << (4 * i);
+  }
+  return w;
+}
+
+template <int NG>
+FRC_DEVICE_INLINE void store_words(uint8_t* p, const uint32_t (&w)[NG]) {
+  if constexpr (NG == 4) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  else if constexpr (NG == 2) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  else
+#pragma unroll
+    for (int j = 0; j < NG; ++j) reinterpret_cast<uint32_t*>(p)[j] = w[j];
+}
+
+// warp -> (eight tokens, K or V, head); lane -> (token, q)
+FRC_DEVICE_INLINE bool q4_warp_item(const KvQ4Params& p, int64_t& tok, int& is_v, int& h, int& q, int64_t& block,
+                                    int& t) {
+  const int64_t warp = (static_cast<int64_t>(blockIdx.x) * kQ4Threads + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  const int64_t tg = warp / (2 * p.nkv);
+  const int rest = static_cast<int>(warp - tg * (2 * p.nkv));
+  is_v = rest >= p.nkv;
+  h = is_v ? rest - p.nkv : rest;
+  tok = tg * 8 + (lane >> 2);
+  q = lane & 3;
+  block = -1;
+  t = 0;
+  if (tok < p.tokens) {
+    const int64_t slot = p.slots[tok];
+    block = q4_block_of_slot(slot, h, p.pages, p.nkv, p.blocks_per_page);
+    t = static_cast<int>(slot) & (kQ4Tokens - 1);
+  }
+  return tg * 8 < p.tokens;  // the same in all lanes
+}
+
+template <typename T, int HD, bool VEC>
+__global__ void __launch_bounds__(kQ4Threads) kv_append_q4_kernel(KvQ4Params p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" :::);
+  constexpr Q4Layout lay(HD);
+  constexpr int NG = HD / kQ4Group;
+  int64_t tok, block;
+  int is_v, h, q, t;
+  if (!q4_warp_item(p, tok, is_v, h, q, block, t)) return;
+  const bool live = block >= 0;
+  const T* src = static_cast<const T*>(is_v ? p.v : p.k) + (live ? tok : 0) * (is_v ? p.v_tok : p.k_tok) +
+                 h * (is_v ? p.v_head : p.k_head);
+  uint8_t* blk = p.cache + (live ? block : 0) * lay.block_bytes();
+  float x[NG][8];
+#pragma unroll
+  for (int j = 0; j < NG; ++j) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[j][i] = 0.f;
+    if (live) load_run<8, VEC>(src + kQ4Group * j + 8 * q, x[j]);
+  }
+  uint32_t w[NG];
+#pragma unroll
+  for (int j = 0; j < NG; ++j) {
+    __half d, m;
+    w[j] = quantise8(x[j], d, m);
+    if (!live) continue;
+    if (is_v) *reinterpret_cast<uint32_t*>(blk + lay.v_word(4 * j + q, t)) = w[j];
+    if (q == (j & 3)) {  // the lanes of a quad share the group's scales
+      *reinterpret_cast<__half*>(blk + (is_v ? lay.v_step(j, t) : lay.k_step(j, t))) = d;
+      *reinterpret_cast<__half*>(blk + (is_v ? lay.v_offset(j, t) : lay.k_offset(t, j))) = m;
+    }
+  }
+  if (live && !is_v) store_words(blk + lay.k_word(t, q, 0), w);
+}
+
+template <typename T, int HD, bool VEC>
+__global__ void __launch_bounds__(kQ4Threads) kv_read_q4_kernel(KvQ4Params p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" :::);
+  constexpr Q4Layout lay(HD);
+  constexpr int NG = HD / kQ4Group;
+  int64_t tok, block;
+  int is_v, h, q, t;
+  if (!q4_warp_item(p, tok, is_v, h, q, block, t) || block < 0) return;  // a row outside the cache stays as it is
+  const uint8_t* blk = p.cache + block * lay.block_bytes();
+  T* dst = static_cast<T*>(const_cast<void*>(is_v ? p.v : p.k)) + tok * (is_v ? p.v_tok : p.k_tok) +
+           h * (is_v ? p.v_head : p.k_head);
+  uint32_t w[NG];
+  float d[NG], m[NG];
+#pragma unroll
+  for (int j = 0; j < NG; ++j) {
+    w[j] = *reinterpret_cast<const uint32_t*>(blk + (is_v ? lay.v_word(4 * j + q, t) : lay.k_word(t, q, j)));
+    d[j] = __half2float(*reinterpret_cast<const __half*>(blk + (is_v ? lay.v_step(j, t) : lay.k_step(j, t))));
+    m[j] = __half2float(*reinterpret_cast<const __half*>(blk + (is_v ? lay.v_offset(j, t) : lay.k_offset(t, j))));
+  }
+#pragma unroll
+  for (int j = 0; j < NG; ++j) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = fmaf(static_cast<float>((w[j] >> (4 * i)) & 15u), d[j], m[j]);
+    store_run<8, VEC>(dst + kQ4Group * j + 8 * q, x);
+  }
+}
+
+template <bool READ>
+int kv_q4_call(const char* what, int type, KvQ4Params p, int hd, int page_size, void* stream) {
+  if (!frc_is_float_type(type)) return frc__fail(FRC_ERR_INVALID, "kv_q4: type must be FRC_F32, FRC_F16 or FRC_BF16");
+  FRC_REQUIRE(hd == 64 || hd == 128, "kv_q4: head_dim must be 64 or 128");
+  FRC_REQUIRE(p.nkv > 0 && p.nkv <= 65535 && p.pages > 0, "kv_q4: bad pages or heads");
+  FRC_REQUIRE(page_size > 0 && page_size % kQ4Tokens == 0, "kv_q4: page_size must be a multiple of 16");
+  p.blocks_per_page = page_size / kQ4Tokens;
+  FRC_REQUIRE(p.pages <= 0x7fffffff / p.blocks_per_page, "kv_q4: too many blocks in the cache");
+  FRC_REQUIRE(p.tokens >= 0 && p.tokens <= 0x7fffffff / (2 * p.nkv), "kv_q4: bad number of tokens");
+  FRC_REQUIRE(p.k_tok >= 0 && p.k_head >= 0 && p.v_tok >= 0 && p.v_head >= 0, "kv_q4: negative stride");
+  if (p.tokens == 0) return FRC_OK;
+  FRC_REQUIRE(p.cache && p.slots && p.k && p.v, "kv_q4: null pointer");
+  FRC_REQUIRE(aligned_to(p.cache, 16), "kv_q4: the cache must be 16-byte aligned");
+  const int run = type == FRC_F32 ? 4 : 8;  // elements of a 16-byte load
+  const bool vec = aligned_to(p.k, 16) && aligned_to(p.v, 16) && p.k_tok % run == 0 && p.k_head % run == 0 &&
+                   p.v_tok % run == 0 && p.v_head % run == 0;
+  const int64_t warps = (p.tokens + 7) / 8 * 2 * p.nkv;
+  const dim3 grid(static_cast<unsigned>((warps * 32 + kQ4Threads - 1) / kQ4Threads));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return frc_with_type(type, [&](auto* z) -> int {
+    using T = std::remove_pointer_t<decltype(z)>;
+    void (*fn)(KvQ4Params);
+    if constexpr (READ)
+      fn = hd == 128 ? (vec ? kv_read_q4_kernel<T, 128, true> : kv_read_q4_kernel<T, 128, false>)
+                     : (vec ? kv_read_q4_kernel<T, 64, true> : kv_read_q4_kernel<T, 64, false>);
+    else
+      fn = hd == 128 ? (vec ? kv_append_q4_kernel<T, 128, true> : kv_append_q4_kernel<T, 128, false>)
+                     : (vec ? kv_append_q4_kernel<T, 64, true> : kv_append_q4_kernel<T, 64, false>);
+    FRC_LAUNCHED(launch_pdl(fn, grid, dim3(kQ4Threads), 0, st, p), what);
+    return FRC_OK;
+  });
+}
+
+}  // namespace frc
+
+extern "C" {
+
+int frc_kv_q4_bytes(int64_t pages, int page_size, int nkv, int hd, size_t* bytes) {
+  FRC_REQUIRE(bytes && pages > 0 && nkv > 0 && page_size > 0 && page_size % frc::kQ4Tokens == 0 &&
+                  (hd == 64 || hd == 128) && pages <= 0x7fffffff / (page_size / frc::kQ4Tokens),
+              "frc_kv_q4_bytes: needs pages, heads, a page_size that is a multiple of 16 and head_dim 64 or 128");
+  *bytes = static_cast<size_t>(pages) * nkv * (page_size / frc::kQ4Tokens) * frc::Q4Layout(hd).block_bytes();
+  return FRC_OK;
+}
+
+int frc_kv_append_q4(int type, const void* k, int64_t k_tok_stride, int64_t k_head_stride, const void* v,
+                     int64_t v_tok_stride, int64_t v_head_stride, int64_t tokens, const int64_t* slots_dev, int nkv,
+                     int hd, int64_t pages, int page_size, void* cache, void* stream) {
+  const frc::KvQ4Params p{static_cast<uint8_t*>(cache), pages, nkv, 0, slots_dev, tokens, k, v,
+                          k_tok_stride, k_head_stride, v_tok_stride, v_head_stride};
+  return frc::kv_q4_call<false>("kv_append_q4 launch", type, p, hd, page_size, stream);
+}
+
+int frc_kv_read_q4(int type, const void* cache, const int64_t* slots_dev, int64_t tokens, int nkv, int hd,
+                   int64_t pages, int page_size, void* k, int64_t k_tok_stride, int64_t k_head_stride, void* v,
+                   int64_t v_tok_stride, int64_t v_head_stride, void* stream) {
+  const frc::KvQ4Params p{static_cast<uint8_t*>(const_cast<void*>(cache)), pages, nkv, 0, slots_dev, tokens, k, v,
+                          k_tok_stride, k_head_stride, v_tok_stride, v_head_stride};
+  return frc::kv_q4_call<true>("kv_read_q4 launch", type, p, hd, page_size, stream);
+}
+
+}  // extern "C"

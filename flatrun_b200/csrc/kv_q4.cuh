@@ -1,0 +1,160 @@
+// The 4-bit paged key/value cache: its layout, and the element types of the
+// serving operators that surround it.
+//
+// A cache is (pages, kv_heads, page_size / 16) blocks.  A block holds 16
+// tokens of one KV head; a token's D channels are quantised in groups of 32,
+// value = d * n + m with an fp16 step d, an fp16 offset m and n in 0..15: 5
+// bits a value with its share of the scales.  Inside a block (NG = D / 32
+// groups; nibble i of a 32-bit word is bits 4i..4i+3, words little-endian):
+//
+//   bytes          what                              read by attention as
+//   [0, 8D)        K nibbles: words (16 tokens, 4, NG); word (q, j) of a
+//                  token has channels 32 j + 8 q .. + 7
+//                                     one 4 NG byte load a lane: the lanes of
+//                                     a quad hold the 32 channels of each group
+//   [8D, 16D)      V nibbles: words (D / 8, 16 tokens); word w has channels
+//                  8 w .. 8 w + 7     one 16-byte load a lane: four tokens
+//   then halves    K steps (NG, 16 tokens), K offsets (16 tokens, NG),
+//                  V steps (NG, 16), V offsets (NG, 16)
+//
+// The order makes every operand of the tensor-core products one aligned
+// vector load away from its fragment, and one block one contiguous copy of
+// 20 D bytes.  No byte is shared by two tokens, so tokens are written without
+// reading the cache.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "frc_common.cuh"
+
+namespace frc {
+
+constexpr int kQ4Tokens = 16;   // tokens of a block
+constexpr int kQ4Group = 32;    // channels of a quantisation group
+
+struct Q4Layout {
+  int hd, ng;
+  __host__ __device__ constexpr explicit Q4Layout(int hd_) : hd(hd_), ng(hd_ / kQ4Group) {}
+  __host__ __device__ constexpr int block_bytes() const { return 20 * hd; }
+  // byte offsets inside a block
+  __host__ __device__ constexpr int k_word(int t, int q, int j) const { return 4 * ((t * 4 + q) * ng + j); }
+  __host__ __device__ constexpr int v_word(int w, int t) const { return 8 * hd + 4 * (w * kQ4Tokens + t); }
+  __host__ __device__ constexpr int k_step(int j, int t) const { return 16 * hd + 2 * (j * kQ4Tokens + t); }
+  __host__ __device__ constexpr int k_offset(int t, int j) const { return 17 * hd + 2 * (t * ng + j); }
+  __host__ __device__ constexpr int v_step(int j, int t) const { return 18 * hd + 2 * (j * kQ4Tokens + t); }
+  __host__ __device__ constexpr int v_offset(int j, int t) const { return 19 * hd + 2 * (j * kQ4Tokens + t); }
+};
+
+// Index of the block that holds slot `slot` of head `h`, or -1 where the slot
+// is outside the cache (a padding row, or a bad index: never touched).
+__host__ __device__ inline int64_t q4_block_of_slot(int64_t slot, int h, int64_t pages, int nkv, int blocks_per_page) {
+  if (slot < 0 || slot >= pages * blocks_per_page * kQ4Tokens) return -1;
+  const uint32_t block = static_cast<uint32_t>(slot >> 4);  // pages * blocks_per_page < 2^31 (checked by the host)
+  const uint32_t page = block / static_cast<uint32_t>(blocks_per_page);
+  return (static_cast<int64_t>(page) * nkv + h) * blocks_per_page + (block - page * blocks_per_page);
+}
+
+// Element types: values are computed in fp32 and rounded once when stored.
+FRC_DEVICE_INLINE float to_f32(float v) { return v; }
+FRC_DEVICE_INLINE float to_f32(__half v) { return __half2float(v); }
+FRC_DEVICE_INLINE float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+FRC_DEVICE_INLINE void from_f32(float v, float& o) { o = v; }
+FRC_DEVICE_INLINE void from_f32(float v, __half& o) { o = __float2half_rn(v); }
+FRC_DEVICE_INLINE void from_f32(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
+
+// N consecutive elements at p as fp32, and back.  VEC: p is aligned to the
+// run (at most 16 bytes); otherwise one element at a time.
+template <int N, bool VEC, typename T>
+FRC_DEVICE_INLINE void load_run(const T* p, float (&v)[N]) {
+  if constexpr (VEC) {
+    constexpr int B = N * sizeof(T) < 16 ? N * sizeof(T) : 16, E = B / sizeof(T);
+    struct alignas(B) Run { T e[E]; };
+#pragma unroll
+    for (int i = 0; i < N / E; ++i) {
+      const Run r = reinterpret_cast<const Run*>(p)[i];
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[i * E + j] = to_f32(r.e[j]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = to_f32(p[i]);
+  }
+}
+
+template <int N, bool VEC, typename T>
+FRC_DEVICE_INLINE void store_run(T* p, const float (&v)[N]) {
+  if constexpr (VEC) {
+    constexpr int B = N * sizeof(T) < 16 ? N * sizeof(T) : 16, E = B / sizeof(T);
+    struct alignas(B) Run { T e[E]; };
+#pragma unroll
+    for (int i = 0; i < N / E; ++i) {
+      Run r;
+#pragma unroll
+      for (int j = 0; j < E; ++j) from_f32(v[i * E + j], r.e[j]);
+      reinterpret_cast<Run*>(p)[i] = r;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) from_f32(v[i], p[i]);
+  }
+}
+
+}  // namespace frc
+
+// ---- host side: shared by the entry points ---------------------------------------
+
+// Defined in frcuda_api.cu: records a message for frc_last_error.
+extern "C" int frc__fail(int code, const char* msg);
+
+namespace frc {
+
+// Launch with the programmatic-stream-serialization attribute: every kernel
+// launched so waits for its predecessor (griddepcontrol.wait) before it
+// touches memory.
+template <typename... P, typename... A>
+inline cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+}  // namespace frc
+
+#define FRC_REQUIRE(cond, msg)                          \
+  do {                                                  \
+    if (!(cond)) return frc__fail(FRC_ERR_INVALID, msg); \
+  } while (0)
+
+#define FRC_LAUNCHED(expr, what)                                                               \
+  do {                                                                                         \
+    const cudaError_t _e = (expr);                                                             \
+    if (_e != cudaSuccess) {                                                                   \
+      char _msg[192];                                                                          \
+      snprintf(_msg, sizeof _msg, "%s: %s", what, cudaGetErrorString(_e));                     \
+      (void)cudaGetLastError();                                                                \
+      return frc__fail(FRC_ERR_CUDA, _msg);                                                    \
+    }                                                                                          \
+  } while (0)
+
+// Calls f with a null pointer of the element type `type` (FRC_F32, FRC_F16
+// or FRC_BF16, checked before).
+template <typename F>
+inline int frc_with_type(int type, F&& f) {
+  if (type == FRC_F32) return f(static_cast<float*>(nullptr));
+  if (type == FRC_F16) return f(static_cast<__half*>(nullptr));
+  return f(static_cast<__nv_bfloat16*>(nullptr));
+}
+inline bool frc_is_float_type(int type) { return type == FRC_F32 || type == FRC_F16 || type == FRC_BF16; }

@@ -243,6 +243,79 @@ int frc_argmax(const float* x, int64_t n, int* out_dev, void* workspace, void* s
 int frc_embed_row(int quant, const void* table, int64_t n, const int* tok_dev, float* out, void* stream);
 int frc_pos_advance(int* pos_dev, void* stream);
 
+/* ---- serving operators around a 4-bit paged KV cache ---------------------- *
+ * No reference counterpart (the reference keeps one sequence's cache in fp32
+ * NumPy arrays, flatrun/model/qwen2.py:1585-1614).  For prompts and for batches
+ * of sequences: queries, keys and values made ready for attention, a KV cache
+ * of 5 bits a value in pages, attention over it, and attention of whole
+ * prompts.  Stream-ordered on the current device, no synchronisation, no
+ * allocation, graph capturable; positions, slots, tables and lengths are read
+ * from device memory, so captured launches replay with new ones.  Strides are
+ * in elements; the channels of a head are contiguous.  Element types: */
+#define FRC_F32   0   /* the GGML type ids, as the quants */
+#define FRC_F16   1
+#define FRC_BF16 30
+/*  frc_qk_norm_rope: of each of `tokens` rows [q (nh*hd) | k (nkv*hd) | v (nkv*hd)]
+ *    (in_type, row_stride between rows): adds `bias` (same layout; NULL: none);
+ *    scales each q and k head by 1 / sqrt(mean(h^2) + eps) and the weights
+ *    q_norm / k_norm (hd; NULL: no norm); rotates the first `rot` channels of
+ *    each q and k head by the angles at position pos_dev[row] of the tables
+ *    [max_pos][rot / 2], pairs (i, i + rot/2), or (2i, 2i + 1) if interleaved;
+ *    writes q, k and v rows (heads contiguous) in out_type.  Rows whose
+ *    position is outside [0, max_pos) are padding: their outputs stay as they
+ *    are.  Computed in fp32.  The outputs may be the parts of the input rows
+ *    themselves (same type and strides).  hd even, at most 256.
+ *  The 4-bit cache: (pages, nkv, page_size / 16) blocks of 20 * hd bytes
+ *    (frc_kv_q4_bytes in all), hd 64 or 128, page_size a multiple of 16; a slot is
+ *    page * page_size + offset.  Of each 32 channels of a token: m = fp16(min),
+ *    d = fp16((max - m) / 15), n = round((x - m) / d) in 0..15 (ties to even,
+ *    exact arithmetic), value d * n + m; values beyond fp16's range are held
+ *    at its ends, and a group with a value that is not finite reads back as
+ *    NaN.  The block's layout stands in csrc/kv_q4.cuh.
+ *  frc_kv_append_q4: quantises rows k[i], v[i] ([nkv][hd]) into slot
+ *    slots_dev[i]; slots outside the cache are skipped (padding rows).  The slots
+ *    of one call must differ: where two rows share one, it holds parts of
+ *    both.
+ *  frc_kv_read_q4: the values of slots_dev[i] into k[i], v[i]; rows whose slot is
+ *    outside the cache stay as they are.
+ *  frc_attention_decode_q4: for each sequence one query token q[b] ([nh][hd])
+ *    over its first lengths[b] cached tokens, the t-th in page
+ *    block_table[b][t / page_size]: softmax(q.k * scale) . v per head, query
+ *    head h reading KV head h / (nh / nkv).  Page numbers outside the cache hide
+ *    their tokens, lengths are held within 0 and max_pages * page_size, and a
+ *    sequence without tokens gives zeros.  `workspace` holds
+ *    frc_attention_decode_q4_workspace bytes, in any state; calls that can
+ *    overlap in time need one each.
+ *  frc_attention_prefill: packed sequences, sequence b being rows
+ *    cu_q[b] .. cu_q[b + 1] of q and out and rows cu_k[b] .. cu_k[b + 1] of k
+ *    and v; causal: the last query of a sequence sees all its keys, each
+ *    earlier one a key less.  A query that sees no key gives zeros; rows of no
+ *    sequence stay as they are.  type FRC_F16 or FRC_BF16, hd 64 or 128;
+ *    pointers 16-byte aligned and strides multiples of 8. */
+int frc_qk_norm_rope(int in_type, int out_type, const void* qkv, int64_t row_stride, int64_t tokens, int nh, int nkv,
+                     int hd, const float* bias, const float* q_norm, const float* k_norm, float eps,
+                     const float* cos_table, const float* sin_table, int64_t max_pos, int rot, int interleaved,
+                     const int* pos_dev, void* q_out, int64_t q_stride, void* k_out, int64_t k_stride, void* v_out,
+                     int64_t v_stride, void* stream);
+int frc_kv_q4_bytes(int64_t pages, int page_size, int nkv, int hd, size_t* bytes);
+int frc_kv_append_q4(int type, const void* k, int64_t k_tok_stride, int64_t k_head_stride, const void* v,
+                     int64_t v_tok_stride, int64_t v_head_stride, int64_t tokens, const int64_t* slots_dev, int nkv,
+                     int hd, int64_t pages, int page_size, void* cache, void* stream);
+int frc_kv_read_q4(int type, const void* cache, const int64_t* slots_dev, int64_t tokens, int nkv, int hd,
+                   int64_t pages, int page_size, void* k, int64_t k_tok_stride, int64_t k_head_stride, void* v,
+                   int64_t v_tok_stride, int64_t v_head_stride, void* stream);
+int frc_attention_decode_q4_workspace(int batch, int nh, int nkv, int hd, size_t* bytes);
+int frc_attention_decode_q4(int type, const void* q, int64_t q_seq_stride, int64_t q_head_stride, const void* cache,
+                            int64_t pages, int page_size, const int* block_table, int64_t table_stride, int max_pages,
+                            const int* lengths, int batch, int nh, int nkv, int hd, float scale, void* workspace,
+                            size_t workspace_bytes, void* out, int64_t out_seq_stride, int64_t out_head_stride,
+                            void* stream);
+int frc_attention_prefill(int type, const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k,
+                          int64_t k_tok_stride, int64_t k_head_stride, const void* v, int64_t v_tok_stride,
+                          int64_t v_head_stride, const int* cu_q, const int* cu_k, int batch, int64_t tokens_q,
+                          int64_t tokens_k, int nh, int nkv, int hd, float scale, int causal, void* out,
+                          int64_t out_tok_stride, int64_t out_head_stride, void* stream);
+
 /* ---- row-sharded projections: all-gather fused into the GEMV ----------- *
  * No reference counterpart: the reference runs on one CPU.  One process per
  * GPU; rank r owns a contiguous row range of every projection and computes
