@@ -6,12 +6,61 @@
 // query head h reading KV head h / (nh / nkv).  A page number outside the
 // cache hides the page's tokens, and a sequence of no (visible) tokens gives
 // zeros, so no table can lead a read out of the cache.
+//
+// Bound: a token and KV head is 5/4 HD bytes, read once for all its query
+// heads, so HBM, if a value costs few instructions.  The products are
+// therefore formed on the stored nibbles, and the scales are applied to sums:
+//
+//   s_t = sum_j d_tj (sum_{c in j} q_c n_tc) + sum_j m_tj (sum_{c in j} q_c)
+//   o_c = sum_t (p_t d_tj) n_tc + sum_t p_t m_tj           (j the group of c)
+//
+// Two nibbles become two fp16 operands with two instructions: bits 0..3 under
+// the exponent of 1024 are 1024 + n, bits 4..7 are 1024 + 16 n, and one add or
+// fused multiply-add leaves n (or n - 8), exact.  (Without the exponent the
+// bits are subnormals, exact too and an instruction less, but the tensor
+// cores align the sum to the operands' exponents, not to their leading bits,
+// which costs its last ten bits: fp32 results were off by 4e-5.)
+//
+//  * q . n: m16n8k16 with the query heads as rows (up to eight; the other eight
+//    rows hold the low parts of fp32 queries), eight tokens as columns, channels as
+//    the contraction, one accumulator a group; times d in fp32.  The queries
+//    are scaled by a power of two to 2^14, so that fp16 holds them exactly for
+//    16-bit types, and as a sum of two for fp32 (22 bits).
+//  * m q: one more product, offsets (fp16 as stored) by the groups' query sums
+//    as two fp16 each.
+//  * p n: 16 channels of one group as rows, the heads as columns, 16 tokens as
+//    the contraction; p d is the fp16 operand, in two parts for fp32, rounded
+//    once for fp16 (by 2^-11) and twice for bf16 (p and p d, an eighth of the
+//    type's own rounding each).  The fragment of p is the one that the first
+//    product leaves in the same lanes.
+//  * p m: one more product, offsets as rows.
+//    Here n - 8 and m + 8 d take the places of n and m: the sums then are as
+//    large as the result, where sum p d n grows with the tokens and cancels
+//    with sum p m (fp32: 2e-6 off at 4097 tokens), and roundings of p d count
+//    relative to a value's distance from its group's middle.  m + 8 d is in two
+//    parts for fp32, rounded to fp16 for 16-bit types as the stored m is.
+//
+// The softmax's reference is not the largest s but the largest s + log2 d (d
+// the token's largest V step, at least 2^-10): so p d stays within one power of
+// two of 1 whatever the size of the values, and p below 2^10.
+//
+// Split: all sequences' blocks of 16 tokens, for each KV head (and part of
+// eight query heads: a unit), form one line, with one empty place before each
+// unit for the work of opening and closing it.  The line is cut into equal
+// ranges, one a warp, 16 warps an SM: lengths need not be known to the host and
+// may differ at will.  A warp streams its blocks through its own ring of shared
+// memory (one bulk copy a block: it is contiguous; the page numbers of 32
+// blocks are looked up at once, one a lane, a batch ahead) and writes the
+// units that lie wholly in its range.  A unit that a boundary cuts is joined from its
+// pieces, by the CTA where the CTA has all of them, otherwise from pieces that
+// the CTAs leave in the workspace, by a second kernel.
 #include <cuda_runtime.h>
 
-#include <cfloat>
+#include <atomic>
 #include <cstdio>
 
 #include "../../include/frcuda.h"
+#include "gemv.cuh"
 #include "kv_q4.cuh"
 
 namespace frc {
@@ -27,62 +76,699 @@ struct AttnQ4Params {
   int max_pages;  // entries of a table row
   const int* lengths;
   int batch, nh, nkv;
+  int parts;  // parts of up to eight query heads of a KV head
   float scale;
   void* out;
   int64_t o_seq, o_head;
+  int q_vec, o_vec;  // rows allow vector loads / stores
+  float* part;       // workspace: [2 grid][8][HD + 4] partial (max, sum, -, -, o)
+  int4* desc;        // workspace: [grid] (sequence, unit, CTAs that follow, -), a head cut at the CTA's end
+  uint32_t* status;
+  uint32_t bias;  // 0x64006400, the halves 1024: a parameter, so that it stays in a register
 };
 
-// One warp for each (sequence, query head): a lane holds HD / 32 channels,
-// and the tokens follow one another with a running maximum and sum.
-template <typename T, int HD>
-__global__ void __launch_bounds__(32) attn_q4_kernel(AttnQ4Params p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" :::);
-  constexpr Q4Layout lay(HD);
-  constexpr int C = HD / 32;
-  const int b = blockIdx.y, h = blockIdx.x, g = h / (p.nh / p.nkv), lane = threadIdx.x;
-  const T* qp = static_cast<const T*>(p.q) + b * p.q_seq + h * p.q_head;
-  float qv[C], acc[C];
-#pragma unroll
-  for (int e = 0; e < C; ++e) {
-    qv[e] = to_f32(qp[C * lane + e]) * p.scale;
-    acc[e] = 0.f;
+constexpr int kAqWarps = 8;
+constexpr int kAqThreads = kAqWarps * 32;
+constexpr int kAqHeads = 8;                       // query heads a unit
+constexpr int kAqGrid = 2 * 148;
+constexpr int kAqMinPlaces = kAqWarps;            // places a CTA, at least: one for each warp
+
+template <int HD>
+struct AqSmem {
+  static constexpr int kStages = HD == 128 ? 3 : 6;  // blocks in flight for each warp
+  static constexpr int kBlock = 20 * HD;
+  static constexpr int kRow = HD + 4;  // floats of a head in a piece
+  static constexpr int kPieces = 2 * kAqWarps;  // of each warp: the unit that ends in its range, the one that goes on
+  alignas(128) uint8_t ring[kAqWarps][kStages][kBlock];
+  alignas(16) float o[kAqWarps][kAqHeads][kRow];
+  float m[kPieces][kAqHeads], l[kPieces][kAqHeads];
+  int4 piece[kPieces];  // (sequence or -1, unit, start, end) in places of the CTA's range
+  uint64_t full[kAqWarps][kStages];
+  int64_t scan[kAqWarps];
+  int64_t first_start;  // place of sequence first_seq in the line
+  int first_seq;
+  int abort;
+  // a warp's last piece lies in its ring, which is free by then
+  FRC_DEVICE_INLINE float* rows(int k) {
+    return k & 1 ? reinterpret_cast<float*>(ring[k >> 1]) : &o[k >> 1][0][0];
   }
-  const int per_page = p.blocks_per_page * kQ4Tokens;
-  const int64_t room = static_cast<int64_t>(p.max_pages) * per_page;
-  const int len = static_cast<int>(p.lengths[b] < room ? p.lengths[b] : room);
-  float mx = -INFINITY, sum = 0.f;
-  for (int t = 0; t < len; ++t) {
-    const int page = p.table[b * p.table_stride + t / per_page];
-    if (page < 0 || page >= p.pages) continue;
-    const uint8_t* blk = p.cache + ((static_cast<int64_t>(page) * p.nkv + g) * p.blocks_per_page +
-                                    t % per_page / kQ4Tokens) * lay.block_bytes();
-    const int u = t % kQ4Tokens;
-    float s = 0.f, v[C];
-#pragma unroll
-    for (int e = 0; e < C; ++e) {
-      const int c = C * lane + e, j = c / 32, w = c / 8;
-      const uint32_t kw = *reinterpret_cast<const uint32_t*>(blk + lay.k_word(u, w & 3, j));
-      const uint32_t vw = *reinterpret_cast<const uint32_t*>(blk + lay.v_word(w, u));
-      const float k = fmaf(static_cast<float>((kw >> (4 * (c & 7))) & 15u),
-                           __half2float(*reinterpret_cast<const __half*>(blk + lay.k_step(j, u))),
-                           __half2float(*reinterpret_cast<const __half*>(blk + lay.k_offset(u, j))));
-      v[e] = fmaf(static_cast<float>((vw >> (4 * (c & 7))) & 15u),
-                  __half2float(*reinterpret_cast<const __half*>(blk + lay.v_step(j, u))),
-                  __half2float(*reinterpret_cast<const __half*>(blk + lay.v_offset(j, u))));
-      s = fmaf(qv[e], k, s);
+  static_assert(kAqHeads * kRow * 4 <= kStages * kBlock, "a piece fits the ring");
+};
+
+FRC_DEVICE_INLINE float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+FRC_DEVICE_INLINE float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+FRC_DEVICE_INLINE void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same into a fresh accumulator.
+FRC_DEVICE_INLINE void mma16816_new(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+FRC_DEVICE_INLINE uint32_t h2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+FRC_DEVICE_INLINE __half2 bits_h2(uint32_t b) { return *reinterpret_cast<const __half2*>(&b); }
+FRC_DEVICE_INLINE uint32_t pack_half2(float lo, float hi) { return h2_bits(__floats2half2_rn(lo, hi)); }
+
+// (w & MASK) | bias in one instruction: the mask is its one constant, the
+// exponents of 1024 a register.
+template <uint32_t MASK>
+FRC_DEVICE_INLINE uint32_t and_or(uint32_t w, uint32_t bias) {
+  uint32_t v;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w), "n"(MASK), "r"(bias));
+  return v;
+}
+
+// Nibbles 0 and 4 (LOW) or 1 and 5 of a word as the halves n - B.
+template <bool LOW, int B>
+FRC_DEVICE_INLINE uint32_t nibbles(uint32_t w, uint32_t bias) {
+  if constexpr (LOW)
+    return h2_bits(__hadd2(bits_h2(and_or<0x000f000fu>(w, bias)), __float2half2_rn(-1024.f - B)));
+  else
+    return h2_bits(__hfma2(bits_h2(and_or<0x00f000f0u>(w, bias)), __float2half2_rn(0.0625f),
+                           __float2half2_rn(-64.f - B)));
+}
+
+// 16-token blocks of a sequence.
+FRC_DEVICE_INLINE int aq_length(const AttnQ4Params& p, int b) {
+  const int64_t room = static_cast<int64_t>(p.max_pages) * p.blocks_per_page * kQ4Tokens;
+  const int n = p.lengths[b];
+  return n < 0 ? 0 : (n < room ? n : static_cast<int>(room));
+}
+FRC_DEVICE_INLINE int aq_blocks(int length) { return static_cast<int>((static_cast<int64_t>(length) + 15) >> 4); }
+
+// Walks the line: the unit that holds a place.  Places count from the start
+// of the CTA's range (a unit may start before it).
+struct AqWalk {
+  int seq, unit, len, nb;  // tokens and blocks of the sequence
+  int u0;                  // place of the unit, which has nb + 1
+  FRC_DEVICE_INLINE void sequence(const AttnQ4Params& p, int s) {
+    seq = s;
+    len = aq_length(p, s);
+    nb = aq_blocks(len);
+  }
+  FRC_DEVICE_INLINE int end() const { return u0 + nb + 1; }
+  FRC_DEVICE_INLINE void to(const AttnQ4Params& p, int place, int units) {
+    while (place >= end()) {
+      u0 = end();
+      if (++unit == units) {
+        unit = 0;
+        sequence(p, seq + 1);
+      }
     }
-    s = warp_sum(s);
-    const float m_new = fmaxf(mx, s), keep = mx == m_new ? 1.f : expf(mx - m_new), w = expf(s - m_new);
-    mx = m_new;
-    sum = fmaf(sum, keep, w);
-#pragma unroll
-    for (int e = 0; e < C; ++e) acc[e] = fmaf(acc[e], keep, w * v[e]);
   }
-  T* op = static_cast<T*>(p.out) + b * p.o_seq + h * p.o_head;
-  const float inv = mx == -INFINITY ? 0.f : 1.f / sum;
+};
+
+// One warp's running state for a unit: O^T fragments, offsets' sums, and the
+// softmax reference and sum of head lane / 4.
+template <int HD, typename T>
+struct AqWarp {
+  static constexpr int NG = HD / kQ4Group;
+  static constexpr bool SPLIT = sizeof(T) == 4;  // operands in two parts
+  static constexpr bool TWICE = std::is_same<T, __nv_bfloat16>::value;  // p rounded to 11 bits before p d is
+  static constexpr float kUp = TWICE ? 1.f : 512.f;  // what the operand p d is scaled by, beside 32
+  uint32_t a[NG][2][4];  // query fragments: (group, k step): rows 0-7 of both k halves, rows 8-15 (low parts) of both
+  uint32_t am;                       // groups' query sums
+  float f_n, f_m;                    // scale of the two score products, with log2 e
+  float o[NG][2][4], om[4];
+  float m_run, base, l_run;  // the reference, what is taken off the scores (five less: p times 32), the sum
+
+  // q of head lane / 4: this lane holds channels 32 j + 8 (lane & 3) .. + 7.
+  FRC_DEVICE_INLINE void load_q(const float (&x)[NG][8], float scale, int lane) {
+    float mx = 0.f;
 #pragma unroll
-  for (int e = 0; e < C; ++e) from_f32(acc[e] * inv, op[C * lane + e]);
+    for (int j = 0; j < NG; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[j][i]));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    // 2^(14 - exponent): the largest becomes 2^14 .. 2^15
+    const int e = max(static_cast<int>(__float_as_uint(mx) >> 23) - 127, -100);
+    const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23);
+    const float down = __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
+    f_n = scale * 1.44269504088896341f * down;
+    f_m = scale * 1.44269504088896341f * down * 64.f;
+    float sum[NG];
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      float y[8], lo[8];
+      sum[j] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        y[i] = x[j][i] * up;
+        sum[j] += y[i];
+        const float h = __half2float(__float2half_rn(y[i]));
+        lo[i] = (y[i] - h) * 2048.f;
+        y[i] = h;
+      }
+      sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
+      sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
+      sum[j] *= 1.f / 64.f;
+      // nibble i of a word: k step i / 2 % 2, k half i % 2, low or high half i / 4
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        a[j][s][0] = pack_half2(y[2 * s], y[2 * s + 4]);
+        a[j][s][1] = pack_half2(y[2 * s + 1], y[2 * s + 5]);
+        a[j][s][2] = pack_half2(lo[2 * s], lo[2 * s + 4]);  // zeros for 16-bit types
+        a[j][s][3] = pack_half2(lo[2 * s + 1], lo[2 * s + 5]);
+      }
+    }
+    // contraction index 2 q, 2 q + 1: the sums of two groups, high parts first, then low parts
+    const int q = lane & 3, pair = q % (NG / 2), part = q / (NG / 2);
+    float s0 = sum[0], s1 = sum[1];
+    if constexpr (NG == 4)
+      if (pair) {
+        s0 = sum[2];
+        s1 = sum[3];
+      }
+    const float h0 = __half2float(__float2half_rn(s0)), h1 = __half2float(__float2half_rn(s1));
+    am = part == 0 ? pack_half2(h0, h1) : (part == 1 ? pack_half2(s0 - h0, s1 - h1) : 0u);
+  }
+
+  FRC_DEVICE_INLINE void reset() {
+#pragma unroll
+    for (int j = 0; j < NG; ++j)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[j][s][i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) om[i] = 0.f;
+    m_run = -INFINITY;
+    base = 0.f;
+    l_run = 0.f;
+  }
+
+  // One block in shared memory; `left` tokens of it (at least one) belong to
+  // the sequence.  Lane (r, q) = (lane / 4, lane % 4) has tokens 4 q .. 4 q + 3.
+  FRC_DEVICE_INLINE void block(const uint8_t* blk, int left, int lane, uint32_t bias) {
+    constexpr Q4Layout lay(HD);
+    const int r = lane >> 2, q = lane & 3;
+    float s[4];
+    uint2 kd[NG];
+#pragma unroll
+    for (int j = 0; j < NG; ++j) kd[j] = *reinterpret_cast<const uint2*>(blk + lay.k_step(j, 4 * q));
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {  // two tiles of eight tokens: column n is token 4 (n / 2) + 2 t + n % 2
+      const int tok = 4 * (r >> 1) + 2 * t + (r & 1);
+      uint32_t w[NG];
+      if constexpr (NG == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(blk + lay.k_word(tok, q, 0));
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+      } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(blk + lay.k_word(tok, q, 0));
+        w[0] = v.x; w[1] = v.y;
+      }
+      float cm[4], x0 = 0.f, x1 = 0.f;
+      mma16816_new(cm, am, 0u, 0u, 0u, *reinterpret_cast<const uint32_t*>(blk + lay.k_offset(tok, 2 * (q % (NG / 2)))),
+                   0u);
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        float c[4];
+        const uint32_t hi = w[j] >> 8;
+        mma16816_new(c, a[j][0][0], a[j][0][2], a[j][0][1], a[j][0][3], nibbles<true, 0>(w[j], bias),
+                     nibbles<false, 0>(w[j], bias));
+        mma16816(c, a[j][1][0], a[j][1][2], a[j][1][1], a[j][1][3], nibbles<true, 0>(hi, bias),
+                 nibbles<false, 0>(hi, bias));
+        if constexpr (SPLIT) {
+          c[0] = fmaf(c[2], 1.f / 2048.f, c[0]);
+          c[1] = fmaf(c[3], 1.f / 2048.f, c[1]);
+        }
+        const float2 d = __half22float2(bits_h2(t ? kd[j].y : kd[j].x));
+        x0 = j ? fmaf(d.x, c[0], x0) : d.x * c[0];
+        x1 = j ? fmaf(d.y, c[1], x1) : d.y * c[1];
+      }
+      s[2 * t] = fmaf(x0, f_n, cm[0] * f_m);
+      s[2 * t + 1] = fmaf(x1, f_n, cm[1] * f_m);
+    }
+    uint2 vd[NG], vm = make_uint2(0u, 0u), vml = make_uint2(0u, 0u);
+#pragma unroll
+    for (int j = 0; j < NG; ++j) vd[j] = *reinterpret_cast<const uint2*>(blk + lay.v_step(j, 4 * q));
+    if (r < NG) {  // offsets m + 8 d of n - 8, in two parts for fp32
+      vm = *reinterpret_cast<const uint2*>(blk + lay.v_offset(r, 4 * q));
+      const uint2 d = *reinterpret_cast<const uint2*>(blk + lay.v_step(r, 4 * q));
+      if constexpr (SPLIT) {
+        offset_parts(d.x, vm.x, vml.x);
+        offset_parts(d.y, vm.y, vml.y);
+      } else {
+        vm.x = h2_bits(__hfma2(bits_h2(d.x), __float2half2_rn(8.f), bits_h2(vm.x)));
+        vm.y = h2_bits(__hfma2(bits_h2(d.y), __float2half2_rn(8.f), bits_h2(vm.y)));
+      }
+    }
+    if (left < kQ4Tokens) {  // what lies behind the last token may be anything, NaN among it
+      const int mine = left - 4 * q;
+      const uint32_t k0 = mine >= 2 ? 0xffffffffu : (mine == 1 ? 0xffffu : 0u);
+      const uint32_t k1 = mine >= 4 ? 0xffffffffu : (mine == 3 ? 0xffffu : 0u);
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        vd[j].x &= k0;
+        vd[j].y &= k1;
+      }
+      vm.x &= k0;
+      vm.y &= k1;
+      vml.x &= k0;
+      vml.y &= k1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i >= mine) s[i] = -INFINITY;
+    }
+    // reference: the largest s + log2 of the largest V step of the lane's four
+    // tokens, taken apart: no less than the largest s + log2 d
+    __half2 dx = __hmax2(bits_h2(vd[0].x), bits_h2(vd[0].y));
+#pragma unroll
+    for (int j = 1; j < NG; ++j) dx = __hmax2(dx, __hmax2(bits_h2(vd[j].x), bits_h2(vd[j].y)));
+    const float dm = fmaxf(__half2float(__hmax(__low2half(dx), __high2half(dx))), 1.f / 1024.f);
+    float m = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])) + lg2(dm);
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    if (__any_sync(0xffffffffu, m > m_run)) {
+      const float m_new = fmaxf(m, m_run);
+      const float keep = m_new == -INFINITY ? 1.f : ex2(m_run - m_new);
+      const float f0 = __shfl_sync(0xffffffffu, keep, 8 * q), f1 = __shfl_sync(0xffffffffu, keep, 8 * q + 4);
+#pragma unroll
+      for (int j = 0; j < NG; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          o[j][t][0] *= f0;
+          o[j][t][1] *= f1;
+          o[j][t][2] *= f0;
+          o[j][t][3] *= f1;
+        }
+      om[0] *= f0;
+      om[1] *= f1;
+      l_run *= keep;
+      m_run = m_new;
+      base = m_new == -INFINITY ? 0.f : m_new - 5.f;
+    }
+    const float p0 = ex2(s[0] - base), p1 = ex2(s[1] - base), p2 = ex2(s[2] - base), p3 = ex2(s[3] - base);
+    l_run += (p0 + p1) + (p2 + p3);
+    const uint32_t h01 = pack_half2(p0, p1), h23 = pack_half2(p2, p3);
+    mma16816(om, vm.x, 0u, vm.y, 0u, h01, h23);
+    if constexpr (SPLIT) {
+      const float2 g01 = __half22float2(bits_h2(h01)), g23 = __half22float2(bits_h2(h23));
+      mma16816(om, vm.x, 0u, vm.y, 0u, pack_half2(p0 - g01.x, p1 - g01.y), pack_half2(p2 - g23.x, p3 - g23.y));
+      mma16816(om, vml.x, 0u, vml.y, 0u, h01, h23);
+    }
+    // rows of a tile: 16 channels of group j: word 4 j + r % 4, of it the nibbles
+    // of its low half (r < 4) or high half: 2 t in row r, 2 t + 1 in row r + 8
+    const uint32_t sel = r < 4 ? 0x5410u : 0x7632u;
+    const float r0 = p0 * kUp, r1 = p1 * kUp, r2 = p2 * kUp, r3 = p3 * kUp;
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      const uint4 v = *reinterpret_cast<const uint4*>(blk + lay.v_word(4 * j + (r & 3), 4 * q));
+      const uint32_t w0 = __byte_perm(v.x, v.y, sel), w1 = __byte_perm(v.z, v.w, sel);
+      uint32_t b0, b1, c0 = 0u, c1 = 0u;
+      if constexpr (TWICE) {
+        b0 = h2_bits(__hmul2(bits_h2(h01), bits_h2(vd[j].x)));
+        b1 = h2_bits(__hmul2(bits_h2(h23), bits_h2(vd[j].y)));
+      } else {
+        const float2 e0 = __half22float2(bits_h2(vd[j].x)), e1 = __half22float2(bits_h2(vd[j].y));
+        const float y0 = r0 * e0.x, y1 = r1 * e0.y, y2 = r2 * e1.x, y3 = r3 * e1.y;
+        b0 = pack_half2(y0, y1);
+        b1 = pack_half2(y2, y3);
+        if constexpr (SPLIT) {
+          const float2 g0 = __half22float2(bits_h2(b0)), g1 = __half22float2(bits_h2(b1));
+          c0 = pack_half2(y0 - g0.x, y1 - g0.y);
+          c1 = pack_half2(y2 - g1.x, y3 - g1.y);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint32_t u0 = t ? w0 >> 8 : w0, u1 = t ? w1 >> 8 : w1;
+        const uint32_t n0 = nibbles<true, 8>(u0, bias), n1 = nibbles<false, 8>(u0, bias);
+        const uint32_t n2 = nibbles<true, 8>(u1, bias), n3 = nibbles<false, 8>(u1, bias);
+        mma16816(o[j][t], n0, n1, n2, n3, b0, b1);
+        if constexpr (SPLIT) mma16816(o[j][t], n0, n1, n2, n3, c0, c1);
+      }
+    }
+  }
+
+  // Two tokens' m + 8 d as the sum of two halves each: m becomes the high part.
+  static FRC_DEVICE_INLINE void offset_parts(uint32_t d, uint32_t& m, uint32_t& low) {
+    const float2 df = __half22float2(bits_h2(d)), mf = __half22float2(bits_h2(m));
+    const float x = fmaf(df.x, 8.f, mf.x), y = fmaf(df.y, 8.f, mf.y);
+    m = pack_half2(x, y);
+    const float2 h = __half22float2(bits_h2(m));
+    low = pack_half2(x - h.x, y - h.y);
+  }
+
+  // The warp's sums: f(head, channel, o[4]) for this lane's channels of its two
+  // heads, after l of head lane / 4 has been summed over its tokens.
+  template <typename F>
+  FRC_DEVICE_INLINE void sums(int lane, F&& f) {
+    const int r = lane >> 2, q = lane & 3;
+    l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
+    l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
+    constexpr float kStep = 1.f / kUp;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float l = __shfl_sync(0xffffffffu, l_run, 4 * (2 * q + e));
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        const float m = __shfl_sync(0xffffffffu, om[e], 4 * j + q);
+        const float v[4] = {fmaf(o[j][0][e], kStep, m), fmaf(o[j][0][2 + e], kStep, m), fmaf(o[j][1][e], kStep, m),
+                            fmaf(o[j][1][2 + e], kStep, m)};
+        f(2 * q + e, kQ4Group * j + 8 * (r & 3) + 4 * (r >> 2), v, l);
+      }
+    }
+  }
+};
+
+// The eight query heads of a unit.
+struct AqHeads {
+  int first, count;
+  FRC_DEVICE_INLINE AqHeads(const AttnQ4Params& p, int unit) {
+    const int group = p.nh / p.nkv, kvh = unit / p.parts;
+    first = kvh * group + (unit - kvh * p.parts) * kAqHeads;
+    count = min(kAqHeads, (kvh + 1) * group - first);
+  }
+};
+
+template <int N, typename T>
+FRC_DEVICE_INLINE void aq_store(const AttnQ4Params& p, int seq, int head, int c, float (&v)[N], float l) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] *= inv;
+  T* op = static_cast<T*>(p.out) + seq * p.o_seq + head * p.o_head + c;
+  if (p.o_vec) store_run<N, true>(op, v);
+  else store_run<N, false>(op, v);
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kAqThreads, 2) attn_q4_kernel(const AttnQ4Params p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  using SM = AqSmem<HD>;
+  constexpr int NS = SM::kStages, NG = HD / kQ4Group;
+  extern __shared__ __align__(128) uint8_t aq_smem[];
+  SM* sh = reinterpret_cast<SM*>(aq_smem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int units = p.nkv * p.parts;
+
+  // ---- the line and this CTA's range of it ----------------------------------------
+  const int per_thread = (p.batch + kAqThreads - 1) / kAqThreads;
+  const int s0 = min(tid * per_thread, p.batch), s1 = min(s0 + per_thread, p.batch);
+  int64_t mine = 0;
+  for (int b = s0; b < s1; ++b) mine += aq_blocks(aq_length(p, b)) + 1;
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) sh->scan[warp] = incl;
+  if (lane == 0) {
+    for (int s = 0; s < NS; ++s) mbar_init(&sh->full[warp][s], 1);
+    if (warp == 0) sh->abort = 0;
+    fence_barrier_init();
+  }
+  if (tid < SM::kPieces) sh->piece[tid] = make_int4(-1, 0, 0, 0);
+  __syncthreads();
+  int64_t total = 0, before = incl - mine;
+#pragma unroll
+  for (int w = 0; w < kAqWarps; ++w) {
+    if (w < warp) before += sh->scan[w];
+    total += sh->scan[w];
+  }
+  total *= units;
+  before *= units;
+  int64_t per = (total + gridDim.x - 1) / gridDim.x;
+  per = per > kAqMinPlaces ? per : kAqMinPlaces;
+  const int64_t c0 = min(static_cast<int64_t>(blockIdx.x) * per, total), c1 = min(c0 + per, total);
+  if (c0 >= before && c0 < before + mine * units) {  // one thread, unless the range is empty
+    int s = s0;
+    for (int64_t next; (next = before + static_cast<int64_t>(aq_blocks(aq_length(p, s)) + 1) * units) <= c0; ++s)
+      before = next;
+    sh->first_seq = s;
+    sh->first_start = before;
+  }
+  if (tid == 0) p.desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  __syncthreads();
+  if (c0 >= c1) return;
+  const int count = static_cast<int>(c1 - c0);  // below 2^30: checked by the host
+  volatile int* abort = &sh->abort;
+
+  // ---- this warp's range [w0, w1) of it ------------------------------------------------
+  const int share = (count + kAqWarps - 1) / kAqWarps;
+  const int w0 = min(warp * share, count), w1 = min(w0 + share, count);
+  if (w0 < w1) {
+    AqWalk walk;
+    {
+      int64_t start = sh->first_start;
+      walk.sequence(p, sh->first_seq);
+      while (c0 + w0 >= start + static_cast<int64_t>(walk.nb + 1) * units) {
+        start += static_cast<int64_t>(walk.nb + 1) * units;
+        walk.sequence(p, walk.seq + 1);
+      }
+      walk.unit = static_cast<int>((c0 + w0 - start) / (walk.nb + 1));
+      walk.u0 = static_cast<int>(start + static_cast<int64_t>(walk.unit) * (walk.nb + 1) - c0);
+    }
+    int page = -1, at = 0, page_next = -1, at_next = 0;  // of place lane of this batch of 32, and of the next
+    auto look_up = [&](int place) {  // the page number of a place's block, and the block's place in the page
+      page_next = -1;
+      if (place < w1) {
+        AqWalk w = walk;
+        w.to(p, place, units);
+        const int blk = place - w.u0 - 1;
+        if (blk >= 0) {
+          const int entry = blk / p.blocks_per_page;
+          at_next = w.unit / p.parts * p.blocks_per_page + (blk - entry * p.blocks_per_page);
+          page_next = p.table[w.seq * p.table_stride + entry];
+        }
+      }
+    };
+    uint32_t seen = 0;  // bit s: stage s holds a block (of a page inside the cache)
+    int issued = 0;
+    auto issue = [&](int s) {  // copies the next place's block, if there is one, into the stage that is free
+      if (w0 + issued >= w1) return;
+      if ((issued & 31) == 0) {
+        page = page_next;
+        at = at_next;
+        look_up(w0 + issued + 32 + lane);
+      }
+      const int pg = __shfl_sync(0xffffffffu, page, issued & 31), in_page = __shfl_sync(0xffffffffu, at, issued & 31);
+      const bool ok = pg >= 0 && pg < p.pages;
+      seen = (seen & ~(1u << s)) | (ok ? 1u << s : 0u);
+      if (lane == 0) {
+        if (ok) {
+          mbar_arrive_expect_tx(&sh->full[warp][s], SM::kBlock);
+          bulk_g2s(sh->ring[warp][s],
+                   p.cache + (static_cast<int64_t>(pg) * p.nkv * p.blocks_per_page + in_page) * SM::kBlock,
+                   SM::kBlock, &sh->full[warp][s]);
+        } else {
+          mbar_arrive(&sh->full[warp][s]);
+        }
+      }
+      ++issued;
+    };
+    look_up(w0 + lane);
+    for (int s = 0; s < NS; ++s) issue(s);
+    int s = 0;  // the stage of `place`, and the parity of its use
+    uint32_t parity = 0;
+
+    AqWarp<HD, T> st;
+    for (int place = w0; place < w1;) {
+      walk.to(p, place, units);
+      const AqHeads heads(p, walk.unit);
+      const int end = min(walk.end(), w1);
+      {
+        float x[NG][8];
+        const T* qp = static_cast<const T*>(p.q) + walk.seq * p.q_seq + (heads.first + (lane >> 2)) * p.q_head +
+                      8 * (lane & 3);
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[j][e] = 0.f;
+          if ((lane >> 2) < heads.count) {
+            if (p.q_vec) load_run<8, true>(qp + kQ4Group * j, x[j]);
+            else load_run<8, false>(qp + kQ4Group * j, x[j]);
+          }
+        }
+        st.load_q(x, p.scale, lane);
+      }
+      st.reset();
+      for (; place < end; ++place) {
+        const bool there = __all_sync(0xffffffffu, wait_phase(&sh->full[warp][s], parity, abort));
+        if (!there && lane == 0) atomicOr(p.status, kStatusFullWaitTimeout);
+        if (there && (seen >> s & 1u))
+          st.block(sh->ring[warp][s], min(kQ4Tokens, walk.len - (place - walk.u0 - 1) * kQ4Tokens), lane, p.bias);
+        __syncwarp();
+        if (there) issue(s);
+        if (++s == NS) {
+          s = 0;
+          parity ^= 1u;
+        }
+      }
+      if (walk.u0 >= w0 && walk.end() <= w1) {
+        st.sums(lane, [&](int h, int c, const float (&v)[4], float l) {
+          float o[4] = {v[0], v[1], v[2], v[3]};
+          if (h < heads.count) aq_store<4, T>(p, walk.seq, heads.first + h, c, o, l);
+        });
+      } else {
+        const int k = 2 * warp + (end == w1 ? 1 : 0);
+        if (end == w1 && *abort)  // after a wait that ran out: no copy may still be landing in the ring
+          for (int j = issued > NS ? issued - NS : 0; j < issued; ++j) {
+            int zero = 0;
+            if (!wait_phase(&sh->full[warp][j % NS], (j / NS) & 1, &zero)) atomicOr(p.status, kStatusDrainTimeout);
+          }
+        float* rows = sh->rows(k);
+        st.sums(lane, [&](int h, int c, const float (&v)[4], float) {
+          *reinterpret_cast<float4*>(rows + h * SM::kRow + c) = make_float4(v[0], v[1], v[2], v[3]);
+        });
+        if ((lane & 3) == 0) {
+          sh->m[k][lane >> 2] = st.m_run;
+          sh->l[k][lane >> 2] = st.l_run;
+        }
+        if (lane == 0) sh->piece[k] = make_int4(walk.seq, walk.unit, walk.u0, walk.end());
+      }
+    }
+    if (*abort)
+      for (int j = issued > NS ? issued - NS : 0; j < issued; ++j) {
+        int zero = 0;
+        if (!wait_phase(&sh->full[warp][j % NS], (j / NS) & 1, &zero)) atomicOr(p.status, kStatusDrainTimeout);
+      }
+  }
+  __syncthreads();
+  // ---- the pieces, in order: warp h joins head h of each cut unit ------------------------
+  for (int k = 0; k < SM::kPieces;) {
+    const int4 pc = sh->piece[k];
+    if (pc.x < 0) {
+      ++k;
+      continue;
+    }
+    int k1 = k + 1;  // pieces of one unit follow one another, with gaps
+    while (k1 < SM::kPieces && (sh->piece[k1].x < 0 || sh->piece[k1].z == pc.z)) ++k1;
+    const AqHeads heads(p, pc.y);
+    const bool whole = pc.z >= 0 && pc.w <= count;
+    if (warp < heads.count) {
+      constexpr int C = HD / 32;
+      float M = -INFINITY;
+      for (int j = k; j < k1; ++j)
+        if (sh->piece[j].x >= 0) M = fmaxf(M, sh->m[j][warp]);
+      const float base = M == -INFINITY ? 0.f : M;
+      float L = 0.f, acc[C];
+#pragma unroll
+      for (int e = 0; e < C; ++e) acc[e] = 0.f;
+      for (int j = k; j < k1; ++j) {
+        if (sh->piece[j].x < 0) continue;
+        const float f = ex2(sh->m[j][warp] - base);
+        L = fmaf(sh->l[j][warp], f, L);
+        float v[C];
+        load_run<C, true>(sh->rows(j) + warp * SM::kRow + C * lane, v);
+#pragma unroll
+        for (int e = 0; e < C; ++e) acc[e] = fmaf(v[e], f, acc[e]);
+      }
+      if (whole) {
+        aq_store<C, T>(p, pc.x, heads.first + warp, C * lane, acc, L);
+      } else {
+        float* row = p.part + ((2 * static_cast<int64_t>(blockIdx.x) + (pc.z >= 0 ? 1 : 0)) * kAqHeads + warp) * SM::kRow;
+        if (lane == 0) {
+          row[0] = M;
+          row[1] = L;
+        }
+        store_run<C, true>(row + 4 + C * lane, acc);
+      }
+    }
+    if (pc.z >= 0 && pc.w > count && tid == 0)  // goes on in the next CTAs
+      p.desc[blockIdx.x] = make_int4(pc.x, pc.y, static_cast<int>((c0 + pc.w - 1) / per - blockIdx.x), 0);
+    k = k1;
+  }
+}
+
+// Joins the pieces of a unit that the CTAs' ranges cut, in their order: block
+// (i, h) the head h of the unit that is cut at the end of CTA i's range.
+constexpr int kAqJoin = 256;
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kAqJoin) attn_q4_join_kernel(const AttnQ4Params p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  constexpr int ROW = AqSmem<HD>::kRow, L4 = HD / 4, G = kAqJoin / L4;  // lanes of four channels, G ranges at a time
+  const int4 d = p.desc[blockIdx.x];
+  if (d.x < 0) return;
+  const int h = blockIdx.y;
+  const AqHeads heads(p, d.y);
+  if (h >= heads.count) return;
+  const int np = d.z + 1, tid = threadIdx.x;
+  __shared__ float f[kAqGrid];
+  __shared__ float red[kAqJoin / 32];
+  __shared__ __align__(16) float acc[G][HD];
+  auto row = [&](int k) {  // the cut unit starts in CTA i (its second part) and goes on as the others' first
+    return p.part + (static_cast<int64_t>(k == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + k)) * kAqHeads + h) * ROW;
+  };
+  float M = -INFINITY;
+  for (int k = tid; k < np; k += kAqJoin) M = fmaxf(M, row(k)[0]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  if ((tid & 31) == 0) red[tid >> 5] = M;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kAqJoin / 32; ++w) M = fmaxf(M, red[w]);
+  const float base = M == -INFINITY ? 0.f : M;
+  for (int k = tid; k < np; k += kAqJoin) f[k] = ex2(row(k)[0] - base);
+  __syncthreads();
+  const int g = tid / L4, c = 4 * (tid % L4);
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  float L = 0.f;
+#pragma unroll 4
+  for (int k = g; k < np; k += G) {
+    const float4 v = *reinterpret_cast<const float4*>(row(k) + 4 + c);
+    L = fmaf(row(k)[1], f[k], L);
+    a.x = fmaf(v.x, f[k], a.x);
+    a.y = fmaf(v.y, f[k], a.y);
+    a.z = fmaf(v.z, f[k], a.z);
+    a.w = fmaf(v.w, f[k], a.w);
+  }
+  *reinterpret_cast<float4*>(&acc[g][c]) = a;
+  __shared__ float ls[G];
+  if (c == 0) ls[g] = L;
+  __syncthreads();
+  if (tid < L4) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+      sum += ls[k];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += acc[k][c + e];
+    }
+    aq_store<4, T>(p, d.x, heads.first + h, c, v, sum);
+  }
+}
+
+__device__ uint32_t g_serving_status;
+
+template <typename T, int HD>
+cudaError_t launch_attn_q4(AttnQ4Params p, int grid, cudaStream_t st) {
+  static std::atomic<uint64_t> ready{0};  // devices on which the kernel may use its shared memory
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !(ready.load() >> dev & 1)) {
+    e = cudaFuncSetAttribute(attn_q4_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(AqSmem<HD>));
+    if (e != cudaSuccess) return e;
+    if (dev < 64) ready.fetch_or(uint64_t(1) << dev);
+  }
+  e = launch_pdl(attn_q4_kernel<T, HD>, dim3(grid), dim3(kAqThreads), sizeof(AqSmem<HD>), st, p);
+  if (e != cudaSuccess || grid == 1) return e;
+  return launch_pdl(attn_q4_join_kernel<T, HD>, dim3(grid, min(kAqHeads, p.nh / p.nkv)), dim3(kAqJoin), 0, st, p);
 }
 
 }  // namespace frc
@@ -92,7 +778,8 @@ extern "C" {
 int frc_attention_decode_q4_workspace(int batch, int nh, int nkv, int hd, size_t* bytes) {
   FRC_REQUIRE(bytes && batch >= 0 && nh > 0 && nkv > 0 && nh % nkv == 0 && (hd == 64 || hd == 128),
               "frc_attention_decode_q4_workspace: bad arguments");
-  *bytes = 16;
+  // partial heads: two units a CTA; and a descriptor a CTA
+  *bytes = static_cast<size_t>(frc::kAqGrid) * (2 * frc::kAqHeads * (hd + 4) * sizeof(float) + sizeof(int4));
   return FRC_OK;
 }
 
@@ -122,13 +809,48 @@ int frc_attention_decode_q4(int type, const void* q, int64_t q_seq_stride, int64
   const int rc = frc_attention_decode_q4_workspace(batch, nh, nkv, hd, &need);
   if (rc) return rc;
   FRC_REQUIRE(workspace_bytes >= need, "frc_attention_decode_q4: workspace is too small");
-  const frc::AttnQ4Params p{q,       q_seq_stride, q_head_stride, static_cast<const uint8_t*>(cache), pages,
-                            page_size / frc::kQ4Tokens, block_table, table_stride, max_pages, lengths, batch, nh, nkv,
-                            scale,   out,          out_seq_stride, out_head_stride};
+  const int parts = (nh / nkv + frc::kAqHeads - 1) / frc::kAqHeads;
+  // no more CTAs than the tables could give places for
+  const int64_t blocks = static_cast<int64_t>(max_pages) * (page_size / frc::kQ4Tokens);
+  FRC_REQUIRE(blocks < (int64_t(1) << 31) && static_cast<int64_t>(nkv) * parts <= 65535,
+              "frc_attention_decode_q4: block table or heads too large");
+  const int64_t most = static_cast<int64_t>(batch) * nkv * parts * ((blocks < (1 << 27) ? blocks : (1 << 27)) + 1);
+  const int64_t want = (most + frc::kAqMinPlaces - 1) / frc::kAqMinPlaces;
+  const int grid = static_cast<int>(want < frc::kAqGrid ? want : frc::kAqGrid);
+  FRC_REQUIRE(most / grid < (int64_t(1) << 30), "frc_attention_decode_q4: block table too large");
+  const size_t es = type == FRC_F32 ? 4 : 2;
+  const int run = type == FRC_F32 ? 4 : 8;  // elements of a 16-byte load
+  void* status = nullptr;
+  FRC_LAUNCHED(cudaGetSymbolAddress(&status, frc::g_serving_status), "cudaGetSymbolAddress(status word)");
+  frc::AttnQ4Params p{};
+  p.q = q;
+  p.q_seq = q_seq_stride;
+  p.q_head = q_head_stride;
+  p.cache = static_cast<const uint8_t*>(cache);
+  p.pages = pages;
+  p.blocks_per_page = page_size / frc::kQ4Tokens;
+  p.table = block_table;
+  p.table_stride = table_stride;
+  p.max_pages = max_pages;
+  p.lengths = lengths;
+  p.batch = batch;
+  p.nh = nh;
+  p.nkv = nkv;
+  p.parts = parts;
+  p.scale = scale;
+  p.out = out;
+  p.o_seq = out_seq_stride;
+  p.o_head = out_head_stride;
+  p.q_vec = frc::aligned_to(q, 16) && q_seq_stride % run == 0 && q_head_stride % run == 0;
+  p.o_vec = frc::aligned_to(out, 4 * es) && out_seq_stride % 4 == 0 && out_head_stride % 4 == 0;
+  p.part = static_cast<float*>(workspace);
+  p.desc = reinterpret_cast<int4*>(p.part + static_cast<size_t>(frc::kAqGrid) * 2 * frc::kAqHeads * (hd + 4));
+  p.status = static_cast<uint32_t*>(status);
+  p.bias = 0x64006400u;
   return frc_with_type(type, [&](auto* z) -> int {
     using T = std::remove_pointer_t<decltype(z)>;
-    void (*fn)(frc::AttnQ4Params) = hd == 128 ? frc::attn_q4_kernel<T, 128> : frc::attn_q4_kernel<T, 64>;
-    FRC_LAUNCHED(frc::launch_pdl(fn, dim3(nh, batch), dim3(32), 0, static_cast<cudaStream_t>(stream), p),
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    FRC_LAUNCHED((hd == 128 ? frc::launch_attn_q4<T, 128>(p, grid, st) : frc::launch_attn_q4<T, 64>(p, grid, st)),
                  "attention_decode_q4 launch");
     return FRC_OK;
   });
