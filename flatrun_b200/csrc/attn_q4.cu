@@ -44,13 +44,13 @@
 // the token's largest V step, at least 2^-10): so p d stays within one power of
 // two of 1 whatever the size of the values, and p below 2^10.
 //
-// Split: all sequences' blocks of 16 tokens, for each KV head (and part of
-// eight query heads: a unit), form one line, with one empty place before each
-// unit for the work of opening and closing it.  The line is cut into equal
+// Split: all sequences' tokens, 32 (two blocks) a place, for each KV head (and
+// part of eight query heads: a unit), form one line, with one empty place before
+// each unit for the work of opening and closing it.  The line is cut into equal
 // ranges, one a warp, 16 warps an SM: lengths need not be known to the host and
 // may differ at will.  A warp streams its blocks through its own ring of shared
-// memory (one bulk copy a block: it is contiguous; the page numbers of 32
-// blocks are looked up at once, one a lane, a batch ahead) and writes the
+// memory (one bulk copy a block: it is contiguous; the page numbers of 16
+// places are looked up at once, a block a lane, a batch ahead) and writes the
 // units that lie wholly in its range.  A unit that a boundary cuts is joined from its
 // pieces, by the CTA where the CTA has all of them, otherwise from pieces that
 // the CTAs leave in the workspace, by a second kernel.
@@ -81,7 +81,8 @@ struct AttnQ4Params {
   void* out;
   int64_t o_seq, o_head;
   int q_vec, o_vec;  // rows allow vector loads / stores
-  float* part;       // workspace: [2 grid][8][HD + 4] partial (max, sum, -, -, o)
+  float* part;       // workspace: [2 grid][8][HD + 4] pieces that CTAs leave (max, sum, -, -, o)
+  float* first;      // workspace: [8 grid][8][HD + 4] warps' first pieces
   int4* desc;        // workspace: [grid] (sequence, unit, CTAs that follow, -), a head cut at the CTA's end
   uint32_t* status;
   uint32_t bias;  // 0x64006400, the halves 1024: a parameter, so that it stays in a register
@@ -95,12 +96,11 @@ constexpr int kAqMinPlaces = kAqWarps;            // places a CTA, at least: one
 
 template <int HD>
 struct AqSmem {
-  static constexpr int kStages = HD == 128 ? 3 : 6;  // blocks in flight for each warp
+  static constexpr int kStages = HD == 128 ? 2 : 4;  // places in flight for each warp
   static constexpr int kBlock = 20 * HD;
   static constexpr int kRow = HD + 4;  // floats of a head in a piece
   static constexpr int kPieces = 2 * kAqWarps;  // of each warp: the unit that ends in its range, the one that goes on
-  alignas(128) uint8_t ring[kAqWarps][kStages][kBlock];
-  alignas(16) float o[kAqWarps][kAqHeads][kRow];
+  alignas(128) uint8_t ring[kAqWarps][kStages][2][kBlock];
   float m[kPieces][kAqHeads], l[kPieces][kAqHeads];
   int4 piece[kPieces];  // (sequence or -1, unit, start, end) in places of the CTA's range
   uint64_t full[kAqWarps][kStages];
@@ -108,11 +108,7 @@ struct AqSmem {
   int64_t first_start;  // place of sequence first_seq in the line
   int first_seq;
   int abort;
-  // a warp's last piece lies in its ring, which is free by then
-  FRC_DEVICE_INLINE float* rows(int k) {
-    return k & 1 ? reinterpret_cast<float*>(ring[k >> 1]) : &o[k >> 1][0][0];
-  }
-  static_assert(kAqHeads * kRow * 4 <= kStages * kBlock, "a piece fits the ring");
+  static_assert(kAqHeads * kRow * 4 <= 2 * kStages * kBlock, "a piece fits the ring");
 };
 
 FRC_DEVICE_INLINE float ex2(float x) {
@@ -167,25 +163,26 @@ FRC_DEVICE_INLINE uint32_t nibbles(uint32_t w, uint32_t bias) {
                            __float2half2_rn(-64.f - B)));
 }
 
-// 16-token blocks of a sequence.
+// Tokens of a sequence that the table covers.
 FRC_DEVICE_INLINE int aq_length(const AttnQ4Params& p, int b) {
   const int64_t room = static_cast<int64_t>(p.max_pages) * p.blocks_per_page * kQ4Tokens;
   const int n = p.lengths[b];
   return n < 0 ? 0 : (n < room ? n : static_cast<int>(room));
 }
-FRC_DEVICE_INLINE int aq_blocks(int length) { return static_cast<int>((static_cast<int64_t>(length) + 15) >> 4); }
+// 32-token places of a sequence.
+FRC_DEVICE_INLINE int aq_places(int length) { return static_cast<int>((static_cast<int64_t>(length) + 31) >> 5); }
 
 // Walks the line: the unit that holds a place.  Places count from the start
 // of the CTA's range (a unit may start before it).
 struct AqWalk {
-  int seq, unit, len, nb;  // tokens and blocks of the sequence
-  int u0;                  // place of the unit, which has nb + 1
+  int seq, unit, len, np;  // tokens and places of the sequence
+  int u0;                  // place of the unit, which has np + 1
   FRC_DEVICE_INLINE void sequence(const AttnQ4Params& p, int s) {
     seq = s;
     len = aq_length(p, s);
-    nb = aq_blocks(len);
+    np = aq_places(len);
   }
-  FRC_DEVICE_INLINE int end() const { return u0 + nb + 1; }
+  FRC_DEVICE_INLINE int end() const { return u0 + np + 1; }
   FRC_DEVICE_INLINE void to(const AttnQ4Params& p, int place, int units) {
     while (place >= end()) {
       u0 = end();
@@ -204,12 +201,14 @@ struct AqWarp {
   static constexpr int NG = HD / kQ4Group;
   static constexpr bool SPLIT = sizeof(T) == 4;  // operands in two parts
   static constexpr bool TWICE = std::is_same<T, __nv_bfloat16>::value;  // p rounded to 11 bits before p d is
-  static constexpr float kUp = TWICE ? 1.f : 512.f;  // what the operand p d is scaled by, beside 32
+  // p at the reference is 2^kLift, and may be 2^(kLift + kSlack), times d up to
+  // kUp times that: p (at most 2^10 / d more) and p d stay below fp16's 65504
+  static constexpr float kLift = 1.f, kSlack = 4.f, kUp = TWICE ? 1.f : 512.f;
   uint32_t a[NG][2][4];  // query fragments: (group, k step): rows 0-7 of both k halves, rows 8-15 (low parts) of both
   uint32_t am;                       // groups' query sums
   float f_n, f_m;                    // scale of the two score products, with log2 e
   float o[NG][2][4], om[4];
-  float m_run, base, l_run;  // the reference, what is taken off the scores (five less: p times 32), the sum
+  float m_run, base, l_run;  // the reference, what is taken off the scores, the sum of p
 
   // q of head lane / 4: this lane holds channels 32 j + 8 (lane & 3) .. + 7.
   FRC_DEVICE_INLINE void load_q(const float (&x)[NG][8], float scale, int lane) {
@@ -277,13 +276,15 @@ struct AqWarp {
     l_run = 0.f;
   }
 
-  // One block in shared memory; `left` tokens of it (at least one) belong to
-  // the sequence.  Lane (r, q) = (lane / 4, lane % 4) has tokens 4 q .. 4 q + 3.
-  FRC_DEVICE_INLINE void block(const uint8_t* blk, int left, int lane, uint32_t bias) {
+  // Lane (r, q) = (lane / 4, lane % 4) has tokens 4 q .. 4 q + 3 of a block.
+
+  // Scores of a block in shared memory, of which (TAIL) `left` tokens belong to
+  // the sequence; dx: the larger of dx and the lane's V steps.
+  template <bool TAIL>
+  FRC_DEVICE_INLINE void scores(const uint8_t* blk, int left, int lane, uint32_t bias, float (&s)[4], __half2& dx) {
     constexpr Q4Layout lay(HD);
     const int r = lane >> 2, q = lane & 3;
-    float s[4];
-    uint2 kd[NG];
+    uint2 kd[NG], vd[NG];
 #pragma unroll
     for (int j = 0; j < NG; ++j) kd[j] = *reinterpret_cast<const uint2*>(blk + lay.k_step(j, 4 * q));
 #pragma unroll
@@ -319,47 +320,39 @@ struct AqWarp {
       s[2 * t] = fmaf(x0, f_n, cm[0] * f_m);
       s[2 * t + 1] = fmaf(x1, f_n, cm[1] * f_m);
     }
-    uint2 vd[NG], vm = make_uint2(0u, 0u), vml = make_uint2(0u, 0u);
 #pragma unroll
     for (int j = 0; j < NG; ++j) vd[j] = *reinterpret_cast<const uint2*>(blk + lay.v_step(j, 4 * q));
-    if (r < NG) {  // offsets m + 8 d of n - 8, in two parts for fp32
-      vm = *reinterpret_cast<const uint2*>(blk + lay.v_offset(r, 4 * q));
-      const uint2 d = *reinterpret_cast<const uint2*>(blk + lay.v_step(r, 4 * q));
-      if constexpr (SPLIT) {
-        offset_parts(d.x, vm.x, vml.x);
-        offset_parts(d.y, vm.y, vml.y);
-      } else {
-        vm.x = h2_bits(__hfma2(bits_h2(d.x), __float2half2_rn(8.f), bits_h2(vm.x)));
-        vm.y = h2_bits(__hfma2(bits_h2(d.y), __float2half2_rn(8.f), bits_h2(vm.y)));
-      }
-    }
-    if (left < kQ4Tokens) {  // what lies behind the last token may be anything, NaN among it
-      const int mine = left - 4 * q;
-      const uint32_t k0 = mine >= 2 ? 0xffffffffu : (mine == 1 ? 0xffffu : 0u);
-      const uint32_t k1 = mine >= 4 ? 0xffffffffu : (mine == 3 ? 0xffffu : 0u);
+    if constexpr (TAIL) {
+      uint32_t k0, k1;
+      own_tokens(left - 4 * q, k0, k1);
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
         vd[j].x &= k0;
         vd[j].y &= k1;
       }
-      vm.x &= k0;
-      vm.y &= k1;
-      vml.x &= k0;
-      vml.y &= k1;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (i >= mine) s[i] = -INFINITY;
+        if (i >= left - 4 * q) s[i] = -INFINITY;
     }
-    // reference: the largest s + log2 of the largest V step of the lane's four
-    // tokens, taken apart: no less than the largest s + log2 d
-    __half2 dx = __hmax2(bits_h2(vd[0].x), bits_h2(vd[0].y));
 #pragma unroll
-    for (int j = 1; j < NG; ++j) dx = __hmax2(dx, __hmax2(bits_h2(vd[j].x), bits_h2(vd[j].y)));
-    const float dm = fmaxf(__half2float(__hmax(__low2half(dx), __high2half(dx))), 1.f / 1024.f);
-    float m = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])) + lg2(dm);
+    for (int j = 0; j < NG; ++j) dx = __hmax2(dx, __hmax2(bits_h2(vd[j].x), bits_h2(vd[j].y)));
+  }
+
+  // Masks of the lane's first and second pair of tokens, of which `mine` count:
+  // what lies behind the last token may be anything, NaN among it.
+  static FRC_DEVICE_INLINE void own_tokens(int mine, uint32_t& k0, uint32_t& k1) {
+    k0 = mine >= 2 ? 0xffffffffu : (mine == 1 ? 0xffffu : 0u);
+    k1 = mine >= 4 ? 0xffffffffu : (mine == 3 ? 0xffffu : 0u);
+  }
+
+  // The reference raised, where it has to be, to m (of the lane's tokens) and
+  // the other lanes' of the head.  It may stay up to kSlack below: the operands
+  // have that room, and most raises of a running maximum are small.
+  FRC_DEVICE_INLINE void refer(float m, int lane) {
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    if (__any_sync(0xffffffffu, m > m_run)) {
+    if (__any_sync(0xffffffffu, m > m_run + kSlack)) {
+      const int q = lane & 3;
       const float m_new = fmaxf(m, m_run);
       const float keep = m_new == -INFINITY ? 1.f : ex2(m_run - m_new);
       const float f0 = __shfl_sync(0xffffffffu, keep, 8 * q), f1 = __shfl_sync(0xffffffffu, keep, 8 * q + 4);
@@ -376,7 +369,41 @@ struct AqWarp {
       om[1] *= f1;
       l_run *= keep;
       m_run = m_new;
-      base = m_new == -INFINITY ? 0.f : m_new - 5.f;
+      base = m_new == -INFINITY ? 0.f : m_new - kLift;
+    }
+  }
+
+  // The block's values, weighted by its scores.
+  template <bool TAIL>
+  FRC_DEVICE_INLINE void values(const uint8_t* blk, int left, int lane, uint32_t bias, const float (&s)[4]) {
+    constexpr Q4Layout lay(HD);
+    const int r = lane >> 2, q = lane & 3;
+    uint2 vd[NG], vm = make_uint2(0u, 0u), vml = make_uint2(0u, 0u);
+#pragma unroll
+    for (int j = 0; j < NG; ++j) vd[j] = *reinterpret_cast<const uint2*>(blk + lay.v_step(j, 4 * q));
+    if (r < NG) {  // offsets m + 8 d of n - 8, in two parts for fp32
+      vm = *reinterpret_cast<const uint2*>(blk + lay.v_offset(r, 4 * q));
+      const uint2 d = *reinterpret_cast<const uint2*>(blk + lay.v_step(r, 4 * q));
+      if constexpr (SPLIT) {
+        offset_parts(d.x, vm.x, vml.x);
+        offset_parts(d.y, vm.y, vml.y);
+      } else {
+        vm.x = h2_bits(__hfma2(bits_h2(d.x), __float2half2_rn(8.f), bits_h2(vm.x)));
+        vm.y = h2_bits(__hfma2(bits_h2(d.y), __float2half2_rn(8.f), bits_h2(vm.y)));
+      }
+    }
+    if constexpr (TAIL) {
+      uint32_t k0, k1;
+      own_tokens(left - 4 * q, k0, k1);
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        vd[j].x &= k0;
+        vd[j].y &= k1;
+      }
+      vm.x &= k0;
+      vm.y &= k1;
+      vml.x &= k0;
+      vml.y &= k1;
     }
     const float p0 = ex2(s[0] - base), p1 = ex2(s[1] - base), p2 = ex2(s[2] - base), p3 = ex2(s[3] - base);
     l_run += (p0 + p1) + (p2 + p3);
@@ -417,6 +444,39 @@ struct AqWarp {
         const uint32_t n2 = nibbles<true, 8>(u1, bias), n3 = nibbles<false, 8>(u1, bias);
         mma16816(o[j][t], n0, n1, n2, n3, b0, b1);
         if constexpr (SPLIT) mma16816(o[j][t], n0, n1, n2, n3, c0, c1);
+      }
+    }
+  }
+
+  // What the reference has to cover of a lane's scores: the largest s + log2
+  // of the largest V step of its tokens, taken apart: no less than the largest
+  // s + log2 d.
+  static FRC_DEVICE_INLINE float largest(const float (&s)[4], float m) {
+    return fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), m);
+  }
+  static FRC_DEVICE_INLINE float log2_of(__half2 dx) { return lg2(__half2float(__hmax(__low2half(dx), __high2half(dx)))); }
+
+  // The blocks of a place (bit e of `seen`: block e is there), of which `left`
+  // tokens belong to the sequence.
+  FRC_DEVICE_INLINE void place(const uint8_t (*blk)[20 * HD], uint32_t seen, int left, int lane, uint32_t bias) {
+    const __half2 least = __float2half2_rn(1.f / 1024.f);
+    if (left >= 2 * kQ4Tokens && seen == 3u) {
+      float s0[4], s1[4];
+      __half2 dx = least;
+      scores<false>(blk[0], 0, lane, bias, s0, dx);
+      scores<false>(blk[1], 0, lane, bias, s1, dx);
+      refer(largest(s0, largest(s1, -INFINITY)) + log2_of(dx), lane);
+      values<false>(blk[0], 0, lane, bias, s0);
+      values<false>(blk[1], 0, lane, bias, s1);
+    } else {
+#pragma unroll 1
+      for (int e = 0; e < 2; ++e) {
+        if (!(seen >> e & 1u)) continue;
+        float s[4];
+        __half2 dx = least;
+        scores<true>(blk[e], left - e * kQ4Tokens, lane, bias, s, dx);
+        refer(largest(s, -INFINITY) + log2_of(dx), lane);
+        values<true>(blk[e], left - e * kQ4Tokens, lane, bias, s);
       }
     }
   }
@@ -487,7 +547,7 @@ __global__ void __launch_bounds__(kAqThreads, 2) attn_q4_kernel(const AttnQ4Para
   const int per_thread = (p.batch + kAqThreads - 1) / kAqThreads;
   const int s0 = min(tid * per_thread, p.batch), s1 = min(s0 + per_thread, p.batch);
   int64_t mine = 0;
-  for (int b = s0; b < s1; ++b) mine += aq_blocks(aq_length(p, b)) + 1;
+  for (int b = s0; b < s1; ++b) mine += aq_places(aq_length(p, b)) + 1;
   int64_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -515,7 +575,7 @@ __global__ void __launch_bounds__(kAqThreads, 2) attn_q4_kernel(const AttnQ4Para
   const int64_t c0 = min(static_cast<int64_t>(blockIdx.x) * per, total), c1 = min(c0 + per, total);
   if (c0 >= before && c0 < before + mine * units) {  // one thread, unless the range is empty
     int s = s0;
-    for (int64_t next; (next = before + static_cast<int64_t>(aq_blocks(aq_length(p, s)) + 1) * units) <= c0; ++s)
+    for (int64_t next; (next = before + static_cast<int64_t>(aq_places(aq_length(p, s)) + 1) * units) <= c0; ++s)
       before = next;
     sh->first_seq = s;
     sh->first_start = before;
@@ -526,6 +586,10 @@ __global__ void __launch_bounds__(kAqThreads, 2) attn_q4_kernel(const AttnQ4Para
   const int count = static_cast<int>(c1 - c0);  // below 2^30: checked by the host
   volatile int* abort = &sh->abort;
 
+  auto piece_rows = [&](int k) {  // a warp's last piece lies in its ring, which is free by then
+    return k & 1 ? reinterpret_cast<float*>(sh->ring[k >> 1])
+                 : p.first + (static_cast<int64_t>(blockIdx.x) * kAqWarps + (k >> 1)) * kAqHeads * SM::kRow;
+  };
   // ---- this warp's range [w0, w1) of it ------------------------------------------------
   const int share = (count + kAqWarps - 1) / kAqWarps;
   const int w0 = min(warp * share, count), w1 = min(w0 + share, count);
@@ -534,52 +598,51 @@ __global__ void __launch_bounds__(kAqThreads, 2) attn_q4_kernel(const AttnQ4Para
     {
       int64_t start = sh->first_start;
       walk.sequence(p, sh->first_seq);
-      while (c0 + w0 >= start + static_cast<int64_t>(walk.nb + 1) * units) {
-        start += static_cast<int64_t>(walk.nb + 1) * units;
+      while (c0 + w0 >= start + static_cast<int64_t>(walk.np + 1) * units) {
+        start += static_cast<int64_t>(walk.np + 1) * units;
         walk.sequence(p, walk.seq + 1);
       }
-      walk.unit = static_cast<int>((c0 + w0 - start) / (walk.nb + 1));
-      walk.u0 = static_cast<int>(start + static_cast<int64_t>(walk.unit) * (walk.nb + 1) - c0);
+      walk.unit = static_cast<int>((c0 + w0 - start) / (walk.np + 1));
+      walk.u0 = static_cast<int>(start + static_cast<int64_t>(walk.unit) * (walk.np + 1) - c0);
     }
-    int page = -1, at = 0, page_next = -1, at_next = 0;  // of place lane of this batch of 32, and of the next
-    auto look_up = [&](int place) {  // the page number of a place's block, and the block's place in the page
-      page_next = -1;
+    int blk = -1, blk_next = -1;  // cache block (or none) lane % 2 of place lane / 2 of this batch of 16, and of the next
+    auto look_up = [&](int batch) {
+      const int place = w0 + batch + (lane >> 1);
+      blk_next = -1;
       if (place < w1) {
         AqWalk w = walk;
         w.to(p, place, units);
-        const int blk = place - w.u0 - 1;
-        if (blk >= 0) {
-          const int entry = blk / p.blocks_per_page;
-          at_next = w.unit / p.parts * p.blocks_per_page + (blk - entry * p.blocks_per_page);
-          page_next = p.table[w.seq * p.table_stride + entry];
+        const int b = 2 * (place - w.u0 - 1) + (lane & 1);  // below 0: the unit's empty place
+        if (b >= 0 && b * kQ4Tokens < w.len) {
+          const int entry = b / p.blocks_per_page;
+          const int page = p.table[w.seq * p.table_stride + entry];
+          if (page >= 0 && page < p.pages)
+            blk_next = (page * p.nkv + w.unit / p.parts) * p.blocks_per_page + (b - entry * p.blocks_per_page);
         }
       }
     };
-    uint32_t seen = 0;  // bit s: stage s holds a block (of a page inside the cache)
+    uint32_t seen = 0;  // two bits a stage: its blocks
     int issued = 0;
-    auto issue = [&](int s) {  // copies the next place's block, if there is one, into the stage that is free
+    auto issue = [&](int s) {  // copies the next place's blocks, if there is one, into the stage that is free
       if (w0 + issued >= w1) return;
-      if ((issued & 31) == 0) {
-        page = page_next;
-        at = at_next;
-        look_up(w0 + issued + 32 + lane);
+      const int at = issued & 15;
+      if (at == 0) {
+        blk = blk_next;
+        look_up(issued + 16);
       }
-      const int pg = __shfl_sync(0xffffffffu, page, issued & 31), in_page = __shfl_sync(0xffffffffu, at, issued & 31);
-      const bool ok = pg >= 0 && pg < p.pages;
-      seen = (seen & ~(1u << s)) | (ok ? 1u << s : 0u);
-      if (lane == 0) {
-        if (ok) {
-          mbar_arrive_expect_tx(&sh->full[warp][s], SM::kBlock);
-          bulk_g2s(sh->ring[warp][s],
-                   p.cache + (static_cast<int64_t>(pg) * p.nkv * p.blocks_per_page + in_page) * SM::kBlock,
-                   SM::kBlock, &sh->full[warp][s]);
-        } else {
-          mbar_arrive(&sh->full[warp][s]);
-        }
+      const uint32_t bits = __ballot_sync(0xffffffffu, blk >= 0) >> (2 * at) & 3u;
+      seen = (seen & ~(3u << (2 * s))) | bits << (2 * s);
+      uint64_t* bar = &sh->full[warp][s];
+      if (lane == 2 * at) {
+        if (bits) mbar_arrive_expect_tx(bar, bits == 3u ? 2 * SM::kBlock : SM::kBlock);
+        else mbar_arrive(bar);
       }
+      __syncwarp();
+      if ((lane >> 1) == at && blk >= 0)
+        bulk_g2s(sh->ring[warp][s][lane & 1], p.cache + static_cast<int64_t>(blk) * SM::kBlock, SM::kBlock, bar);
       ++issued;
     };
-    look_up(w0 + lane);
+    look_up(0);
     for (int s = 0; s < NS; ++s) issue(s);
     int s = 0;  // the stage of `place`, and the parity of its use
     uint32_t parity = 0;
@@ -606,10 +669,12 @@ __global__ void __launch_bounds__(kAqThreads, 2) attn_q4_kernel(const AttnQ4Para
       }
       st.reset();
       for (; place < end; ++place) {
-        const bool there = __all_sync(0xffffffffu, wait_phase(&sh->full[warp][s], parity, abort));
+        bool there = __all_sync(0xffffffffu, mbar_try_wait(&sh->full[warp][s], parity));
+        if (!there) there = __all_sync(0xffffffffu, wait_phase(&sh->full[warp][s], parity, abort));
         if (!there && lane == 0) atomicOr(p.status, kStatusFullWaitTimeout);
-        if (there && (seen >> s & 1u))
-          st.block(sh->ring[warp][s], min(kQ4Tokens, walk.len - (place - walk.u0 - 1) * kQ4Tokens), lane, p.bias);
+        if (there && (seen >> (2 * s) & 3u))
+          st.place(sh->ring[warp][s], seen >> (2 * s) & 3u, walk.len - (place - walk.u0 - 1) * 2 * kQ4Tokens, lane,
+                   p.bias);
         __syncwarp();
         if (there) issue(s);
         if (++s == NS) {
@@ -629,7 +694,7 @@ __global__ void __launch_bounds__(kAqThreads, 2) attn_q4_kernel(const AttnQ4Para
             int zero = 0;
             if (!wait_phase(&sh->full[warp][j % NS], (j / NS) & 1, &zero)) atomicOr(p.status, kStatusDrainTimeout);
           }
-        float* rows = sh->rows(k);
+        float* rows = piece_rows(k);
         st.sums(lane, [&](int h, int c, const float (&v)[4], float) {
           *reinterpret_cast<float4*>(rows + h * SM::kRow + c) = make_float4(v[0], v[1], v[2], v[3]);
         });
@@ -647,39 +712,45 @@ __global__ void __launch_bounds__(kAqThreads, 2) attn_q4_kernel(const AttnQ4Para
       }
   }
   __syncthreads();
-  // ---- the pieces, in order: warp h joins head h of each cut unit ------------------------
-  for (int k = 0; k < SM::kPieces;) {
-    const int4 pc = sh->piece[k];
-    if (pc.x < 0) {
-      ++k;
-      continue;
-    }
-    int k1 = k + 1;  // pieces of one unit follow one another, with gaps
-    while (k1 < SM::kPieces && (sh->piece[k1].x < 0 || sh->piece[k1].z == pc.z)) ++k1;
-    const AqHeads heads(p, pc.y);
-    const bool whole = pc.z >= 0 && pc.w <= count;
+  // ---- the pieces, in order: warp h joins head h of each cut unit; lane k has piece k ----
+  static_assert(SM::kPieces <= 32, "a piece a lane");
+  const int4 pc = sh->piece[lane & (SM::kPieces - 1)];
+  const bool own = lane < SM::kPieces && pc.x >= 0;
+  for (uint32_t left = __ballot_sync(0xffffffffu, own); left;) {
+    const int k = __ffs(left) - 1;
+    const int seq = __shfl_sync(0xffffffffu, pc.x, k), unit = __shfl_sync(0xffffffffu, pc.y, k);
+    const int u0 = __shfl_sync(0xffffffffu, pc.z, k), u1 = __shfl_sync(0xffffffffu, pc.w, k);
+    const uint32_t same = __ballot_sync(0xffffffffu, own && pc.z == u0);
+    left &= ~same;
+    const AqHeads heads(p, unit);
     if (warp < heads.count) {
       constexpr int C = HD / 32;
-      float M = -INFINITY;
-      for (int j = k; j < k1; ++j)
-        if (sh->piece[j].x >= 0) M = fmaxf(M, sh->m[j][warp]);
-      const float base = M == -INFINITY ? 0.f : M;
-      float L = 0.f, acc[C];
+      const bool mine = same >> lane & 1u;
+      float M = mine ? sh->m[lane][warp] : -INFINITY;
+      const float m = M;
+#pragma unroll
+      for (int o = 1; o < SM::kPieces; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+      M = __shfl_sync(0xffffffffu, M, 0);
+      const float f = mine ? ex2(m - (M == -INFINITY ? 0.f : M)) : 0.f;
+      float L = mine ? sh->l[lane][warp] * f : 0.f, acc[C];
+#pragma unroll
+      for (int o = 1; o < SM::kPieces; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+      L = __shfl_sync(0xffffffffu, L, 0);
 #pragma unroll
       for (int e = 0; e < C; ++e) acc[e] = 0.f;
-      for (int j = k; j < k1; ++j) {
-        if (sh->piece[j].x < 0) continue;
-        const float f = ex2(sh->m[j][warp] - base);
-        L = fmaf(sh->l[j][warp], f, L);
+#pragma unroll 4
+      for (uint32_t todo = same; todo; todo &= todo - 1) {
+        const int j = __ffs(todo) - 1;
+        const float fj = __shfl_sync(0xffffffffu, f, j);
         float v[C];
-        load_run<C, true>(sh->rows(j) + warp * SM::kRow + C * lane, v);
+        load_run<C, true>(piece_rows(j) + warp * SM::kRow + C * lane, v);
 #pragma unroll
-        for (int e = 0; e < C; ++e) acc[e] = fmaf(v[e], f, acc[e]);
+        for (int e = 0; e < C; ++e) acc[e] = fmaf(v[e], fj, acc[e]);
       }
-      if (whole) {
-        aq_store<C, T>(p, pc.x, heads.first + warp, C * lane, acc, L);
+      if (u0 >= 0 && u1 <= count) {
+        aq_store<C, T>(p, seq, heads.first + warp, C * lane, acc, L);
       } else {
-        float* row = p.part + ((2 * static_cast<int64_t>(blockIdx.x) + (pc.z >= 0 ? 1 : 0)) * kAqHeads + warp) * SM::kRow;
+        float* row = p.part + ((2 * static_cast<int64_t>(blockIdx.x) + (u0 >= 0 ? 1 : 0)) * kAqHeads + warp) * SM::kRow;
         if (lane == 0) {
           row[0] = M;
           row[1] = L;
@@ -687,9 +758,8 @@ __global__ void __launch_bounds__(kAqThreads, 2) attn_q4_kernel(const AttnQ4Para
         store_run<C, true>(row + 4 + C * lane, acc);
       }
     }
-    if (pc.z >= 0 && pc.w > count && tid == 0)  // goes on in the next CTAs
-      p.desc[blockIdx.x] = make_int4(pc.x, pc.y, static_cast<int>((c0 + pc.w - 1) / per - blockIdx.x), 0);
-    k = k1;
+    if (u0 >= 0 && u1 > count && tid == 0)  // goes on in the next CTAs
+      p.desc[blockIdx.x] = make_int4(seq, unit, static_cast<int>((c0 + u1 - 1) / per - blockIdx.x), 0);
   }
 }
 
@@ -778,8 +848,9 @@ extern "C" {
 int frc_attention_decode_q4_workspace(int batch, int nh, int nkv, int hd, size_t* bytes) {
   FRC_REQUIRE(bytes && batch >= 0 && nh > 0 && nkv > 0 && nh % nkv == 0 && (hd == 64 || hd == 128),
               "frc_attention_decode_q4_workspace: bad arguments");
-  // partial heads: two units a CTA; and a descriptor a CTA
-  *bytes = static_cast<size_t>(frc::kAqGrid) * (2 * frc::kAqHeads * (hd + 4) * sizeof(float) + sizeof(int4));
+  // pieces of units, two a CTA and one a warp; and a descriptor a CTA
+  *bytes = static_cast<size_t>(frc::kAqGrid) *
+           ((2 + frc::kAqWarps) * frc::kAqHeads * (hd + 4) * sizeof(float) + sizeof(int4));
   return FRC_OK;
 }
 
@@ -794,7 +865,7 @@ int frc_attention_decode_q4(int type, const void* q, int64_t q_seq_stride, int64
               "frc_attention_decode_q4: needs nh a multiple of nkv");
   FRC_REQUIRE(page_size > 0 && page_size % frc::kQ4Tokens == 0,
               "frc_attention_decode_q4: page_size must be a multiple of 16");
-  FRC_REQUIRE(pages > 0 && pages <= 0x7fffffff / (page_size / frc::kQ4Tokens),
+  FRC_REQUIRE(pages > 0 && pages <= 0x7fffffff / (page_size / frc::kQ4Tokens) / nkv,
               "frc_attention_decode_q4: bad number of pages");
   FRC_REQUIRE(batch >= 0 && batch <= 65535 && max_pages >= 0 && table_stride >= 0,
               "frc_attention_decode_q4: bad batch or block table");
@@ -812,9 +883,9 @@ int frc_attention_decode_q4(int type, const void* q, int64_t q_seq_stride, int64
   const int parts = (nh / nkv + frc::kAqHeads - 1) / frc::kAqHeads;
   // no more CTAs than the tables could give places for
   const int64_t blocks = static_cast<int64_t>(max_pages) * (page_size / frc::kQ4Tokens);
-  FRC_REQUIRE(blocks < (int64_t(1) << 31) && static_cast<int64_t>(nkv) * parts <= 65535,
+  FRC_REQUIRE(blocks < (int64_t(1) << 48) && static_cast<int64_t>(nkv) * parts <= 65535,
               "frc_attention_decode_q4: block table or heads too large");
-  const int64_t most = static_cast<int64_t>(batch) * nkv * parts * ((blocks < (1 << 27) ? blocks : (1 << 27)) + 1);
+  const int64_t most = static_cast<int64_t>(batch) * nkv * parts * ((blocks < (1 << 27) ? (blocks + 1) / 2 : (1 << 26)) + 1);
   const int64_t want = (most + frc::kAqMinPlaces - 1) / frc::kAqMinPlaces;
   const int grid = static_cast<int>(want < frc::kAqGrid ? want : frc::kAqGrid);
   FRC_REQUIRE(most / grid < (int64_t(1) << 30), "frc_attention_decode_q4: block table too large");
@@ -844,7 +915,8 @@ int frc_attention_decode_q4(int type, const void* q, int64_t q_seq_stride, int64
   p.q_vec = frc::aligned_to(q, 16) && q_seq_stride % run == 0 && q_head_stride % run == 0;
   p.o_vec = frc::aligned_to(out, 4 * es) && out_seq_stride % 4 == 0 && out_head_stride % 4 == 0;
   p.part = static_cast<float*>(workspace);
-  p.desc = reinterpret_cast<int4*>(p.part + static_cast<size_t>(frc::kAqGrid) * 2 * frc::kAqHeads * (hd + 4));
+  p.first = p.part + static_cast<size_t>(frc::kAqGrid) * 2 * frc::kAqHeads * (hd + 4);
+  p.desc = reinterpret_cast<int4*>(p.first + static_cast<size_t>(frc::kAqGrid) * frc::kAqWarps * frc::kAqHeads * (hd + 4));
   p.status = static_cast<uint32_t*>(status);
   p.bias = 0x64006400u;
   return frc_with_type(type, [&](auto* z) -> int {
