@@ -7,12 +7,41 @@
 // every key, each earlier one a key less (so a prompt may follow tokens that
 // are there already).  A query that sees no key gives zeros, and rows behind
 // the last sequence stay as they are.
+//
+// Bound by the tensor cores and, as much, by the exponentials: a tile of 128
+// queries by 128 keys is 2 * 128^3 multiply-adds (1024 cycles at 4096 a cycle)
+// and 128^2 exponentials (1024 cycles at 16 a cycle).  Two tiles of queries
+// therefore take turns: while one's scores pass through the softmax, the
+// other's products run.  A CTA owns 256 queries of a head and an SM:
+//
+//   warp 9        loads: the two query tiles once, then K and V tiles of 128
+//                 keys through a ring (TMA, 128-byte swizzle)
+//   warp 8        issues tcgen05.mma: S = Q K^T (128 x 128 fp32 in tensor
+//                 memory), and O += P V with P read from tensor memory, where
+//                 it takes the place of S; V is the transposed operand as it lies
+//   warps 0-3,    softmax of tile 0 and 1, a row a thread: maximum, exponentials,
+//   warps 4-7     P rounded to the type of the inputs; at the end O / sum
+//
+// The running maximum is a reference that may stay 2^8 behind: O in tensor
+// memory is rescaled only when a row passes that, which few tiles do.  Scores,
+// maxima, sums and O are fp32; P is rounded to the inputs' type, as its operand
+// must be, and the sum is of the unrounded values.
+//
+// What is masked has no part in the result whatever it holds: scores are
+// replaced, V rows behind the last key are zeroed in shared memory, and a row
+// that comes out not finite (a NaN or infinity among the keys of its tile that it
+// does not see makes 0 * NaN) is computed again from the keys it sees alone.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdio>
+#include <cstring>
 
 #include "../../include/frcuda.h"
+#include "gemv.cuh"
 #include "kv_q4.cuh"
+#include "launch.cuh"
 
 namespace frc {
 
@@ -21,53 +50,539 @@ struct PrefillParams {
   int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
   const int *cu_q, *cu_k;
   int batch;
-  int64_t tokens_q, tokens_k;
+  int tokens_q, tokens_k;
   int nh, nkv;
-  float scale;
+  int q_mul, k_mul, v_mul;  // 0: the heads are one (stride 0), 1: the map's second coordinate is the head
+  float scale;              // not negative; times log2 e
+  float signed_scale;       // as given
+  int negate;               // scale was negative: Q is negated in the product
   int causal;
+  int q_blocks;
   void* out;
   int64_t o_tok, o_head;
+  int o_vec;
+  uint32_t* status;
 };
 
-// One warp for each (query, head).
+constexpr int kPfRows = 128;     // queries of a tile, keys of a tile
+constexpr int kPfTiles = 2;      // query tiles of a CTA
+constexpr int kPfThreads = 320;
+constexpr float kPfSlack = 8.f;  // powers of two that the reference may stay behind
+
+template <int HD>
+struct PfSmem {
+  static constexpr int kHalf = kPfRows * 128;           // 64 channels of 128 rows, swizzled: 16 KB
+  static constexpr int kTile = HD / 64 * kHalf;
+  static constexpr int kStages = HD == 128 ? 5 : 8;
+  alignas(1024) uint8_t q[kPfTiles][kTile];
+  alignas(1024) uint8_t ring[kStages][kTile];
+  uint64_t q_full, full[kStages], empty[kStages];
+  uint64_t s_full[kPfTiles], p_ready[kPfTiles], o_done[kPfTiles], drain;
+  uint32_t tmem;
+  int abort;
+};
+
+// ---- tcgen05 ---------------------------------------------------------------------
+// Descriptor of a tile of rows of 128 bytes, 128-byte swizzle (8-row atoms of
+// 1024 bytes).  K-major (rows are M or N): the stride is between atoms and the
+// leading offset unused.  MN-major (rows are K): the stride is between groups
+// of eight rows of K, the leading offset between blocks of 64 columns.
+FRC_DEVICE_INLINE uint64_t pf_desc(uint32_t addr, uint32_t leading) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | static_cast<uint64_t>((leading >> 4) & 0x3FFFu) << 16 |
+         static_cast<uint64_t>(1024u >> 4) << 32 | static_cast<uint64_t>(1u) << 46 | static_cast<uint64_t>(2u) << 61;
+}
+
+template <typename T>
+__host__ __device__ constexpr uint32_t pf_idesc(int n, bool b_mn_major) {
+  constexpr uint32_t fmt = sizeof(T) == 2 && !std::is_same<T, __half>::value ? 1u : 0u;  // bf16 : fp16
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | (b_mn_major ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(kPfRows >> 4) << 24);
+}
+constexpr uint32_t kPfNegateA = 1u << 13;
+
+// D (tensor memory) (+)= A (shared) B (shared)
+FRC_DEVICE_INLINE void pf_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// D (tensor memory) (+)= A (tensor memory) B (shared)
+FRC_DEVICE_INLINE void pf_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+FRC_DEVICE_INLINE void pf_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+FRC_DEVICE_INLINE void pf_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+FRC_DEVICE_INLINE void pf_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+#define FRC_R8(r, i) "=r"((r)[i]), "=r"((r)[i + 1]), "=r"((r)[i + 2]), "=r"((r)[i + 3]), "=r"((r)[i + 4]), "=r"((r)[i + 5]), "=r"((r)[i + 6]), "=r"((r)[i + 7])
+#define FRC_I8(r, i) "r"((r)[i]), "r"((r)[i + 1]), "r"((r)[i + 2]), "r"((r)[i + 3]), "r"((r)[i + 4]), "r"((r)[i + 5]), "r"((r)[i + 6]), "r"((r)[i + 7])
+
+// 32 columns of the lane's row; valid after tmem_wait_ld.
+FRC_DEVICE_INLINE void tmem_ld32(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : FRC_R8(r, 0), FRC_R8(r, 8), FRC_R8(r, 16), FRC_R8(r, 24)
+      : "r"(addr));
+}
+FRC_DEVICE_INLINE void tmem_st32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::FRC_I8(r, 0), FRC_I8(r, 8), FRC_I8(r, 16),
+      FRC_I8(r, 24), "r"(addr)
+      : "memory");
+}
+FRC_DEVICE_INLINE void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+FRC_DEVICE_INLINE void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+FRC_DEVICE_INLINE void pf_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
+FRC_DEVICE_INLINE float pf_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+FRC_DEVICE_INLINE uint32_t pf_pack(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// Two fp32 operations in one instruction.
+FRC_DEVICE_INLINE uint64_t pf_two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+FRC_DEVICE_INLINE void pf_split(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+FRC_DEVICE_INLINE uint64_t pf_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+FRC_DEVICE_INLINE uint64_t pf_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// The rows of a CTA.
+struct PfWork {
+  int head, q_start, q_len, k_start, k_len;  // the sequence
+  int q0;                                    // first query of the CTA in it
+  // Block `rank` of the queries, from the last one on (the longest first where
+  // there is one sequence): all lanes of a warp call it.  False: there is none.
+  FRC_DEVICE_INLINE bool find(const PrefillParams& p, int rank, int lane) {
+    for (int top = p.batch; top > 0; top -= 32) {
+      const int b = top - 1 - lane;
+      int a0 = 0, a1 = 0;
+      if (b >= 0) {
+        a0 = min(max(p.cu_q[b], 0), p.tokens_q);
+        a1 = min(max(p.cu_q[b + 1], a0), p.tokens_q);
+      }
+      const int n = (a1 - a0 + kPfTiles * kPfRows - 1) / (kPfTiles * kPfRows);
+      int incl = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, rank < incl);
+      if (!hit) {
+        rank -= __shfl_sync(0xffffffffu, incl, 31);
+        continue;
+      }
+      const int l = __ffs(hit) - 1;
+      q_start = __shfl_sync(0xffffffffu, a0, l);
+      q_len = __shfl_sync(0xffffffffu, a1, l) - q_start;
+      const int blocks = __shfl_sync(0xffffffffu, n, l);
+      const int in_seq = rank - (__shfl_sync(0xffffffffu, incl, l) - blocks);
+      q0 = (blocks - 1 - in_seq) * kPfTiles * kPfRows;
+      const int s = top - 1 - l;
+      k_start = min(max(p.cu_k[s], 0), p.tokens_k);
+      k_len = min(max(p.cu_k[s + 1], k_start), p.tokens_k) - k_start;
+      return true;
+    }
+    return false;
+  }
+  FRC_DEVICE_INLINE int rows(int tile) const { return min(max(q_len - q0 - tile * kPfRows, 0), kPfRows); }
+  // Keys that query `row` of the sequence sees.
+  FRC_DEVICE_INLINE int seen(const PrefillParams& p, int row) const {
+    return p.causal ? min(max(row + 1 + k_len - q_len, 0), k_len) : k_len;
+  }
+  // Key tiles of a query tile.
+  FRC_DEVICE_INLINE int tiles(const PrefillParams& p, int tile) const {
+    const int n = rows(tile);
+    return n == 0 ? 0 : (seen(p, q0 + tile * kPfRows + n - 1) + kPfRows - 1) / kPfRows;
+  }
+};
+
+// One row from the keys it sees alone: a warp, HD / 32 channels a lane.
 template <typename T, int HD>
-__global__ void __launch_bounds__(32) attn_prefill_kernel(PrefillParams p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" :::);
+__device__ __noinline__ void pf_row_again(const PrefillParams& p, const PfWork& w, int row, int lane) {
   constexpr int C = HD / 32;
-  const int64_t i = blockIdx.x;
-  const int h = blockIdx.y, g = h / (p.nh / p.nkv), lane = threadIdx.x;
-  int b = 0;
-  while (b < p.batch && p.cu_q[b + 1] <= i) ++b;
-  if (b == p.batch || p.cu_q[b] > i) return;
-  const int64_t k0 = max(p.cu_k[b], 0);
-  int64_t k1 = min(static_cast<int64_t>(p.cu_k[b + 1]), p.tokens_k);
-  if (p.causal) k1 -= p.cu_q[b + 1] - 1 - i;
-  const T* qp = static_cast<const T*>(p.q) + i * p.q_tok + h * p.q_head;
+  const int h = w.head, g = h / (p.nh / p.nkv);
+  const T* qp = static_cast<const T*>(p.q) + (w.q_start + row) * p.q_tok + h * p.q_head;
   float qv[C], acc[C];
 #pragma unroll
   for (int e = 0; e < C; ++e) {
-    qv[e] = to_f32(qp[C * lane + e]) * p.scale;
+    qv[e] = to_f32(qp[C * lane + e]);
     acc[e] = 0.f;
   }
   float mx = -INFINITY, sum = 0.f;
-  for (int64_t j = k0; j < k1; ++j) {
-    const T* kp = static_cast<const T*>(p.k) + j * p.k_tok + g * p.k_head + C * lane;
-    const T* vp = static_cast<const T*>(p.v) + j * p.v_tok + g * p.v_head + C * lane;
+  const int n = w.seen(p, row);
+  for (int j = 0; j < n; ++j) {
+    const int64_t t = w.k_start + j;
+    const T* kp = static_cast<const T*>(p.k) + t * p.k_tok + g * p.k_head + C * lane;
+    const T* vp = static_cast<const T*>(p.v) + t * p.v_tok + g * p.v_head + C * lane;
     float s = 0.f;
 #pragma unroll
     for (int e = 0; e < C; ++e) s = fmaf(qv[e], to_f32(kp[e]), s);
-    s = warp_sum(s);
-    const float m_new = fmaxf(mx, s), keep = mx == m_new ? 1.f : expf(mx - m_new), w = expf(s - m_new);
+    s = warp_sum(s) * p.signed_scale;
+    const float m_new = fmaxf(mx, s), keep = mx == m_new ? 1.f : expf(mx - m_new), x = expf(s - m_new);
     mx = m_new;
-    sum = fmaf(sum, keep, w);
+    sum = fmaf(sum, keep, x);
 #pragma unroll
-    for (int e = 0; e < C; ++e) acc[e] = fmaf(acc[e], keep, w * to_f32(vp[e]));
+    for (int e = 0; e < C; ++e) acc[e] = fmaf(acc[e], keep, x * to_f32(vp[e]));
   }
-  T* op = static_cast<T*>(p.out) + i * p.o_tok + h * p.o_head;
-  const float inv = mx == -INFINITY ? 0.f : 1.f / sum;
+  T* op = static_cast<T*>(p.out) + (w.q_start + row) * p.o_tok + h * p.o_head;
 #pragma unroll
-  for (int e = 0; e < C; ++e) from_f32(acc[e] * inv, op[C * lane + e]);
+  for (int e = 0; e < C; ++e) from_f32(acc[e] / sum, op[C * lane + e]);
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kPfThreads, 1)
+    attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                        const __grid_constant__ CUtensorMap vmap, const PrefillParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  using SM = PfSmem<HD>;
+  constexpr int NS = SM::kStages, H = HD / 64;
+  extern __shared__ __align__(1024) uint8_t pf_smem[];
+  SM* sh = reinterpret_cast<SM*>(pf_smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  PfWork w;
+  w.head = blockIdx.x % p.nh;
+  if (!w.find(p, blockIdx.x / p.nh, lane)) return;  // the same in all threads
+  const int n0 = w.tiles(p, 0), n1 = w.tiles(p, 1), n = max(n0, n1);
+  const int kvh = w.head / (p.nh / p.nkv);
+  if (smem_u32(pf_smem) & 1023u) {  // swizzled tiles need 1024-byte alignment
+    if (threadIdx.x == 0) atomicOr(p.status, kStatusSmemMisaligned);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    mbar_init(&sh->q_full, 1);
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&sh->full[s], 1);
+      mbar_init(&sh->empty[s], 1);
+    }
+    for (int t = 0; t < kPfTiles; ++t) {
+      mbar_init(&sh->s_full[t], 1);
+      mbar_init(&sh->p_ready[t], 4);
+      mbar_init(&sh->o_done[t], 1);
+    }
+    mbar_init(&sh->drain, 1);
+    sh->abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh->tmem)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  pf_fence_before();
+  __syncthreads();
+  pf_fence_after();
+  const uint32_t tmem = sh->tmem;  // S of tile t at column 128 t, O at 256 + HD t
+  volatile int* abort = &sh->abort;
+
+  if (warp == 9) {
+    // ---- loads -----------------------------------------------------------------------
+    if (lane == 0 && n > 0) {
+      const int q_tiles = w.rows(1) > 0 ? 2 : 1;
+      mbar_arrive_expect_tx(&sh->q_full, q_tiles * SM::kTile);
+      for (int t = 0; t < q_tiles; ++t)
+        for (int h = 0; h < H; ++h)
+          pf_load_3d(sh->q[t] + h * SM::kHalf, &qmap, 64 * h, w.head * p.q_mul, w.q_start + w.q0 + t * kPfRows,
+                     &sh->q_full);
+      int issued = 0;
+      for (; issued < 2 * n; ++issued) {  // K 0, V 0, K 1, V 1, ...
+        const int s = issued % NS;
+        if (issued >= NS && !wait_phase(&sh->empty[s], (issued / NS - 1) & 1, abort)) {
+          atomicOr(p.status, kStatusEmptyWaitTimeout);
+          break;
+        }
+        mbar_arrive_expect_tx(&sh->full[s], SM::kTile);
+        const int key = w.k_start + (issued >> 1) * kPfRows;
+        for (int h = 0; h < H; ++h)
+          pf_load_3d(sh->ring[s] + h * SM::kHalf, issued & 1 ? &vmap : &kmap, 64 * h,
+                     kvh * (issued & 1 ? p.v_mul : p.k_mul), key, &sh->full[s]);
+      }
+      // no copy may still be landing when the CTA exits
+      int zero = 0;
+      bool ok = wait_phase(&sh->q_full, 0, &zero);
+      for (int i = issued > NS ? issued - NS : 0; i < issued; ++i) ok = wait_phase(&sh->full[i % NS], (i / NS) & 1, &zero) && ok;
+      if (!ok) atomicOr(p.status, kStatusDrainTimeout);
+    }
+  } else if (warp == 8) {
+    // ---- products: one thread issues, the warp waits -------------------------------------
+    if (n > 0) {
+      constexpr uint32_t id_pv = pf_idesc<T>(HD, true);
+      const uint32_t id_qk = pf_idesc<T>(kPfRows, false) | (p.negate ? kPfNegateA : 0u);
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, wait_phase(bar, parity & 1, abort));
+      };
+      auto qk = [&](int t, int stage) {
+        if (lane == 0) {
+          const uint32_t a = smem_u32(sh->q[t]), b = smem_u32(sh->ring[stage]);
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k) {
+            const uint32_t off = k / 4 * SM::kHalf + k % 4 * 32;
+            pf_mma_ss(tmem + 128 * t, pf_desc(a + off, 16), pf_desc(b + off, 16), id_qk, k > 0);
+          }
+          pf_commit(&sh->s_full[t]);
+        }
+      };
+      auto pv = [&](int t, int stage, bool first) {
+        if (lane == 0) {
+          const uint32_t b = smem_u32(sh->ring[stage]);
+#pragma unroll
+          for (int k = 0; k < kPfRows / 16; ++k)
+            pf_mma_ts(tmem + 256 + HD * t, tmem + 128 * t + 8 * k, pf_desc(b + k * 2048, SM::kHalf), id_pv,
+                      !first || k > 0);
+          pf_commit(&sh->o_done[t]);
+        }
+      };
+      auto release = [&](int stage) {
+        if (lane == 0) pf_commit(&sh->empty[stage]);
+      };
+      bool ok = wait(&sh->q_full, 0) && wait(&sh->full[0], 0);
+      if (ok) {
+        pf_fence_after();
+        if (n0 > 0) qk(0, 0);
+        if (n1 > 0) qk(1, 0);
+        release(0);
+      }
+      for (int j = 0; ok && j < n; ++j) {
+        const int iv = 2 * j + 1, sv = iv % NS, ik = 2 * j + 2, sk = ik % NS;
+        ok = wait(&sh->full[sv], iv / NS);
+        if (!ok) break;
+        const int left = w.k_len - j * kPfRows;
+        if (left < kPfRows) {  // rows behind the last key: zeros, whatever lies there
+          uint4* row = reinterpret_cast<uint4*>(sh->ring[sv]);
+          for (int h = 0; h < H; ++h)
+            for (int i = left * 8 + lane; i < kPfRows * 8; i += 32) row[h * (SM::kHalf / 16) + i] = make_uint4(0, 0, 0, 0);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
+        bool k_there = false;
+#pragma unroll
+        for (int t = 0; t < kPfTiles; ++t) {
+          const int nt = t ? n1 : n0;
+          if (j >= nt) continue;
+          ok = ok && wait(&sh->p_ready[t], j);
+          if (!ok) break;
+          pf_fence_after();
+          pv(t, sv, j == 0);
+          if (j + 1 < nt) {
+            if (!k_there) ok = wait(&sh->full[sk], ik / NS);
+            if (!ok) break;
+            k_there = true;
+            pf_fence_after();
+            qk(t, sk);
+          }
+        }
+        if (!ok) break;
+        release(sv);
+        if (j + 1 < n) release(sk);
+      }
+      if (!ok && lane == 0) {
+        atomicOr(p.status, kStatusFullWaitTimeout);
+        *abort = 1;
+      }
+      // no product may be in flight at the teardown
+      if (lane == 0) {
+        pf_commit(&sh->drain);
+        int zero = 0;
+        if (!wait_phase(&sh->drain, 0, &zero)) atomicOr(p.status, kStatusDrainTimeout);
+      }
+    }
+  } else {
+    // ---- softmax: warps 4 t .. 4 t + 3 have tile t, a row a thread ------------------------
+    const int t = warp >> 2, nt = t ? n1 : n0;
+    const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+    const uint32_t s_at = tmem + lanes + 128 * t, o_at = tmem + lanes + 256 + HD * t;
+    const int r = 32 * (warp & 3) + lane, row = w.q0 + kPfRows * t + r;
+    const bool live = r < w.rows(t);
+    const int seen = live ? w.seen(p, row) : 0;
+    const float scale = p.scale;
+    float m_ref = -INFINITY, sum = 0.f;  // reference in units of the unscaled score
+    bool ok = true;
+    for (int j = 0; j < nt; ++j) {
+      ok = __all_sync(0xffffffffu, wait_phase(&sh->s_full[t], j & 1, abort));
+      if (!ok) break;
+      pf_fence_after();
+      uint32_t x[kPfRows];
+#pragma unroll
+      for (int c = 0; c < kPfRows; c += 32) tmem_ld32(s_at + c, x + c);
+      tmem_wait_ld();
+      const int mine = seen - j * kPfRows;  // columns that the row sees
+      if (!__all_sync(0xffffffffu, mine >= kPfRows)) {
+#pragma unroll
+        for (int c = 0; c < kPfRows; ++c) x[c] = c < mine ? x[c] : 0xff800000u;
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < kPfRows; c += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1])));
+      const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      if (__any_sync(0xffffffffu, (m - m_ref) * scale > kPfSlack)) {
+        const float m_new = fmaxf(m, m_ref);
+        const float keep = m_new == -INFINITY ? 1.f : pf_ex2((m_ref - m_new) * scale);
+        m_ref = m_new;
+        sum *= keep;
+        if (j > 0) {
+          ok = __all_sync(0xffffffffu, wait_phase(&sh->o_done[t], (j - 1) & 1, abort));
+          if (!ok) break;
+          pf_fence_after();
+#pragma unroll
+          for (int c = 0; c < HD; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_at + c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+            tmem_st32(o_at + c, o);
+          }
+        }
+      }
+      const float base = m_ref == -INFINITY ? 0.f : -m_ref * scale;
+      const uint64_t scale2 = pf_two(scale, scale), base2 = pf_two(base, base);
+      uint64_t part[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int c = 0; c < kPfRows; c += 64) {
+        uint32_t y[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const int i = c + 2 * e;
+          float a, b;
+          pf_split(pf_fma2(pf_two(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, base2), a, b);
+          a = pf_ex2(a);
+          b = pf_ex2(b);
+          part[e & 3] = pf_add2(part[e & 3], pf_two(a, b));
+          y[e] = pf_pack<T>(a, b);
+        }
+        tmem_st32(s_at + c / 2, y);
+      }
+      float a0, a1;
+      pf_split(pf_add2(pf_add2(part[0], part[1]), pf_add2(part[2], part[3])), a0, a1);
+      sum += a0 + a1;
+      tmem_wait_st();
+      pf_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->p_ready[t]);
+    }
+    // ---- O / sum ---------------------------------------------------------------------
+    if (ok && nt > 0) ok = __all_sync(0xffffffffu, wait_phase(&sh->o_done[t], (nt - 1) & 1, abort));
+    if (!ok) {
+      if (lane == 0) atomicOr(p.status, kStatusFullWaitTimeout);
+    } else {
+      pf_fence_after();
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      T* op = static_cast<T*>(p.out) + static_cast<int64_t>(w.q_start + row) * p.o_tok + w.head * p.o_head;
+      bool finite = true;
+#pragma unroll
+      for (int c = 0; c < HD; c += 32) {
+        float v[32];
+        if (nt > 0) {
+          uint32_t o[32];
+          tmem_ld32(o_at + c, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            v[e] = __uint_as_float(o[e]) * inv;
+            finite = finite && fabsf(v[e]) <= 3.402823466e38f;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = 0.f;
+        }
+        if (live) {
+          if (seen == 0)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = 0.f;
+          if (p.o_vec) store_run<32, true>(op + c, v);
+          else store_run<32, false>(op + c, v);
+        }
+      }
+      __syncwarp();
+      for (uint32_t again = __ballot_sync(0xffffffffu, live && seen > 0 && !finite); again; again &= again - 1)
+        pf_row_again<T, HD>(p, w, w.q0 + kPfRows * t + 32 * (warp & 3) + __ffs(again) - 1, lane);
+    }
+  }
+  // ---- teardown: every warp here, no product or tensor-memory access in flight -----------
+  pf_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    pf_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+// Map of (tokens, heads, hd) in boxes of 128 tokens of 64 channels; a head
+// stride of 0 (a broadcast head) is a map of one head.
+inline bool pf_map(CUtensorMap* map, int type, const void* base, int64_t tokens, int heads, int hd, int64_t tok_stride,
+                   int64_t head_stride, int* mul) {
+  auto encode = tensor_map_encoder();
+  if (!encode) return false;
+  *mul = head_stride == 0 ? 0 : 1;
+  const bool one = heads == 1 || head_stride == 0;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(one ? 1 : heads),
+                              static_cast<cuuint64_t>(tokens)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(one ? hd : head_stride) * 2,
+                                 static_cast<cuuint64_t>(tokens == 1 ? hd : tok_stride) * 2};
+  const cuuint32_t box[3] = {64, 1, kPfRows}, step[3] = {1, 1, 1};
+  std::memset(map, 0, sizeof *map);
+  return encode(map, type == FRC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int HD>
+cudaError_t launch_prefill(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const PrefillParams& p,
+                           cudaStream_t st) {
+  static std::atomic<uint64_t> ready{0};  // devices on which the kernel may use its shared memory
+  const cudaError_t e = allow_smem(attn_prefill_kernel<T, HD>, sizeof(PfSmem<HD>), ready);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(attn_prefill_kernel<T, HD>, dim3(static_cast<unsigned>(p.q_blocks) * p.nh), dim3(kPfThreads),
+                    sizeof(PfSmem<HD>), st, q, k, v, p);
 }
 
 }  // namespace frc
@@ -81,25 +596,67 @@ extern "C" int frc_attention_prefill(int type, const void* q, int64_t q_tok_stri
   FRC_REQUIRE(type == FRC_F16 || type == FRC_BF16, "frc_attention_prefill: type must be FRC_F16 or FRC_BF16");
   FRC_REQUIRE(hd == 64 || hd == 128, "frc_attention_prefill: head_dim must be 64 or 128");
   FRC_REQUIRE(nh > 0 && nkv > 0 && nh <= 65535 && nh % nkv == 0, "frc_attention_prefill: needs nh a multiple of nkv");
-  FRC_REQUIRE(batch >= 0 && tokens_q >= 0 && tokens_k >= 0 && tokens_q <= 0x7fffffff && tokens_k <= 0x7fffffff,
+  FRC_REQUIRE(batch >= 0 && tokens_q >= 0 && tokens_k >= 0 && tokens_q <= (1 << 30) && tokens_k <= (1 << 30),
               "frc_attention_prefill: bad batch or tokens");
   const int64_t strides[] = {q_tok_stride, q_head_stride, k_tok_stride, k_head_stride,
                              v_tok_stride, v_head_stride, out_tok_stride, out_head_stride};
   for (const int64_t s : strides)
-    FRC_REQUIRE(s >= 0 && s % 8 == 0, "frc_attention_prefill: strides must be multiples of 8 elements");
+    FRC_REQUIRE(s >= 0 && s % 8 == 0 && s < (int64_t(1) << 38),
+                "frc_attention_prefill: strides must be multiples of 8 elements, below 2^38");
+  FRC_REQUIRE((q_tok_stride > 0 || tokens_q <= 1) && ((k_tok_stride > 0 && v_tok_stride > 0) || tokens_k <= 1),
+              "frc_attention_prefill: token strides must not be zero");
+  FRC_REQUIRE(scale == scale && scale - scale == 0.f, "frc_attention_prefill: scale must be finite");
   if (batch == 0 || tokens_q == 0) return FRC_OK;
   FRC_REQUIRE(q && ((k && v) || tokens_k == 0) && cu_q && cu_k && out, "frc_attention_prefill: null pointer");
   FRC_REQUIRE(frc::aligned_to(q, 16) && frc::aligned_to(k, 16) && frc::aligned_to(v, 16) && frc::aligned_to(out, 16),
               "frc_attention_prefill: q, k, v and out must be 16-byte aligned");
-  const frc::PrefillParams p{q, k, v, q_tok_stride, q_head_stride, k_tok_stride, k_head_stride, v_tok_stride,
-                             v_head_stride, cu_q, cu_k, batch, tokens_q, tokens_k, nh, nkv, scale, causal, out,
-                             out_tok_stride, out_head_stride};
-  return frc_with_type(type, [&](auto* z) -> int {
-    using T = std::remove_pointer_t<decltype(z)>;
-    void (*fn)(frc::PrefillParams) = hd == 128 ? frc::attn_prefill_kernel<T, 128> : frc::attn_prefill_kernel<T, 64>;
-    FRC_LAUNCHED(frc::launch_pdl(fn, dim3(static_cast<unsigned>(tokens_q), nh), dim3(32), 0,
-                                 static_cast<cudaStream_t>(stream), p),
-                 "attention_prefill launch");
-    return FRC_OK;
-  });
+  frc::PrefillParams p{};
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.q_tok = q_tok_stride;
+  p.q_head = q_head_stride;
+  p.k_tok = k_tok_stride;
+  p.k_head = k_head_stride;
+  p.v_tok = v_tok_stride;
+  p.v_head = v_head_stride;
+  p.cu_q = cu_q;
+  p.cu_k = cu_k;
+  p.batch = batch;
+  p.tokens_q = static_cast<int>(tokens_q);
+  p.tokens_k = static_cast<int>(tokens_k);
+  p.nh = nh;
+  p.nkv = nkv;
+  p.signed_scale = scale;
+  p.negate = scale < 0.f;
+  // a scale of 0 weighs all keys alike: so does one that takes any finite score to next to nothing
+  const float size = scale < 0.f ? -scale : scale;
+  p.scale = size < 1e-30f ? 1e-30f : size * 1.44269504088896341f;
+  p.causal = causal != 0;
+  // at most: a partly filled block for each sequence that has a query
+  const int64_t per = frc::kPfTiles * frc::kPfRows;
+  const int64_t blocks = tokens_q / per + (batch < tokens_q ? batch : tokens_q);
+  FRC_REQUIRE(blocks * nh <= 0x7fffffff, "frc_attention_prefill: too many queries");
+  p.q_blocks = static_cast<int>(blocks);
+  p.out = out;
+  p.o_tok = out_tok_stride;
+  p.o_head = out_head_stride;
+  p.o_vec = 1;
+  FRC_LAUNCHED(frc::serving_status(&p.status), "status word");
+  CUtensorMap qm, km, vm;
+  const bool none = tokens_k == 0;  // no key is read: any valid map will do
+  if (!frc::pf_map(&qm, type, q, tokens_q, nh, hd, q_tok_stride, q_head_stride, &p.q_mul) ||
+      !frc::pf_map(&km, type, none ? q : k, none ? tokens_q : tokens_k, none ? nh : nkv, hd,
+                   none ? q_tok_stride : k_tok_stride, none ? q_head_stride : k_head_stride, &p.k_mul) ||
+      !frc::pf_map(&vm, type, none ? q : v, none ? tokens_q : tokens_k, none ? nh : nkv, hd,
+                   none ? q_tok_stride : v_tok_stride, none ? q_head_stride : v_head_stride, &p.v_mul))
+    return frc__fail(FRC_ERR_CUDA, "frc_attention_prefill: cuTensorMapEncodeTiled failed");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool bf = type == FRC_BF16;
+  FRC_LAUNCHED((hd == 128 ? (bf ? frc::launch_prefill<__nv_bfloat16, 128>(qm, km, vm, p, st)
+                                : frc::launch_prefill<__half, 128>(qm, km, vm, p, st))
+                          : (bf ? frc::launch_prefill<__nv_bfloat16, 64>(qm, km, vm, p, st)
+                                : frc::launch_prefill<__half, 64>(qm, km, vm, p, st))),
+               "attention_prefill launch");
+  return FRC_OK;
 }

@@ -823,19 +823,25 @@ __global__ void __launch_bounds__(kAqJoin) attn_q4_join_kernel(const AttnQ4Param
   }
 }
 
-__device__ uint32_t g_serving_status;
+static __device__ uint32_t g_serving_status;
+
+cudaError_t serving_status(uint32_t** word) {
+  static std::atomic<uint32_t*> known[64];  // by device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  *word = dev < 64 ? known[dev].load() : nullptr;
+  if (*word) return cudaSuccess;
+  e = cudaGetSymbolAddress(reinterpret_cast<void**>(word), g_serving_status);
+  if (e == cudaSuccess && dev < 64) known[dev].store(*word);
+  return e;
+}
 
 template <typename T, int HD>
 cudaError_t launch_attn_q4(AttnQ4Params p, int grid, cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};  // devices on which the kernel may use its shared memory
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  cudaError_t e = allow_smem(attn_q4_kernel<T, HD>, sizeof(AqSmem<HD>), ready);
   if (e != cudaSuccess) return e;
-  if (dev >= 64 || !(ready.load() >> dev & 1)) {
-    e = cudaFuncSetAttribute(attn_q4_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(AqSmem<HD>));
-    if (e != cudaSuccess) return e;
-    if (dev < 64) ready.fetch_or(uint64_t(1) << dev);
-  }
   e = launch_pdl(attn_q4_kernel<T, HD>, dim3(grid), dim3(kAqThreads), sizeof(AqSmem<HD>), st, p);
   if (e != cudaSuccess || grid == 1) return e;
   return launch_pdl(attn_q4_join_kernel<T, HD>, dim3(grid, min(kAqHeads, p.nh / p.nkv)), dim3(kAqJoin), 0, st, p);
@@ -891,9 +897,8 @@ int frc_attention_decode_q4(int type, const void* q, int64_t q_seq_stride, int64
   FRC_REQUIRE(most / grid < (int64_t(1) << 30), "frc_attention_decode_q4: block table too large");
   const size_t es = type == FRC_F32 ? 4 : 2;
   const int run = type == FRC_F32 ? 4 : 8;  // elements of a 16-byte load
-  void* status = nullptr;
-  FRC_LAUNCHED(cudaGetSymbolAddress(&status, frc::g_serving_status), "cudaGetSymbolAddress(status word)");
   frc::AttnQ4Params p{};
+  FRC_LAUNCHED(frc::serving_status(&p.status), "status word");
   p.q = q;
   p.q_seq = q_seq_stride;
   p.q_head = q_head_stride;
@@ -917,7 +922,6 @@ int frc_attention_decode_q4(int type, const void* q, int64_t q_seq_stride, int64
   p.part = static_cast<float*>(workspace);
   p.first = p.part + static_cast<size_t>(frc::kAqGrid) * 2 * frc::kAqHeads * (hd + 4);
   p.desc = reinterpret_cast<int4*>(p.first + static_cast<size_t>(frc::kAqGrid) * frc::kAqWarps * frc::kAqHeads * (hd + 4));
-  p.status = static_cast<uint32_t*>(status);
   p.bias = 0x64006400u;
   return frc_with_type(type, [&](auto* z) -> int {
     using T = std::remove_pointer_t<decltype(z)>;

@@ -52,6 +52,10 @@ struct frc_weight {
   uint8_t* dev;
 };
 
+namespace frc {
+cudaError_t serving_status(uint32_t** word);  // attn_q4.cu: the serving kernels' own status word
+}
+
 namespace {
 
 constexpr int kMaxGemvBatch = 16;
@@ -626,6 +630,12 @@ int frc_device_status(int device, uint32_t* flags) {
   FRC_CUDA(cudaDeviceSynchronize(), "cudaDeviceSynchronize");
   FRC_CUDA(cudaMemcpy(flags, ds->status, sizeof(uint32_t), cudaMemcpyDeviceToHost), "status read");
   FRC_CUDA(cudaMemset(ds->status, 0, sizeof(uint32_t)), "status clear");
+  uint32_t* serving = nullptr;
+  uint32_t more = 0;
+  FRC_CUDA(frc::serving_status(&serving), "serving status word");
+  FRC_CUDA(cudaMemcpy(&more, serving, sizeof(uint32_t), cudaMemcpyDeviceToHost), "status read");
+  FRC_CUDA(cudaMemset(serving, 0, sizeof(uint32_t)), "status clear");
+  *flags |= more;
   return FRC_OK;
 }
 

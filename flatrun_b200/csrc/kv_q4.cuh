@@ -26,6 +26,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "frc_common.cuh"
@@ -128,6 +129,23 @@ inline cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
+
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device,
+// once a device.
+template <typename K>
+inline cudaError_t allow_smem(K kernel, size_t bytes, std::atomic<uint64_t>& ready) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && (ready.load() >> dev & 1)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (e == cudaSuccess && dev < 64) ready.fetch_or(uint64_t(1) << dev);
+  return e;
+}
+
+// Address of the serving kernels' status word on the current device
+// (attn_q4.cu): bits of bounded waits that ran out, read by frc_device_status.
+cudaError_t serving_status(uint32_t** word);
 
 inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
