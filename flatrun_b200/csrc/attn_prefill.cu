@@ -66,7 +66,13 @@ struct PrefillParams {
 
 constexpr int kPfRows = 128;     // queries of a tile, keys of a tile
 constexpr int kPfTiles = 2;      // query tiles of a CTA
-constexpr int kPfThreads = 320;
+constexpr int kPfThreads = 384;
+// Registers: the CTA is launched with 168 a thread; the softmax warps, which
+// hold a row of scores, take over what the other four warps leave (two of
+// them are there for that alone): 2 * 216 + 72 = 3 * 168.
+constexpr int kPfRegsSoftmax = 216, kPfRegsOther = 72;
+constexpr int kPfPoly = 4;        // one pair of exponentials in this many is a polynomial
+constexpr int kPfFirst = 96;     // keys whose P is handed over before the rest
 constexpr float kPfSlack = 8.f;  // powers of two that the reference may stay behind
 
 template <int HD>
@@ -77,7 +83,7 @@ struct PfSmem {
   alignas(1024) uint8_t q[kPfTiles][kTile];
   alignas(1024) uint8_t ring[kStages][kTile];
   uint64_t q_full, full[kStages], empty[kStages];
-  uint64_t s_full[kPfTiles], p_ready[kPfTiles], o_done[kPfTiles], drain;
+  uint64_t s_full[kPfTiles], p_ready[kPfTiles][2], o_done[kPfTiles], drain;
   uint32_t tmem;
   int abort;
 };
@@ -100,27 +106,46 @@ __host__ __device__ constexpr uint32_t pf_idesc(int n, bool b_mn_major) {
 }
 constexpr uint32_t kPfNegateA = 1u << 13;
 
-// D (tensor memory) (+)= A (shared) B (shared)
-FRC_DEVICE_INLINE void pf_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// One lane of the warp, the same each time.
+FRC_DEVICE_INLINE uint32_t pf_elect() {
+  uint32_t one;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one;
+}
+
+// The whole warp calls these, with the same operands in all lanes (so that they
+// stay in uniform registers, which the instructions read); the elected lane issues.
+// D (tensor memory) (+)= A (shared) B (shared)
+FRC_DEVICE_INLINE void pf_mma_ss(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one)
       : "memory");
 }
 // D (tensor memory) (+)= A (tensor memory) B (shared)
-FRC_DEVICE_INLINE void pf_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+FRC_DEVICE_INLINE void pf_mma_ts(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one)
       : "memory");
 }
-FRC_DEVICE_INLINE void pf_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+FRC_DEVICE_INLINE void pf_commit(uint32_t one, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(one)
+      : "memory");
 }
 FRC_DEVICE_INLINE void pf_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 FRC_DEVICE_INLINE void pf_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -136,11 +161,16 @@ FRC_DEVICE_INLINE void tmem_ld32(uint32_t addr, uint32_t* r) {
       : FRC_R8(r, 0), FRC_R8(r, 8), FRC_R8(r, 16), FRC_R8(r, 24)
       : "r"(addr));
 }
-FRC_DEVICE_INLINE void tmem_st32(uint32_t addr, const uint32_t* r) {
+FRC_DEVICE_INLINE void tmem_ld16u(uint32_t addr, uint32_t* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::FRC_I8(r, 0), FRC_I8(r, 8), FRC_I8(r, 16),
-      FRC_I8(r, 24), "r"(addr)
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : FRC_R8(r, 0), FRC_R8(r, 8)
+      : "r"(addr));
+}
+FRC_DEVICE_INLINE void tmem_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::FRC_I8(r, 0),
+      FRC_I8(r, 8), "r"(addr)
       : "memory");
 }
 FRC_DEVICE_INLINE void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -189,6 +219,61 @@ FRC_DEVICE_INLINE uint64_t pf_add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+
+// The larger of two values, NaN if one is.
+FRC_DEVICE_INLINE float pf_max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+constexpr float kPfC1 = 0.6931241750717163f, kPfC2 = 0.24024099111557007f, kPfC3 = 0.05590642988681793f,
+                kPfC4 = 0.009582855738699436f;
+
+// exp2 of two values on the multiply-add units: with x = n + f, n whole and f
+// in [-1/2, 1/2], 2^n goes into the exponent and 2^f is 1 + f (c1 + c2 f + c3 f^2 +
+// c4 f^3), whose coefficients make the largest relative error least (2.9e-6, a
+// hundredth of fp16's rounding of P).  Below -127: exactly 0.  NaN gives a value
+// that rounds to infinity in either type, so its row comes out not finite.
+FRC_DEVICE_INLINE void pf_ex2_poly(uint64_t x, float& a, float& b) {
+  float x0, x1;
+  pf_split(x, x0, x1);
+  x = pf_two(pf_max_nan(x0, -127.f), pf_max_nan(x1, -127.f));
+  const uint64_t t = pf_add2(x, pf_two(12582912.f, 12582912.f));  // 1.5 * 2^23: n in the low bits
+  const uint64_t n = pf_add2(t, pf_two(-12582912.f, -12582912.f));
+  const uint64_t f = pf_fma2(n, pf_two(-1.f, -1.f), x);
+  uint64_t y = pf_fma2(f, pf_two(kPfC4, kPfC4), pf_two(kPfC3, kPfC3));
+  y = pf_fma2(y, f, pf_two(kPfC2, kPfC2));
+  y = pf_fma2(y, f, pf_two(kPfC1, kPfC1));
+  y = pf_fma2(y, f, pf_two(1.f, 1.f));
+  float t0, t1;
+  pf_split(t, t0, t1);
+  pf_split(y, a, b);
+  a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t0) << 23));
+  b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
+}
+
+// P of 32 scores: 2^(x scale + base), their sums, and the values rounded and
+// packed.  One pair in kPfPoly goes to the multiply-add units, the others to the
+// special-function unit, which alone would take as long as the products.
+template <typename T>
+FRC_DEVICE_INLINE void pf_exps(const uint32_t* x, uint64_t scale2, float base, uint64_t (&part)[4], uint32_t (&y)[16]) {
+  const uint64_t base2 = pf_two(base, base);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const uint64_t v = pf_fma2(pf_two(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), scale2, base2);
+    float a, b;
+    if (e % kPfPoly == kPfPoly - 1) {
+      pf_ex2_poly(v, a, b);
+    } else {
+      pf_split(v, a, b);
+      a = pf_ex2(a);
+      b = pf_ex2(b);
+    }
+    part[e & 3] = pf_add2(part[e & 3], pf_two(a, b));
+    y[e] = pf_pack<T>(a, b);
+  }
 }
 
 // The rows of a CTA.
@@ -285,7 +370,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   constexpr int NS = SM::kStages, H = HD / 64;
   extern __shared__ __align__(1024) uint8_t pf_smem[];
   SM* sh = reinterpret_cast<SM*>(pf_smem);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   PfWork w;
   w.head = blockIdx.x % p.nh;
   if (!w.find(p, blockIdx.x / p.nh, lane)) return;  // the same in all threads
@@ -303,7 +388,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     }
     for (int t = 0; t < kPfTiles; ++t) {
       mbar_init(&sh->s_full[t], 1);
-      mbar_init(&sh->p_ready[t], 4);
+      mbar_init(&sh->p_ready[t][0], 4);
+      mbar_init(&sh->p_ready[t][1], 4);
       mbar_init(&sh->o_done[t], 1);
     }
     mbar_init(&sh->drain, 1);
@@ -320,6 +406,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   const uint32_t tmem = sh->tmem;  // S of tile t at column 128 t, O at 256 + HD t
   volatile int* abort = &sh->abort;
 
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPfRegsOther));
   if (warp == 9) {
     // ---- loads -----------------------------------------------------------------------
     if (lane == 0 && n > 0) {
@@ -356,30 +444,26 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       auto wait = [&](uint64_t* bar, uint32_t parity) {
         return __all_sync(0xffffffffu, wait_phase(bar, parity & 1, abort));
       };
+      const uint32_t one = pf_elect();
+      const uint64_t q_desc = pf_desc(smem_u32(sh->q[0]), 16);
+      const uint64_t k_desc = pf_desc(smem_u32(sh->ring[0]), 16), v_desc = pf_desc(smem_u32(sh->ring[0]), SM::kHalf);
       auto qk = [&](int t, int stage) {
-        if (lane == 0) {
-          const uint32_t a = smem_u32(sh->q[t]), b = smem_u32(sh->ring[stage]);
+        const uint64_t a = q_desc + t * (SM::kTile >> 4), b = k_desc + stage * (SM::kTile >> 4);
 #pragma unroll
-          for (int k = 0; k < HD / 16; ++k) {
-            const uint32_t off = k / 4 * SM::kHalf + k % 4 * 32;
-            pf_mma_ss(tmem + 128 * t, pf_desc(a + off, 16), pf_desc(b + off, 16), id_qk, k > 0);
-          }
-          pf_commit(&sh->s_full[t]);
+        for (int k = 0; k < HD / 16; ++k) {
+          constexpr int kStep = 32 >> 4;
+          const int off = k / 4 * (SM::kHalf >> 4) + k % 4 * kStep;
+          pf_mma_ss(one, tmem + 128 * t, a + off, b + off, id_qk, k > 0);
         }
+        pf_commit(one, &sh->s_full[t]);
       };
-      auto pv = [&](int t, int stage, bool first) {
-        if (lane == 0) {
-          const uint32_t b = smem_u32(sh->ring[stage]);
+      auto pv = [&](int t, int stage, auto k0, auto k1, bool first) {
+        const uint64_t b = v_desc + stage * (SM::kTile >> 4);
 #pragma unroll
-          for (int k = 0; k < kPfRows / 16; ++k)
-            pf_mma_ts(tmem + 256 + HD * t, tmem + 128 * t + 8 * k, pf_desc(b + k * 2048, SM::kHalf), id_pv,
-                      !first || k > 0);
-          pf_commit(&sh->o_done[t]);
-        }
+        for (int k = k0(); k < k1(); ++k)
+          pf_mma_ts(one, tmem + 256 + HD * t, tmem + 128 * t + 8 * k, b + k * (2048 >> 4), id_pv, !first || k > 0);
       };
-      auto release = [&](int stage) {
-        if (lane == 0) pf_commit(&sh->empty[stage]);
-      };
+      auto release = [&](int stage) { pf_commit(one, &sh->empty[stage]); };
       bool ok = wait(&sh->q_full, 0) && wait(&sh->full[0], 0);
       if (ok) {
         pf_fence_after();
@@ -404,10 +488,15 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         for (int t = 0; t < kPfTiles; ++t) {
           const int nt = t ? n1 : n0;
           if (j >= nt) continue;
-          ok = ok && wait(&sh->p_ready[t], j);
+          ok = ok && wait(&sh->p_ready[t][0], j);
           if (!ok) break;
           pf_fence_after();
-          pv(t, sv, j == 0);
+          pv(t, sv, [] { return 0; }, [] { return kPfFirst / 16; }, j == 0);
+          ok = wait(&sh->p_ready[t][1], j);
+          if (!ok) break;
+          pf_fence_after();
+          pv(t, sv, [] { return kPfFirst / 16; }, [] { return kPfRows / 16; }, false);
+          pf_commit(one, &sh->o_done[t]);
           if (j + 1 < nt) {
             if (!k_there) ok = wait(&sh->full[sk], ik / NS);
             if (!ok) break;
@@ -425,13 +514,13 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         *abort = 1;
       }
       // no product may be in flight at the teardown
-      if (lane == 0) {
-        pf_commit(&sh->drain);
-        int zero = 0;
-        if (!wait_phase(&sh->drain, 0, &zero)) atomicOr(p.status, kStatusDrainTimeout);
-      }
+      pf_commit(one, &sh->drain);
+      int zero = 0;
+      if (!wait_phase(&sh->drain, 0, &zero) && lane == 0) atomicOr(p.status, kStatusDrainTimeout);
     }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPfRegsSoftmax));
     // ---- softmax: warps 4 t .. 4 t + 3 have tile t, a row a thread ------------------------
     const int t = warp >> 2, nt = t ? n1 : n0;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
@@ -440,7 +529,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     const bool live = r < w.rows(t);
     const int seen = live ? w.seen(p, row) : 0;
     const float scale = p.scale;
-    float m_ref = -INFINITY, sum = 0.f;  // reference in units of the unscaled score
+    float m_ref = -INFINITY, base = 0.f, sum = 0.f;  // reference in units of the unscaled score, and scaled
     bool ok = true;
     for (int j = 0; j < nt; ++j) {
       ok = __all_sync(0xffffffffu, wait_phase(&sh->s_full[t], j & 1, abort));
@@ -455,6 +544,12 @@ __global__ void __launch_bounds__(kPfThreads, 1)
 #pragma unroll
         for (int c = 0; c < kPfRows; ++c) x[c] = c < mine ? x[c] : 0xff800000u;
       }
+      // the first quarter's exponentials run with the old reference while the
+      // maximum is formed, and again in the few tiles that raise it
+      const uint64_t scale2 = pf_two(scale, scale);
+      uint64_t part[4] = {0, 0, 0, 0};
+      uint32_t y[16];
+      pf_exps<T>(x, scale2, base, part, y);
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int c = 0; c < kPfRows; c += 8)
@@ -466,47 +561,45 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         const float m_new = fmaxf(m, m_ref);
         const float keep = m_new == -INFINITY ? 1.f : pf_ex2((m_ref - m_new) * scale);
         m_ref = m_new;
+        base = m_new == -INFINITY ? 0.f : -m_new * scale;
         sum *= keep;
         if (j > 0) {
           ok = __all_sync(0xffffffffu, wait_phase(&sh->o_done[t], (j - 1) & 1, abort));
           if (!ok) break;
           pf_fence_after();
-#pragma unroll
-          for (int c = 0; c < HD; c += 32) {
-            uint32_t o[32];
-            tmem_ld32(o_at + c, o);
+#pragma unroll 1
+          for (int c = 0; c < HD; c += 16) {
+            uint32_t o[16];
+            tmem_ld16u(o_at + c, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-            tmem_st32(o_at + c, o);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+            tmem_st16(o_at + c, o);
           }
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[e] = 0;
+        pf_exps<T>(x, scale2, base, part, y);
       }
-      const float base = m_ref == -INFINITY ? 0.f : -m_ref * scale;
-      const uint64_t scale2 = pf_two(scale, scale), base2 = pf_two(base, base);
-      uint64_t part[4] = {0, 0, 0, 0};
+      tmem_st16(s_at, y);
 #pragma unroll
-      for (int c = 0; c < kPfRows; c += 64) {
-        uint32_t y[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const int i = c + 2 * e;
-          float a, b;
-          pf_split(pf_fma2(pf_two(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, base2), a, b);
-          a = pf_ex2(a);
-          b = pf_ex2(b);
-          part[e & 3] = pf_add2(part[e & 3], pf_two(a, b));
-          y[e] = pf_pack<T>(a, b);
+      for (int c = 32; c < kPfRows; c += 32) {
+        pf_exps<T>(x + c, scale2, base, part, y);
+        tmem_st16(s_at + c / 2, y);
+        if (c == kPfFirst - 32) {  // P's first part can be multiplied
+          tmem_wait_st();
+          pf_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->p_ready[t][0]);
         }
-        tmem_st32(s_at + c / 2, y);
       }
-      float a0, a1;
-      pf_split(pf_add2(pf_add2(part[0], part[1]), pf_add2(part[2], part[3])), a0, a1);
-      sum += a0 + a1;
       tmem_wait_st();
       pf_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->p_ready[t]);
+      if (lane == 0) mbar_arrive(&sh->p_ready[t][1]);
+      float a0, a1;
+      pf_split(pf_add2(pf_add2(part[0], part[1]), pf_add2(part[2], part[3])), a0, a1);
+      sum += a0 + a1;
     }
     // ---- O / sum ---------------------------------------------------------------------
     if (ok && nt > 0) ok = __all_sync(0xffffffffu, wait_phase(&sh->o_done[t], (nt - 1) & 1, abort));
