@@ -60,7 +60,6 @@ struct PrefillParams {
   int q_blocks;
   void* out;
   int64_t o_tok, o_head;
-  int o_vec;
   uint32_t* status;
 };
 
@@ -82,8 +81,10 @@ struct PfSmem {
   static constexpr int kStages = HD == 128 ? 5 : 8;
   alignas(1024) uint8_t q[kPfTiles][kTile];
   alignas(1024) uint8_t ring[kStages][kTile];
-  uint64_t q_full, full[kStages], empty[kStages];
-  uint64_t s_full[kPfTiles], p_ready[kPfTiles][2], o_done[kPfTiles], drain;
+  uint64_t q_full, q_empty, full[kStages], empty[kStages];
+  uint64_t s_full[kPfTiles], p_ready[kPfTiles][2], o_done[kPfTiles], o_free[kPfTiles], drain;
+  alignas(16) uint4 next[2];  // answers to the requests for the next item, by turns
+  uint64_t next_full[2], next_empty[2];
   uint32_t tmem;
   int abort;
 };
@@ -221,6 +222,12 @@ FRC_DEVICE_INLINE uint64_t pf_add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+FRC_DEVICE_INLINE float pf_max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
 // The larger of two values, NaN if one is.
 FRC_DEVICE_INLINE float pf_max_nan(float a, float b) {
   float y;
@@ -274,6 +281,32 @@ FRC_DEVICE_INLINE void pf_exps(const uint32_t* x, uint64_t scale2, float base, u
     part[e & 3] = pf_add2(part[e & 3], pf_two(a, b));
     y[e] = pf_pack<T>(a, b);
   }
+}
+
+// Asks for a block of the grid that has not started; the answer (16 bytes)
+// arrives on `bar`.
+FRC_DEVICE_INLINE void pf_ask(uint4* answer, uint64_t* bar) {
+  mbar_arrive_expect_tx(bar, 16);
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+          smem_u32(answer)),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+// Its index, or -1 where none is left.
+FRC_DEVICE_INLINE int pf_answer(const uint4* answer) {
+  int block;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
+      "ld.shared.b128 r, [%1];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "mov.b32 %0, -1;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, r;\n\t}"
+      : "=r"(block)
+      : "r"(smem_u32(answer))
+      : "memory");
+  fence_proxy_async_smem();  // before the next answer is written over it
+  return block;
 }
 
 // The rows of a CTA.
@@ -365,23 +398,18 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap vmap, const PrefillParams p) {
   griddep_wait();
-  griddep_launch_dependents();
   using SM = PfSmem<HD>;
   constexpr int NS = SM::kStages, H = HD / 64;
   extern __shared__ __align__(1024) uint8_t pf_smem[];
   SM* sh = reinterpret_cast<SM*>(pf_smem);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  PfWork w;
-  w.head = blockIdx.x % p.nh;
-  if (!w.find(p, blockIdx.x / p.nh, lane)) return;  // the same in all threads
-  const int n0 = w.tiles(p, 0), n1 = w.tiles(p, 1), n = max(n0, n1);
-  const int kvh = w.head / (p.nh / p.nkv);
   if (smem_u32(pf_smem) & 1023u) {  // swizzled tiles need 1024-byte alignment
     if (threadIdx.x == 0) atomicOr(p.status, kStatusSmemMisaligned);
     return;
   }
   if (threadIdx.x == 0) {
     mbar_init(&sh->q_full, 1);
+    mbar_init(&sh->q_empty, 1);
     for (int s = 0; s < NS; ++s) {
       mbar_init(&sh->full[s], 1);
       mbar_init(&sh->empty[s], 1);
@@ -391,6 +419,9 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       mbar_init(&sh->p_ready[t][0], 4);
       mbar_init(&sh->p_ready[t][1], 4);
       mbar_init(&sh->o_done[t], 1);
+      mbar_init(&sh->o_free[t], 4);
+      mbar_init(&sh->next_full[t], 1);
+      mbar_init(&sh->next_empty[t], 9);  // the softmax warps and the product warp
     }
     mbar_init(&sh->drain, 1);
     sh->abort = 0;
@@ -405,45 +436,76 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   pf_fence_after();
   const uint32_t tmem = sh->tmem;  // S of tile t at column 128 t, O at 256 + HD t
   volatile int* abort = &sh->abort;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {  // a warp's bounded wait
+    return __all_sync(0xffffffffu, wait_phase(bar, parity & 1, abort));
+  };
+  // Item `i` of this CTA: the block it was launched as, then those it took over.
+  PfWork w;
+  int block = blockIdx.x;
+  auto open = [&] {  // false: none, nor any behind it
+    w.head = block % p.nh;
+    return w.find(p, block / p.nh, lane);
+  };
 
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPfRegsOther));
-  if (warp == 9) {
-    // ---- loads -----------------------------------------------------------------------
-    if (lane == 0 && n > 0) {
-      const int q_tiles = w.rows(1) > 0 ? 2 : 1;
-      mbar_arrive_expect_tx(&sh->q_full, q_tiles * SM::kTile);
-      for (int t = 0; t < q_tiles; ++t)
-        for (int h = 0; h < H; ++h)
-          pf_load_3d(sh->q[t] + h * SM::kHalf, &qmap, 64 * h, w.head * p.q_mul, w.q_start + w.q0 + t * kPfRows,
-                     &sh->q_full);
-      int issued = 0;
-      for (; issued < 2 * n; ++issued) {  // K 0, V 0, K 1, V 1, ...
-        const int s = issued % NS;
-        if (issued >= NS && !wait_phase(&sh->empty[s], (issued / NS - 1) & 1, abort)) {
-          atomicOr(p.status, kStatusEmptyWaitTimeout);
-          break;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPfRegsOther));
+    if (warp == 9) {
+      // ---- loads -----------------------------------------------------------------------
+      int issued = 0, items = 0;  // K and V tiles, items that had queries
+      bool ok = true;
+      for (int i = 0;; ++i) {
+        // the request for item i + 1, when the answer before the last has been read
+        if (i >= 2) ok = wait(&sh->next_empty[i & 1], (i >> 1) - 1) && ok;
+        if (!ok) break;
+        if (lane == 0) pf_ask(&sh->next[i & 1], &sh->next_full[i & 1]);
+        const bool any = open();
+        const int n = any ? max(w.tiles(p, 0), w.tiles(p, 1)) : 0;
+        const int kvh = w.head / (p.nh / p.nkv);
+        if (n > 0) {
+          if (items > 0) ok = wait(&sh->q_empty, items - 1);
+          if (ok && lane == 0) {
+            const int q_tiles = w.rows(1) > 0 ? 2 : 1;
+            mbar_arrive_expect_tx(&sh->q_full, q_tiles * SM::kTile);
+            for (int t = 0; t < q_tiles; ++t)
+              for (int h = 0; h < H; ++h)
+                pf_load_3d(sh->q[t] + h * SM::kHalf, &qmap, 64 * h, w.head * p.q_mul, w.q_start + w.q0 + t * kPfRows,
+                           &sh->q_full);
+          }
+          if (ok) ++items;
+          for (int l = 0; ok && l < 2 * n; ++l) {  // K 0, V 0, K 1, V 1, ...
+            const int s = issued % NS;
+            if (issued >= NS) ok = wait(&sh->empty[s], issued / NS - 1);
+            if (!ok) break;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&sh->full[s], SM::kTile);
+              const int key = w.k_start + (l >> 1) * kPfRows;
+              for (int h = 0; h < H; ++h)
+                pf_load_3d(sh->ring[s] + h * SM::kHalf, l & 1 ? &vmap : &kmap, 64 * h,
+                           kvh * (l & 1 ? p.v_mul : p.k_mul), key, &sh->full[s]);
+            }
+            ++issued;
+          }
         }
-        mbar_arrive_expect_tx(&sh->full[s], SM::kTile);
-        const int key = w.k_start + (issued >> 1) * kPfRows;
-        for (int h = 0; h < H; ++h)
-          pf_load_3d(sh->ring[s] + h * SM::kHalf, issued & 1 ? &vmap : &kmap, 64 * h,
-                     kvh * (issued & 1 ? p.v_mul : p.k_mul), key, &sh->full[s]);
+        // the answer is waited for in any case: it must not land after the CTA
+        int zero = 0;
+        ok = __all_sync(0xffffffffu, wait_phase(&sh->next_full[i & 1], (i >> 1) & 1, &zero)) && ok;
+        block = pf_answer(&sh->next[i & 1]);
+        if (!ok || !any || block < 0) break;
+      }
+      if (!ok) {
+        *abort = 1;
+        if (lane == 0) atomicOr(p.status, kStatusEmptyWaitTimeout);
       }
       // no copy may still be landing when the CTA exits
       int zero = 0;
-      bool ok = wait_phase(&sh->q_full, 0, &zero);
-      for (int i = issued > NS ? issued - NS : 0; i < issued; ++i) ok = wait_phase(&sh->full[i % NS], (i / NS) & 1, &zero) && ok;
-      if (!ok) atomicOr(p.status, kStatusDrainTimeout);
-    }
-  } else if (warp == 8) {
-    // ---- products: one thread issues, the warp waits -------------------------------------
-    if (n > 0) {
+      bool landed = items == 0 || wait_phase(&sh->q_full, (items - 1) & 1, &zero);
+      for (int l = issued > NS ? issued - NS : 0; l < issued; ++l)
+        landed = wait_phase(&sh->full[l % NS], (l / NS) & 1, &zero) && landed;
+      if (!landed && lane == 0) atomicOr(p.status, kStatusDrainTimeout);
+    } else if (warp == 8) {
+      // ---- products: the elected lane issues -----------------------------------------------
       constexpr uint32_t id_pv = pf_idesc<T>(HD, true);
       const uint32_t id_qk = pf_idesc<T>(kPfRows, false) | (p.negate ? kPfNegateA : 0u);
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        return __all_sync(0xffffffffu, wait_phase(bar, parity & 1, abort));
-      };
       const uint32_t one = pf_elect();
       const uint64_t q_desc = pf_desc(smem_u32(sh->q[0]), 16);
       const uint64_t k_desc = pf_desc(smem_u32(sh->ring[0]), 16), v_desc = pf_desc(smem_u32(sh->ring[0]), SM::kHalf);
@@ -451,8 +513,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         const uint64_t a = q_desc + t * (SM::kTile >> 4), b = k_desc + stage * (SM::kTile >> 4);
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
-          constexpr int kStep = 32 >> 4;
-          const int off = k / 4 * (SM::kHalf >> 4) + k % 4 * kStep;
+          const int off = k / 4 * (SM::kHalf >> 4) + k % 4 * (32 >> 4);
           pf_mma_ss(one, tmem + 128 * t, a + off, b + off, id_qk, k > 0);
         }
         pf_commit(one, &sh->s_full[t]);
@@ -464,148 +525,176 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           pf_mma_ts(one, tmem + 256 + HD * t, tmem + 128 * t + 8 * k, b + k * (2048 >> 4), id_pv, !first || k > 0);
       };
       auto release = [&](int stage) { pf_commit(one, &sh->empty[stage]); };
-      bool ok = wait(&sh->q_full, 0) && wait(&sh->full[0], 0);
-      if (ok) {
-        pf_fence_after();
-        if (n0 > 0) qk(0, 0);
-        if (n1 > 0) qk(1, 0);
-        release(0);
-      }
-      for (int j = 0; ok && j < n; ++j) {
-        const int iv = 2 * j + 1, sv = iv % NS, ik = 2 * j + 2, sk = ik % NS;
-        ok = wait(&sh->full[sv], iv / NS);
-        if (!ok) break;
-        const int left = w.k_len - j * kPfRows;
-        if (left < kPfRows) {  // rows behind the last key: zeros, whatever lies there
-          uint4* row = reinterpret_cast<uint4*>(sh->ring[sv]);
-          for (int h = 0; h < H; ++h)
-            for (int i = left * 8 + lane; i < kPfRows * 8; i += 32) row[h * (SM::kHalf / 16) + i] = make_uint4(0, 0, 0, 0);
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-        }
-        bool k_there = false;
-#pragma unroll
-        for (int t = 0; t < kPfTiles; ++t) {
-          const int nt = t ? n1 : n0;
-          if (j >= nt) continue;
-          ok = ok && wait(&sh->p_ready[t][0], j);
+      bool ok = true;
+      int used = 0, items = 0;                           // K and V tiles, items that had queries
+      int done[kPfTiles] = {0, 0}, outs[kPfTiles] = {0, 0};  // key tiles and items of each query tile
+      for (int i = 0; ok; ++i) {
+        const bool any = open();
+        const int nt[kPfTiles] = {any ? w.tiles(p, 0) : 0, any ? w.tiles(p, 1) : 0};
+        const int n = max(nt[0], nt[1]);
+        if (n > 0) {
+          ok = wait(&sh->q_full, items) && wait(&sh->full[used % NS], used / NS);
           if (!ok) break;
+          ++items;
           pf_fence_after();
-          pv(t, sv, [] { return 0; }, [] { return kPfFirst / 16; }, j == 0);
-          ok = wait(&sh->p_ready[t][1], j);
-          if (!ok) break;
-          pf_fence_after();
-          pv(t, sv, [] { return kPfFirst / 16; }, [] { return kPfRows / 16; }, false);
-          pf_commit(one, &sh->o_done[t]);
-          if (j + 1 < nt) {
-            if (!k_there) ok = wait(&sh->full[sk], ik / NS);
+          for (int t = 0; t < kPfTiles; ++t)
+            if (nt[t] > 0) qk(t, used % NS);
+          release(used % NS);
+          if (n == 1) pf_commit(one, &sh->q_empty);
+          ++used;
+          for (int j = 0; ok && j < n; ++j) {
+            const int sv = used % NS, sk = (used + 1) % NS;
+            ok = wait(&sh->full[sv], used / NS);
             if (!ok) break;
-            k_there = true;
-            pf_fence_after();
-            qk(t, sk);
+            const int left = w.k_len - j * kPfRows;
+            if (left < kPfRows) {  // rows behind the last key: zeros, whatever lies there
+              uint4* row = reinterpret_cast<uint4*>(sh->ring[sv]);
+              for (int h = 0; h < H; ++h)
+                for (int e = left * 8 + lane; e < kPfRows * 8; e += 32)
+                  row[h * (SM::kHalf / 16) + e] = make_uint4(0, 0, 0, 0);
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+            }
+            bool k_there = false;
+#pragma unroll
+            for (int t = 0; t < kPfTiles; ++t) {
+              if (j >= nt[t]) continue;
+              // the last item's O has been read before it is overwritten
+              if (j == 0 && outs[t] > 0) ok = ok && wait(&sh->o_free[t], outs[t] - 1);
+              ok = ok && wait(&sh->p_ready[t][0], done[t]);
+              if (!ok) break;
+              pf_fence_after();
+              pv(t, sv, [] { return 0; }, [] { return kPfFirst / 16; }, j == 0);
+              ok = wait(&sh->p_ready[t][1], done[t]);
+              if (!ok) break;
+              pf_fence_after();
+              pv(t, sv, [] { return kPfFirst / 16; }, [] { return kPfRows / 16; }, false);
+              pf_commit(one, &sh->o_done[t]);
+              ++done[t];
+              if (j + 1 < nt[t]) {
+                if (!k_there) ok = wait(&sh->full[sk], (used + 1) / NS);
+                if (!ok) break;
+                k_there = true;
+                pf_fence_after();
+                qk(t, sk);
+              }
+            }
+            if (!ok) break;
+            release(sv);
+            ++used;
+            if (j + 1 < n) {
+              release(sk);
+              ++used;
+              if (j + 2 == n) pf_commit(one, &sh->q_empty);  // the queries' last use
+            }
           }
+          for (int t = 0; t < kPfTiles; ++t) outs[t] += nt[t] > 0;
         }
+        ok = ok && wait(&sh->next_full[i & 1], i >> 1);
         if (!ok) break;
-        release(sv);
-        if (j + 1 < n) release(sk);
+        block = pf_answer(&sh->next[i & 1]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->next_empty[i & 1]);
+        if (!any || block < 0) break;
       }
-      if (!ok && lane == 0) {
-        atomicOr(p.status, kStatusFullWaitTimeout);
+      if (!ok) {
         *abort = 1;
+        if (lane == 0) atomicOr(p.status, kStatusFullWaitTimeout);
       }
       // no product may be in flight at the teardown
       pf_commit(one, &sh->drain);
       int zero = 0;
       if (!wait_phase(&sh->drain, 0, &zero) && lane == 0) atomicOr(p.status, kStatusDrainTimeout);
     }
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPfRegsSoftmax));
     // ---- softmax: warps 4 t .. 4 t + 3 have tile t, a row a thread ------------------------
-    const int t = warp >> 2, nt = t ? n1 : n0;
+    const int t = warp >> 2;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t s_at = tmem + lanes + 128 * t, o_at = tmem + lanes + 256 + HD * t;
-    const int r = 32 * (warp & 3) + lane, row = w.q0 + kPfRows * t + r;
-    const bool live = r < w.rows(t);
-    const int seen = live ? w.seen(p, row) : 0;
+    const int r = 32 * (warp & 3) + lane;
     const float scale = p.scale;
-    float m_ref = -INFINITY, base = 0.f, sum = 0.f;  // reference in units of the unscaled score, and scaled
+    const uint64_t scale2 = pf_two(scale, scale);
     bool ok = true;
-    for (int j = 0; j < nt; ++j) {
-      ok = __all_sync(0xffffffffu, wait_phase(&sh->s_full[t], j & 1, abort));
-      if (!ok) break;
-      pf_fence_after();
-      uint32_t x[kPfRows];
+    int done = 0;  // key tiles
+    for (int i = 0; ok; ++i) {
+      const bool any = open();
+      const int nt = any ? w.tiles(p, t) : 0, row = w.q0 + kPfRows * t + r;
+      const bool live = any && r < w.rows(t);
+      const int seen = live ? w.seen(p, row) : 0;
+      float m_ref = -INFINITY, base = 0.f, sum = 0.f;  // reference in units of the unscaled score, and scaled
+      for (int j = 0; j < nt; ++j, ++done) {
+        ok = wait(&sh->s_full[t], done);
+        if (!ok) break;
+        pf_fence_after();
+        uint32_t x[kPfRows];
 #pragma unroll
-      for (int c = 0; c < kPfRows; c += 32) tmem_ld32(s_at + c, x + c);
-      tmem_wait_ld();
-      const int mine = seen - j * kPfRows;  // columns that the row sees
-      if (!__all_sync(0xffffffffu, mine >= kPfRows)) {
+        for (int c = 0; c < kPfRows; c += 32) tmem_ld32(s_at + c, x + c);
+        tmem_wait_ld();
+        const int mine = seen - j * kPfRows;  // columns that the row sees
+        if (!__all_sync(0xffffffffu, mine >= kPfRows)) {
 #pragma unroll
-        for (int c = 0; c < kPfRows; ++c) x[c] = c < mine ? x[c] : 0xff800000u;
-      }
-      // the first quarter's exponentials run with the old reference while the
-      // maximum is formed, and again in the few tiles that raise it
-      const uint64_t scale2 = pf_two(scale, scale);
-      uint64_t part[4] = {0, 0, 0, 0};
-      uint32_t y[16];
-      pf_exps<T>(x, scale2, base, part, y);
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          for (int c = 0; c < kPfRows; ++c) x[c] = c < mine ? x[c] : 0xff800000u;
+        }
+        // the first quarter's exponentials run with the old reference while the
+        // maximum is formed, and again in the few tiles that raise it
+        uint64_t part[4] = {0, 0, 0, 0};
+        uint32_t y[16];
+        pf_exps<T>(x, scale2, base, part, y);
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < kPfRows; c += 8)
+        for (int c = 0; c < kPfRows; c += 8)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1])));
-      const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      if (__any_sync(0xffffffffu, (m - m_ref) * scale > kPfSlack)) {
-        const float m_new = fmaxf(m, m_ref);
-        const float keep = m_new == -INFINITY ? 1.f : pf_ex2((m_ref - m_new) * scale);
-        m_ref = m_new;
-        base = m_new == -INFINITY ? 0.f : -m_new * scale;
-        sum *= keep;
-        if (j > 0) {
-          ok = __all_sync(0xffffffffu, wait_phase(&sh->o_done[t], (j - 1) & 1, abort));
-          if (!ok) break;
-          pf_fence_after();
+          for (int e = 0; e < 4; ++e)
+            mx[e] = pf_max3(mx[e], __uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1]));
+        const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        if (__any_sync(0xffffffffu, (m - m_ref) * scale > kPfSlack)) {
+          const float m_new = fmaxf(m, m_ref);
+          const float keep = m_new == -INFINITY ? 1.f : pf_ex2((m_ref - m_new) * scale);
+          m_ref = m_new;
+          base = m_new == -INFINITY ? 0.f : -m_new * scale;
+          sum *= keep;
+          if (j > 0) {
+            ok = wait(&sh->o_done[t], done - 1);
+            if (!ok) break;
+            pf_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < HD; c += 16) {
-            uint32_t o[16];
-            tmem_ld16u(o_at + c, o);
-            tmem_wait_ld();
+            for (int c = 0; c < HD; c += 16) {
+              uint32_t o[16];
+              tmem_ld16u(o_at + c, o);
+              tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-            tmem_st16(o_at + c, o);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+              tmem_st16(o_at + c, o);
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) part[e] = 0;
+          pf_exps<T>(x, scale2, base, part, y);
+        }
+        tmem_st16(s_at, y);
+#pragma unroll
+        for (int c = 32; c < kPfRows; c += 32) {
+          pf_exps<T>(x + c, scale2, base, part, y);
+          tmem_st16(s_at + c / 2, y);
+          if (c == kPfFirst - 32) {  // P's first part can be multiplied
+            tmem_wait_st();
+            pf_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->p_ready[t][0]);
           }
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) part[e] = 0;
-        pf_exps<T>(x, scale2, base, part, y);
+        tmem_wait_st();
+        pf_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->p_ready[t][1]);
+        float a0, a1;
+        pf_split(pf_add2(pf_add2(part[0], part[1]), pf_add2(part[2], part[3])), a0, a1);
+        sum += a0 + a1;
       }
-      tmem_st16(s_at, y);
-#pragma unroll
-      for (int c = 32; c < kPfRows; c += 32) {
-        pf_exps<T>(x + c, scale2, base, part, y);
-        tmem_st16(s_at + c / 2, y);
-        if (c == kPfFirst - 32) {  // P's first part can be multiplied
-          tmem_wait_st();
-          pf_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh->p_ready[t][0]);
-        }
-      }
-      tmem_wait_st();
-      pf_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->p_ready[t][1]);
-      float a0, a1;
-      pf_split(pf_add2(pf_add2(part[0], part[1]), pf_add2(part[2], part[3])), a0, a1);
-      sum += a0 + a1;
-    }
-    // ---- O / sum ---------------------------------------------------------------------
-    if (ok && nt > 0) ok = __all_sync(0xffffffffu, wait_phase(&sh->o_done[t], (nt - 1) & 1, abort));
-    if (!ok) {
-      if (lane == 0) atomicOr(p.status, kStatusFullWaitTimeout);
-    } else {
+      // ---- O / sum ---------------------------------------------------------------------
+      if (ok && nt > 0) ok = wait(&sh->o_done[t], done - 1);
+      if (!ok) break;
       pf_fence_after();
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       T* op = static_cast<T*>(p.out) + static_cast<int64_t>(w.q_start + row) * p.o_tok + w.head * p.o_head;
@@ -617,27 +706,33 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           uint32_t o[32];
           tmem_ld32(o_at + c, o);
           tmem_wait_ld();
+          if (c == HD - 32) {
+            pf_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->o_free[t]);
+          }
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            v[e] = __uint_as_float(o[e]) * inv;
+            v[e] = seen == 0 ? 0.f : __uint_as_float(o[e]) * inv;
             finite = finite && fabsf(v[e]) <= 3.402823466e38f;
           }
         } else {
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = 0.f;
         }
-        if (live) {
-          if (seen == 0)
-#pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = 0.f;
-          if (p.o_vec) store_run<32, true>(op + c, v);
-          else store_run<32, false>(op + c, v);
-        }
+        if (live) store_run<32, true>(op + c, v);
       }
       __syncwarp();
-      for (uint32_t again = __ballot_sync(0xffffffffu, live && seen > 0 && !finite); again; again &= again - 1)
+      for (uint32_t again = __ballot_sync(0xffffffffu, live && !finite); again; again &= again - 1)
         pf_row_again<T, HD>(p, w, w.q0 + kPfRows * t + 32 * (warp & 3) + __ffs(again) - 1, lane);
+      ok = wait(&sh->next_full[i & 1], i >> 1);
+      if (!ok) break;
+      block = pf_answer(&sh->next[i & 1]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->next_empty[i & 1]);
+      if (!any || block < 0) break;
     }
+    if (!ok && lane == 0) atomicOr(p.status, kStatusFullWaitTimeout);
   }
   // ---- teardown: every warp here, no product or tensor-memory access in flight -----------
   pf_fence_before();
@@ -734,7 +829,6 @@ extern "C" int frc_attention_prefill(int type, const void* q, int64_t q_tok_stri
   p.out = out;
   p.o_tok = out_tok_stride;
   p.o_head = out_head_stride;
-  p.o_vec = 1;
   FRC_LAUNCHED(frc::serving_status(&p.status), "status word");
   CUtensorMap qm, km, vm;
   const bool none = tokens_k == 0;  // no key is read: any valid map will do
