@@ -52,7 +52,8 @@ struct PrefillParams {
   int batch;
   int tokens_q, tokens_k;
   int nh, nkv;
-  int q_mul, k_mul, v_mul;  // 0: the heads are one (stride 0), 1: the map's second coordinate is the head
+  int heads, queries;       // query heads of a tile (of one KV head), and queries of each: heads * queries <= 128
+  int k_mul, v_mul;         // 0: the heads are one (stride 0), 1: the map's second coordinate is the head
   float scale;              // not negative; times log2 e
   float signed_scale;       // as given
   int negate;               // scale was negative: Q is negated in the product
@@ -63,15 +64,15 @@ struct PrefillParams {
   uint32_t* status;
 };
 
-constexpr int kPfRows = 128;     // queries of a tile, keys of a tile
+constexpr int kPfRows = 128;     // rows (queries of some heads) of a tile, keys of a tile
 constexpr int kPfTiles = 2;      // query tiles of a CTA
 constexpr int kPfThreads = 384;
 // Registers: the CTA is launched with 168 a thread; the softmax warps, which
 // hold a row of scores, take over what the other four warps leave (two of
 // them are there for that alone): 2 * 216 + 72 = 3 * 168.
 constexpr int kPfRegsSoftmax = 216, kPfRegsOther = 72;
-constexpr int kPfPoly = 4;        // one pair of exponentials in this many is a polynomial
-constexpr int kPfFirst = 96;     // keys whose P is handed over before the rest
+constexpr int kPfFirst = 64;     // keys whose P is handed over before the rest
+static_assert(kPfFirst % 32 == 0 && kPfFirst >= 64 && kPfFirst < kPfRows, "a multiple of 32 behind the first 32");
 constexpr float kPfSlack = 8.f;  // powers of two that the reference may stay behind
 
 template <int HD>
@@ -228,42 +229,10 @@ FRC_DEVICE_INLINE float pf_max3(float a, float b, float c) {
   return y;
 }
 
-// The larger of two values, NaN if one is.
-FRC_DEVICE_INLINE float pf_max_nan(float a, float b) {
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
-}
-
-constexpr float kPfC1 = 0.6931241750717163f, kPfC2 = 0.24024099111557007f, kPfC3 = 0.05590642988681793f,
-                kPfC4 = 0.009582855738699436f;
-
-// exp2 of two values on the multiply-add units: with x = n + f, n whole and f
-// in [-1/2, 1/2], 2^n goes into the exponent and 2^f is 1 + f (c1 + c2 f + c3 f^2 +
-// c4 f^3), whose coefficients make the largest relative error least (2.9e-6, a
-// hundredth of fp16's rounding of P).  Below -127: exactly 0.  NaN gives a value
-// that rounds to infinity in either type, so its row comes out not finite.
-FRC_DEVICE_INLINE void pf_ex2_poly(uint64_t x, float& a, float& b) {
-  float x0, x1;
-  pf_split(x, x0, x1);
-  x = pf_two(pf_max_nan(x0, -127.f), pf_max_nan(x1, -127.f));
-  const uint64_t t = pf_add2(x, pf_two(12582912.f, 12582912.f));  // 1.5 * 2^23: n in the low bits
-  const uint64_t n = pf_add2(t, pf_two(-12582912.f, -12582912.f));
-  const uint64_t f = pf_fma2(n, pf_two(-1.f, -1.f), x);
-  uint64_t y = pf_fma2(f, pf_two(kPfC4, kPfC4), pf_two(kPfC3, kPfC3));
-  y = pf_fma2(y, f, pf_two(kPfC2, kPfC2));
-  y = pf_fma2(y, f, pf_two(kPfC1, kPfC1));
-  y = pf_fma2(y, f, pf_two(1.f, 1.f));
-  float t0, t1;
-  pf_split(t, t0, t1);
-  pf_split(y, a, b);
-  a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t0) << 23));
-  b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
-}
-
 // P of 32 scores: 2^(x scale + base), their sums, and the values rounded and
-// packed.  One pair in kPfPoly goes to the multiply-add units, the others to the
-// special-function unit, which alone would take as long as the products.
+// packed.  (A quarter of the exponentials as polynomials on the multiply-add
+// units took a third more instructions and gained nothing: 1042 against 1016 us
+// for 64 heads of 8192 tokens.)
 template <typename T>
 FRC_DEVICE_INLINE void pf_exps(const uint32_t* x, uint64_t scale2, float base, uint64_t (&part)[4], uint32_t (&y)[16]) {
   const uint64_t base2 = pf_two(base, base);
@@ -271,13 +240,9 @@ FRC_DEVICE_INLINE void pf_exps(const uint32_t* x, uint64_t scale2, float base, u
   for (int e = 0; e < 16; ++e) {
     const uint64_t v = pf_fma2(pf_two(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), scale2, base2);
     float a, b;
-    if (e % kPfPoly == kPfPoly - 1) {
-      pf_ex2_poly(v, a, b);
-    } else {
-      pf_split(v, a, b);
-      a = pf_ex2(a);
-      b = pf_ex2(b);
-    }
+    pf_split(v, a, b);
+    a = pf_ex2(a);
+    b = pf_ex2(b);
     part[e & 3] = pf_add2(part[e & 3], pf_two(a, b));
     y[e] = pf_pack<T>(a, b);
   }
@@ -309,13 +274,20 @@ FRC_DEVICE_INLINE int pf_answer(const uint4* answer) {
   return block;
 }
 
-// The rows of a CTA.
+// A work item.
 struct PfWork {
-  int head, q_start, q_len, k_start, k_len;  // the sequence
-  int q0;                                    // first query of the CTA in it
-  // Block `rank` of the queries, from the last one on (the longest first where
-  // there is one sequence): all lanes of a warp call it.  False: there is none.
-  FRC_DEVICE_INLINE bool find(const PrefillParams& p, int rank, int lane) {
+  int head, kvh;                       // first query head, KV head
+  int q_start, q_len, k_start, k_len;  // the sequence
+  int q0;                              // first query of the item in it
+  // Item `block`: of its heads, block `block / units` of the queries, from the last
+  // one on (the longest first where there is one sequence).  All lanes of a warp
+  // call it.  False: there is none, nor any behind it.
+  FRC_DEVICE_INLINE bool find(const PrefillParams& p, int block, int lane) {
+    const int units = p.nh / p.heads;
+    int rank = block / units;
+    head = (block - rank * units) * p.heads;
+    kvh = head / (p.nh / p.nkv);
+    const int span = kPfTiles * p.queries;
     for (int top = p.batch; top > 0; top -= 32) {
       const int b = top - 1 - lane;
       int a0 = 0, a1 = 0;
@@ -323,7 +295,7 @@ struct PfWork {
         a0 = min(max(p.cu_q[b], 0), p.tokens_q);
         a1 = min(max(p.cu_q[b + 1], a0), p.tokens_q);
       }
-      const int n = (a1 - a0 + kPfTiles * kPfRows - 1) / (kPfTiles * kPfRows);
+      const int n = (a1 - a0 + span - 1) / span;
       int incl = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -340,7 +312,7 @@ struct PfWork {
       q_len = __shfl_sync(0xffffffffu, a1, l) - q_start;
       const int blocks = __shfl_sync(0xffffffffu, n, l);
       const int in_seq = rank - (__shfl_sync(0xffffffffu, incl, l) - blocks);
-      q0 = (blocks - 1 - in_seq) * kPfTiles * kPfRows;
+      q0 = (blocks - 1 - in_seq) * span;
       const int s = top - 1 - l;
       k_start = min(max(p.cu_k[s], 0), p.tokens_k);
       k_len = min(max(p.cu_k[s + 1], k_start), p.tokens_k) - k_start;
@@ -348,23 +320,26 @@ struct PfWork {
     }
     return false;
   }
-  FRC_DEVICE_INLINE int rows(int tile) const { return min(max(q_len - q0 - tile * kPfRows, 0), kPfRows); }
-  // Keys that query `row` of the sequence sees.
-  FRC_DEVICE_INLINE int seen(const PrefillParams& p, int row) const {
-    return p.causal ? min(max(row + 1 + k_len - q_len, 0), k_len) : k_len;
+  // Queries of a tile.
+  FRC_DEVICE_INLINE int queries(const PrefillParams& p, int tile) const {
+    return min(max(q_len - q0 - tile * p.queries, 0), p.queries);
+  }
+  // Keys that query `i` of the sequence sees.
+  FRC_DEVICE_INLINE int seen(const PrefillParams& p, int i) const {
+    return p.causal ? min(max(i + 1 + k_len - q_len, 0), k_len) : k_len;
   }
   // Key tiles of a query tile.
   FRC_DEVICE_INLINE int tiles(const PrefillParams& p, int tile) const {
-    const int n = rows(tile);
-    return n == 0 ? 0 : (seen(p, q0 + tile * kPfRows + n - 1) + kPfRows - 1) / kPfRows;
+    const int n = queries(p, tile);
+    return n == 0 ? 0 : (seen(p, q0 + tile * p.queries + n - 1) + kPfRows - 1) / kPfRows;
   }
 };
 
-// One row from the keys it sees alone: a warp, HD / 32 channels a lane.
+// Query `row` of head h from the keys it sees alone: a warp, HD / 32 channels a lane.
 template <typename T, int HD>
-__device__ __noinline__ void pf_row_again(const PrefillParams& p, const PfWork& w, int row, int lane) {
+__device__ __noinline__ void pf_row_again(const PrefillParams& p, const PfWork& w, int h, int row, int lane) {
   constexpr int C = HD / 32;
-  const int h = w.head, g = h / (p.nh / p.nkv);
+  const int g = w.kvh;
   const T* qp = static_cast<const T*>(p.q) + (w.q_start + row) * p.q_tok + h * p.q_head;
   float qv[C], acc[C];
 #pragma unroll
@@ -427,6 +402,12 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     sh->abort = 0;
     fence_barrier_init();
   }
+  // rows that no query is loaded to: zeros, so that they raise no reference
+  for (int t = 0; t < kPfTiles; ++t)
+    for (int h = 0; h < H; ++h)
+      for (int i = p.heads * p.queries * 8 + threadIdx.x; i < kPfRows * 8; i += kPfThreads)
+        reinterpret_cast<uint4*>(sh->q[t] + h * SM::kHalf)[i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
   if (warp == 8) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh->tmem)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -442,10 +423,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   // Item `i` of this CTA: the block it was launched as, then those it took over.
   PfWork w;
   int block = blockIdx.x;
-  auto open = [&] {  // false: none, nor any behind it
-    w.head = block % p.nh;
-    return w.find(p, block / p.nh, lane);
-  };
+  auto open = [&] { return w.find(p, block, lane); };
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPfRegsOther));
@@ -460,15 +438,14 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         if (lane == 0) pf_ask(&sh->next[i & 1], &sh->next_full[i & 1]);
         const bool any = open();
         const int n = any ? max(w.tiles(p, 0), w.tiles(p, 1)) : 0;
-        const int kvh = w.head / (p.nh / p.nkv);
         if (n > 0) {
           if (items > 0) ok = wait(&sh->q_empty, items - 1);
           if (ok && lane == 0) {
-            const int q_tiles = w.rows(1) > 0 ? 2 : 1;
-            mbar_arrive_expect_tx(&sh->q_full, q_tiles * SM::kTile);
+            const int q_tiles = w.queries(p, 1) > 0 ? 2 : 1;
+            mbar_arrive_expect_tx(&sh->q_full, q_tiles * H * 128 * p.heads * p.queries);
             for (int t = 0; t < q_tiles; ++t)
               for (int h = 0; h < H; ++h)
-                pf_load_3d(sh->q[t] + h * SM::kHalf, &qmap, 64 * h, w.head * p.q_mul, w.q_start + w.q0 + t * kPfRows,
+                pf_load_3d(sh->q[t] + h * SM::kHalf, &qmap, 64 * h, w.head, w.q_start + w.q0 + t * p.queries,
                            &sh->q_full);
           }
           if (ok) ++items;
@@ -481,7 +458,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
               const int key = w.k_start + (l >> 1) * kPfRows;
               for (int h = 0; h < H; ++h)
                 pf_load_3d(sh->ring[s] + h * SM::kHalf, l & 1 ? &vmap : &kmap, 64 * h,
-                           kvh * (l & 1 ? p.v_mul : p.k_mul), key, &sh->full[s]);
+                           w.kvh * (l & 1 ? p.v_mul : p.k_mul), key, &sh->full[s]);
             }
             ++issued;
           }
@@ -612,16 +589,16 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     const int t = warp >> 2;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t s_at = tmem + lanes + 128 * t, o_at = tmem + lanes + 256 + HD * t;
-    const int r = 32 * (warp & 3) + lane;
+    const int r = 32 * (warp & 3) + lane, my_query = r / p.heads, my_head = r - my_query * p.heads;
     const float scale = p.scale;
     const uint64_t scale2 = pf_two(scale, scale);
     bool ok = true;
     int done = 0;  // key tiles
     for (int i = 0; ok; ++i) {
       const bool any = open();
-      const int nt = any ? w.tiles(p, t) : 0, row = w.q0 + kPfRows * t + r;
-      const bool live = any && r < w.rows(t);
-      const int seen = live ? w.seen(p, row) : 0;
+      const int nt = any ? w.tiles(p, t) : 0, row = w.q0 + p.queries * t + my_query;
+      const bool live = any && my_query < w.queries(p, t);
+      const int seen = live ? w.seen(p, row) : w.k_len;  // rows without a query: nothing to mask
       float m_ref = -INFINITY, base = 0.f, sum = 0.f;  // reference in units of the unscaled score, and scaled
       for (int j = 0; j < nt; ++j, ++done) {
         ok = wait(&sh->s_full[t], done);
@@ -697,7 +674,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       if (!ok) break;
       pf_fence_after();
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      T* op = static_cast<T*>(p.out) + static_cast<int64_t>(w.q_start + row) * p.o_tok + w.head * p.o_head;
+      T* op = static_cast<T*>(p.out) + static_cast<int64_t>(w.q_start + row) * p.o_tok + (w.head + my_head) * p.o_head;
       bool finite = true;
 #pragma unroll
       for (int c = 0; c < HD; c += 32) {
@@ -724,7 +701,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       }
       __syncwarp();
       for (uint32_t again = __ballot_sync(0xffffffffu, live && !finite); again; again &= again - 1)
-        pf_row_again<T, HD>(p, w, w.q0 + kPfRows * t + 32 * (warp & 3) + __ffs(again) - 1, lane);
+        pf_row_again<T, HD>(p, w, w.head + __shfl_sync(0xffffffffu, my_head, __ffs(again) - 1),
+                            __shfl_sync(0xffffffffu, row, __ffs(again) - 1), lane);
       ok = wait(&sh->next_full[i & 1], i >> 1);
       if (!ok) break;
       block = pf_answer(&sh->next[i & 1]);
@@ -743,24 +721,32 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   }
 }
 
-// Map of (tokens, heads, hd) in boxes of 128 tokens of 64 channels; a head
-// stride of 0 (a broadcast head) is a map of one head.
+// Map of (tokens, heads, hd) in boxes of 64 channels of `box_heads` heads of
+// `box_tokens` tokens; a head stride of 0 (a broadcast head) is a map of one head.
 inline bool pf_map(CUtensorMap* map, int type, const void* base, int64_t tokens, int heads, int hd, int64_t tok_stride,
-                   int64_t head_stride, int* mul) {
+                   int64_t head_stride, int box_heads, int box_tokens) {
   auto encode = tensor_map_encoder();
   if (!encode) return false;
-  *mul = head_stride == 0 ? 0 : 1;
   const bool one = heads == 1 || head_stride == 0;
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(one ? 1 : heads),
                               static_cast<cuuint64_t>(tokens)};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(one ? hd : head_stride) * 2,
                                  static_cast<cuuint64_t>(tokens == 1 ? hd : tok_stride) * 2};
-  const cuuint32_t box[3] = {64, 1, kPfRows}, step[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens)};
+  const cuuint32_t step[3] = {1, 1, 1};
   std::memset(map, 0, sizeof *map);
   return encode(map, type == FRC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
                 const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Query heads of a tile: the most of a KV head's (a divisor of their number)
+// that leave at most 4 of a tile's 128 rows unused.
+inline int pf_heads(int group) {
+  for (int d = group < kPfRows ? group : kPfRows; d > 1; --d)
+    if (group % d == 0 && kPfRows / d * d >= kPfRows - 4) return d;
+  return 1;
 }
 
 template <typename T, int HD>
@@ -769,7 +755,7 @@ cudaError_t launch_prefill(const CUtensorMap& q, const CUtensorMap& k, const CUt
   static std::atomic<uint64_t> ready{0};  // devices on which the kernel may use its shared memory
   const cudaError_t e = allow_smem(attn_prefill_kernel<T, HD>, sizeof(PfSmem<HD>), ready);
   if (e != cudaSuccess) return e;
-  return launch_pdl(attn_prefill_kernel<T, HD>, dim3(static_cast<unsigned>(p.q_blocks) * p.nh), dim3(kPfThreads),
+  return launch_pdl(attn_prefill_kernel<T, HD>, dim3(static_cast<unsigned>(p.q_blocks) * (p.nh / p.heads)), dim3(kPfThreads),
                     sizeof(PfSmem<HD>), st, q, k, v, p);
 }
 
@@ -793,6 +779,8 @@ extern "C" int frc_attention_prefill(int type, const void* q, int64_t q_tok_stri
                 "frc_attention_prefill: strides must be multiples of 8 elements, below 2^38");
   FRC_REQUIRE((q_tok_stride > 0 || tokens_q <= 1) && ((k_tok_stride > 0 && v_tok_stride > 0) || tokens_k <= 1),
               "frc_attention_prefill: token strides must not be zero");
+  FRC_REQUIRE((q_head_stride > 0 && out_head_stride > 0) || nh == 1,
+              "frc_attention_prefill: the heads of q and out must not be one");
   FRC_REQUIRE(scale == scale && scale - scale == 0.f, "frc_attention_prefill: scale must be finite");
   if (batch == 0 || tokens_q == 0) return FRC_OK;
   FRC_REQUIRE(q && ((k && v) || tokens_k == 0) && cu_q && cu_k && out, "frc_attention_prefill: null pointer");
@@ -821,10 +809,14 @@ extern "C" int frc_attention_prefill(int type, const void* q, int64_t q_tok_stri
   const float size = scale < 0.f ? -scale : scale;
   p.scale = size < 1e-30f ? 1e-30f : size * 1.44269504088896341f;
   p.causal = causal != 0;
+  p.heads = frc::pf_heads(nh / nkv);
+  p.queries = frc::kPfRows / p.heads;
+  p.k_mul = k_head_stride != 0;
+  p.v_mul = v_head_stride != 0;
   // at most: a partly filled block for each sequence that has a query
-  const int64_t per = frc::kPfTiles * frc::kPfRows;
+  const int64_t per = frc::kPfTiles * p.queries;
   const int64_t blocks = tokens_q / per + (batch < tokens_q ? batch : tokens_q);
-  FRC_REQUIRE(blocks * nh <= 0x7fffffff, "frc_attention_prefill: too many queries");
+  FRC_REQUIRE(blocks * (nh / p.heads) <= 0x7fffffff, "frc_attention_prefill: too many queries");
   p.q_blocks = static_cast<int>(blocks);
   p.out = out;
   p.o_tok = out_tok_stride;
@@ -832,11 +824,12 @@ extern "C" int frc_attention_prefill(int type, const void* q, int64_t q_tok_stri
   FRC_LAUNCHED(frc::serving_status(&p.status), "status word");
   CUtensorMap qm, km, vm;
   const bool none = tokens_k == 0;  // no key is read: any valid map will do
-  if (!frc::pf_map(&qm, type, q, tokens_q, nh, hd, q_tok_stride, q_head_stride, &p.q_mul) ||
+  const int rows = frc::kPfRows;
+  if (!frc::pf_map(&qm, type, q, tokens_q, nh, hd, q_tok_stride, q_head_stride, p.heads, p.queries) ||
       !frc::pf_map(&km, type, none ? q : k, none ? tokens_q : tokens_k, none ? nh : nkv, hd,
-                   none ? q_tok_stride : k_tok_stride, none ? q_head_stride : k_head_stride, &p.k_mul) ||
+                   none ? q_tok_stride : k_tok_stride, none ? q_head_stride : k_head_stride, 1, rows) ||
       !frc::pf_map(&vm, type, none ? q : v, none ? tokens_q : tokens_k, none ? nh : nkv, hd,
-                   none ? q_tok_stride : v_tok_stride, none ? q_head_stride : v_head_stride, &p.v_mul))
+                   none ? q_tok_stride : v_tok_stride, none ? q_head_stride : v_head_stride, 1, rows))
     return frc__fail(FRC_ERR_CUDA, "frc_attention_prefill: cuTensorMapEncodeTiled failed");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool bf = type == FRC_BF16;
