@@ -75,6 +75,7 @@ SIGNATURES: dict[str, list] = {
                                 _p, _sz, _p, _i64, _i64, _p],
     "frc_attention_prefill": [_i, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i, _i64, _i64, _i, _i, _i,
                               ctypes.c_float, _i, _p, _i64, _i64, _p],
+    "frc_serving_call": [_i, _cp, _sz, _p],
     "frc_gemv": [_i, _p, _sz, _i64, _i64, _p, _i64, _p, _p],
     "frc_gemv_noalloc": [_i, _p, _sz, _i64, _i64, _p, _i64, _p, _p],
     "frc_ipc_alloc": [_sz, ctypes.POINTER(_p), _p],
@@ -116,7 +117,7 @@ class LibraryMissing(ImportError):
     pass
 
 
-_lib = None
+_lib: ctypes.CDLL | None = None
 _lock = threading.Lock()
 
 

@@ -29,6 +29,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import numpy as np
 import torch
@@ -39,44 +40,67 @@ _TYPE = {torch.float32: _lib.FRC_F32, torch.float16: _lib.FRC_F16, torch.bfloat1
 _BLOCK = 16  # tokens of a cache block
 
 
+# The records of frc_serving_call (include/frcuda.h): one ctypes argument in
+# place of two dozen, which cost a quarter of a microsecond each.
+_ROPE = (0, struct.Struct("qqQqqqqqQQQdQQqqqQQqQqQq"))
+_APPEND = (1, struct.Struct("qQqqQqqqQqqqqQ"))
+_READ = (2, struct.Struct("qQQqqqqqQqqQqq"))
+_DECODE = (3, struct.Struct("qQqqQqqQqqQqqqqdQqQqq"))
+_PREFILL = (4, struct.Struct("qQqqQqqQqqQQqqqqqqdqQqq"))
+
+# The current device, and the raw handle of a device's current stream: as
+# torch.cuda.current_device() and torch.cuda.current_stream(i).cuda_stream,
+# without a Python object each.
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
 def _need(cond: bool, what: str) -> None:
     if not cond:
         raise ValueError(what)
 
 
-def _launch(device: torch.device, fn, *args) -> None:
-    """fn(*args, stream) with `device` current, on its current stream."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+def _launch(device: int, op, *args) -> None:
+    """The operator with `device` current, on its current stream."""
+    lib = _lib._lib or _lib.load()
+    number, record = op
+    if device == _current_device():
+        rc = lib.frc_serving_call(number, record.pack(*args), record.size, _raw_stream(device))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            rc = lib.frc_serving_call(number, record.pack(*args), record.size, _raw_stream(device))
     if rc:
         _lib.check(rc)
 
 
-def _same_cuda_device(tensors) -> torch.device:
-    device = tensors[0].device
+def _same_cuda_device(*tensors) -> int:
     grad = torch.is_grad_enabled()
+    first = tensors[0]
+    i = first.get_device()
     for t in tensors:
-        if t.device != device:
-            raise ValueError(f"tensors on different devices: {device} and {t.device}")
         if grad and t.requires_grad:
             raise ValueError("the operator has no backward pass: call it under torch.no_grad()")
-    _need(device.type == "cuda", f"tensors must be on a CUDA device, not {device}")
-    return device
+        if t.get_device() != i:
+            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
+    if not first.is_cuda:
+        raise ValueError(f"tensors must be on a CUDA device, not {first.device}")
+    return i
 
 
 def _index(t: torch.Tensor, name: str, dtype: torch.dtype, shape) -> None:
-    _need(t.dtype == dtype and tuple(t.shape) == tuple(shape) and t.is_contiguous(),
-          f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}")
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}")
 
 
-def _rows(t: torch.Tensor, name: str, shape, dtype: torch.dtype) -> None:
-    """A (rows, heads, head_dim) tensor with contiguous channels."""
-    _need(tuple(t.shape) == tuple(shape) and t.dtype == dtype,
-          f"{name} must be a {dtype} tensor of shape {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
-    _need(t.stride(-1) == 1 or t.shape[-1] == 1 or t.numel() == 0, f"the channels of {name} must be contiguous")
+def _rows(t: torch.Tensor, name: str, shape, dtype: torch.dtype):
+    """Strides of the rows and heads of a (rows, heads, head_dim) tensor with contiguous channels."""
+    if t.shape != shape or t.dtype != dtype:
+        raise ValueError(f"{name} must be a {dtype} tensor of shape {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
+    rows, heads, channels = t.stride()
+    if channels != 1 and shape[2] > 1 and t.numel():
+        raise ValueError(f"the channels of {name} must be contiguous")
+    return rows, heads
 
 
 # ---- position rotation ----------------------------------------------------------------
@@ -150,44 +174,61 @@ def qk_norm_rope(qkv, heads: int, kv_heads: int, cos, sin, positions, *, bias=No
     in `out_dtype` (default: qkv's); `out` = (q, k, v) to write to, which may
     be views of qkv itself.
     """
-    _need(qkv.dim() == 2 and qkv.dtype in _TYPE, "qkv must be a 2-D fp32, fp16 or bf16 tensor")
-    _need(heads > 0 and kv_heads > 0, "heads and kv_heads must be positive")
+    in_type = _TYPE.get(qkv.dtype)
+    if qkv.dim() != 2 or in_type is None:
+        raise ValueError("qkv must be a 2-D fp32, fp16 or bf16 tensor")
+    if heads <= 0 or kv_heads <= 0:
+        raise ValueError("heads and kv_heads must be positive")
     tokens, n = qkv.shape
-    _need(n % (heads + 2 * kv_heads) == 0, f"rows of {n} do not hold {heads} + 2 * {kv_heads} heads")
-    hd = n // (heads + 2 * kv_heads)
-    _need(hd > 0 and hd % 2 == 0 and hd <= 256, f"head_dim must be even and at most 256, not {hd}")
-    _need(qkv.stride(1) == 1, "the rows of qkv must be contiguous")
-    _need(cos.dim() == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype == torch.float32 and
-          cos.is_contiguous() and sin.is_contiguous() and cos.shape[0] > 0,
-          "cos and sin must be contiguous fp32 tensors of one shape (max_pos, rot / 2)")
-    rot = 2 * cos.shape[1]
-    _need(rot <= hd, f"the tables rotate {rot} of {hd} channels")
+    row, column = qkv.stride()
+    hd, rest = divmod(n, heads + 2 * kv_heads)
+    if rest:
+        raise ValueError(f"rows of {n} do not hold {heads} + 2 * {kv_heads} heads")
+    if hd <= 0 or hd % 2 or hd > 256:
+        raise ValueError(f"head_dim must be even and at most 256, not {hd}")
+    if column != 1:
+        raise ValueError("the rows of qkv must be contiguous")
+    if (cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32 or
+            not cos.is_contiguous() or not sin.is_contiguous() or cos.shape[0] == 0):
+        raise ValueError("cos and sin must be contiguous fp32 tensors of one shape (max_pos, rot / 2)")
+    max_pos, pairs = cos.shape
+    if 2 * pairs > hd:
+        raise ValueError(f"the tables rotate {2 * pairs} of {hd} channels")
     _index(positions, "positions", torch.int32, (tokens,))
     used = [qkv, cos, sin, positions]
+    weights = []
     for t, name, size in ((bias, "bias", n), (q_norm, "q_norm", hd), (k_norm, "k_norm", hd)):
-        if t is not None:
+        if t is None:
+            weights.append(0)
+        else:
             _index(t, name, torch.float32, (size,))
             used.append(t)
+            weights.append(t.data_ptr())
     if out is None:
         dtype = out_dtype or qkv.dtype
-        _need(dtype in _TYPE, f"out_dtype must be fp32, fp16 or bf16, not {dtype}")
+        if dtype not in _TYPE:
+            raise ValueError(f"out_dtype must be fp32, fp16 or bf16, not {dtype}")
         out = tuple(torch.zeros((tokens, h, hd), dtype=dtype, device=qkv.device) for h in (heads, kv_heads, kv_heads))
     else:
-        _need(len(out) == 3, "out must be (q, k, v)")
+        if len(out) != 3:
+            raise ValueError("out must be (q, k, v)")
         dtype = out[0].dtype
-        _need(dtype in _TYPE and out_dtype in (None, dtype), "out has another type than out_dtype, or not fp32/fp16/bf16")
-        for t, name, h in zip(out, ("q", "k", "v"), (heads, kv_heads, kv_heads)):
-            _rows(t, f"out {name}", (tokens, h, hd), dtype)
-            _need(t.stride(1) == hd or h == 1 or tokens == 0, f"the heads of out {name} must be contiguous")
-    device = _same_cuda_device([*used, *out])
+        if dtype not in _TYPE or out_dtype not in (None, dtype):
+            raise ValueError("out has another type than out_dtype, or not fp32, fp16 or bf16")
+    strides = []
+    for t, name, h in zip(out, ("out q", "out k", "out v"), (heads, kv_heads, kv_heads)):
+        r, s = _rows(t, name, (tokens, h, hd), dtype)
+        if s != hd and h > 1 and tokens:
+            raise ValueError(f"the heads of {name} must be contiguous")
+        if r < h * hd and tokens > 1:
+            raise ValueError(f"the rows of {name} overlap")
+        strides.append(r if tokens > 1 else h * hd)
     q, k, v = out
-    _launch(device, _lib.load().frc_qk_norm_rope, _TYPE[qkv.dtype], _TYPE[dtype], qkv.data_ptr(),
-            qkv.stride(0) if tokens > 1 else n, tokens, heads, kv_heads, hd,
-            bias.data_ptr() if bias is not None else None, q_norm.data_ptr() if q_norm is not None else None,
-            k_norm.data_ptr() if k_norm is not None else None, eps, cos.data_ptr(), sin.data_ptr(), cos.shape[0], rot,
-            1 if interleaved else 0, positions.data_ptr(), q.data_ptr(), q.stride(0) if tokens > 1 else heads * hd,
-            k.data_ptr(), k.stride(0) if tokens > 1 else kv_heads * hd, v.data_ptr(),
-            v.stride(0) if tokens > 1 else kv_heads * hd)
+    device = _same_cuda_device(*used, q, k, v)
+    _launch(device, _ROPE, in_type, _TYPE[dtype], qkv.data_ptr(), row if tokens > 1 else n, tokens,
+            heads, kv_heads, hd, weights[0], weights[1], weights[2], eps, cos.data_ptr(), sin.data_ptr(), max_pos,
+            2 * pairs, 1 if interleaved else 0, positions.data_ptr(), q.data_ptr(), strides[0], k.data_ptr(), strides[1],
+            v.data_ptr(), strides[2])
     return out
 
 
@@ -203,10 +244,10 @@ def kv_cache_q4(pages: int, page_size: int, kv_heads: int, head_dim: int, device
 
 
 def _cache(cache) -> tuple[int, int, int, int]:
-    _need(cache.dim() == 4 and cache.dtype == torch.uint8 and cache.is_contiguous() and cache.numel() > 0 and
-          cache.shape[3] in (20 * 64, 20 * 128),
-          "the cache must be a contiguous uint8 tensor (pages, kv_heads, page_size / 16, 20 * head_dim), "
-          "head_dim 64 or 128")
+    if cache.dim() != 4 or cache.dtype != torch.uint8 or not cache.is_contiguous() or cache.numel() == 0 or \
+            cache.shape[3] not in (20 * 64, 20 * 128):
+        raise ValueError("the cache must be a contiguous uint8 tensor (pages, kv_heads, page_size / 16, 20 * head_dim), "
+                         "head_dim 64 or 128")
     pages, kv_heads, blocks, nbytes = cache.shape
     return pages, kv_heads, blocks * _BLOCK, nbytes // 20
 
@@ -216,14 +257,17 @@ def kv_append_q4(cache, k, v, slots) -> None:
     (int64, page * page_size + offset) of the cache.  Slots outside the cache
     are skipped (use -1 for padding rows); the others of one call must differ."""
     pages, nkv, page, hd = _cache(cache)
-    _need(k.dtype in _TYPE, f"keys must be fp32, fp16 or bf16, not {k.dtype}")
+    dtype = _TYPE.get(k.dtype)
+    if dtype is None:
+        raise ValueError(f"keys must be fp32, fp16 or bf16, not {k.dtype}")
     tokens = k.shape[0] if k.dim() else 0
-    _rows(k, "k", (tokens, nkv, hd), k.dtype)
-    _rows(v, "v", (tokens, nkv, hd), k.dtype)
+    shape = (tokens, nkv, hd)
+    k_row, k_head = _rows(k, "k", shape, k.dtype)
+    v_row, v_head = _rows(v, "v", shape, k.dtype)
     _index(slots, "slots", torch.int64, (tokens,))
-    device = _same_cuda_device((cache, k, v, slots))
-    _launch(device, _lib.load().frc_kv_append_q4, _TYPE[k.dtype], k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-            v.stride(0), v.stride(1), tokens, slots.data_ptr(), nkv, hd, pages, page, cache.data_ptr())
+    device = _same_cuda_device(cache, k, v, slots)
+    _launch(device, _APPEND, dtype, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
+            tokens, slots.data_ptr(), nkv, hd, pages, page, cache.data_ptr())
 
 
 def kv_read_q4(cache, slots, *, dtype=None, out=None):
@@ -232,21 +276,26 @@ def kv_read_q4(cache, slots, *, dtype=None, out=None):
     is outside the cache are left as they are (zeros where this call makes
     the outputs)."""
     pages, nkv, page, hd = _cache(cache)
-    _need(slots.dim() == 1, "slots must have one dimension")
+    if slots.dim() != 1:
+        raise ValueError("slots must have one dimension")
     tokens = slots.shape[0]
     _index(slots, "slots", torch.int64, (tokens,))
+    shape = (tokens, nkv, hd)
     if out is None:
         dtype = dtype or torch.float32
-        _need(dtype in _TYPE, f"dtype must be fp32, fp16 or bf16, not {dtype}")
-        out = tuple(torch.zeros((tokens, nkv, hd), dtype=dtype, device=cache.device) for _ in range(2))
-    _need(len(out) == 2 and out[0].dtype in _TYPE and dtype in (None, out[0].dtype),
-          "out must be (k, v) in fp32, fp16 or bf16, of the type asked for")
+        if dtype not in _TYPE:
+            raise ValueError(f"dtype must be fp32, fp16 or bf16, not {dtype}")
+        out = tuple(torch.zeros(shape, dtype=dtype, device=cache.device) for _ in range(2))
+    if len(out) != 2 or out[0].dtype not in _TYPE or dtype not in (None, out[0].dtype):
+        raise ValueError("out must be (k, v) in fp32, fp16 or bf16, of the type asked for")
     k, v = out
-    _rows(k, "out k", (tokens, nkv, hd), k.dtype)
-    _rows(v, "out v", (tokens, nkv, hd), k.dtype)
-    device = _same_cuda_device((cache, slots, k, v))
-    _launch(device, _lib.load().frc_kv_read_q4, _TYPE[k.dtype], cache.data_ptr(), slots.data_ptr(), tokens, nkv, hd,
-            pages, page, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1))
+    k_row, k_head = _rows(k, "out k", shape, k.dtype)
+    v_row, v_head = _rows(v, "out v", shape, k.dtype)
+    if tokens and (min(k_row, v_row) <= 0 < tokens - 1 or min(k_head, v_head) <= 0 < nkv - 1):
+        raise ValueError("the rows or heads of out overlap")
+    device = _same_cuda_device(cache, slots, k, v)
+    _launch(device, _READ, _TYPE[k.dtype], cache.data_ptr(), slots.data_ptr(), tokens, nkv, hd,
+            pages, page, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head)
     return out
 
 
@@ -275,23 +324,30 @@ def attention_decode_q4(q, cache, block_table, lengths, *, scale: float | None =
     q's type, into `out` where given.
     """
     pages, nkv, page, hd = _cache(cache)
-    _need(q.dim() == 3 and q.dtype in _TYPE, "q must be (batch, heads, head_dim) in fp32, fp16 or bf16")
-    batch, nh = q.shape[0], q.shape[1]
-    _rows(q, "q", (batch, nh, hd), q.dtype)
-    _need(nh > 0 and nh % nkv == 0, f"{nh} query heads are not a multiple of the cache's {nkv}")
-    _need(block_table.dim() == 2, "block_table must be (batch, max_pages)")
-    _index(block_table, "block_table", torch.int32, (batch, block_table.shape[1]))
+    dtype = _TYPE.get(q.dtype)
+    if q.dim() != 3 or dtype is None:
+        raise ValueError("q must be (batch, heads, head_dim) in fp32, fp16 or bf16")
+    batch, nh, _ = q.shape
+    shape = (batch, nh, hd)
+    q_seq, q_head = _rows(q, "q", shape, q.dtype)
+    if nh == 0 or nh % nkv:
+        raise ValueError(f"{nh} query heads are not a multiple of the cache's {nkv}")
+    if block_table.dim() != 2:
+        raise ValueError("block_table must be (batch, max_pages)")
+    max_pages = block_table.shape[1]
+    _index(block_table, "block_table", torch.int32, (batch, max_pages))
     _index(lengths, "lengths", torch.int32, (batch,))
     if out is None:
-        out = torch.empty((batch, nh, hd), dtype=q.dtype, device=q.device)
-    else:
-        _rows(out, "out", (batch, nh, hd), q.dtype)
-    device = _same_cuda_device((q, cache, block_table, lengths, out))
-    ws = torch.empty(_decode_q4_workspace(batch, nh, nkv, hd), dtype=torch.uint8, device=device)
-    _launch(device, _lib.load().frc_attention_decode_q4, _TYPE[q.dtype], q.data_ptr(), q.stride(0), q.stride(1),
-            cache.data_ptr(), pages, page, block_table.data_ptr(), block_table.shape[1], block_table.shape[1],
-            lengths.data_ptr(), batch, nh, nkv, hd, hd ** -0.5 if scale is None else scale, ws.data_ptr(), ws.numel(),
-            out.data_ptr(), out.stride(0), out.stride(1))
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    o_seq, o_head = _rows(out, "out", shape, q.dtype)
+    if batch and (o_seq <= 0 < batch - 1 or o_head <= 0 < nh - 1):
+        raise ValueError("the rows or heads of out overlap")
+    device = _same_cuda_device(q, cache, block_table, lengths, out)
+    nbytes = _decode_q4_workspace(batch, nh, nkv, hd)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    _launch(device, _DECODE, dtype, q.data_ptr(), q_seq, q_head, cache.data_ptr(), pages,
+            page, block_table.data_ptr(), max_pages, max_pages, lengths.data_ptr(), batch, nh, nkv, hd,
+            hd ** -0.5 if scale is None else scale, ws.data_ptr(), nbytes, out.data_ptr(), o_seq, o_head)
     return out
 
 
@@ -307,32 +363,37 @@ def attention_prefill(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: f
     sees no key gives zeros; rows of no sequence are left as they are (zeros
     where this call makes the output).  `scale` defaults to head_dim^-1/2.
     """
-    _need(q.dim() == 3 and q.dtype in (torch.float16, torch.bfloat16), "q must be (tokens, heads, head_dim), fp16 or bf16")
-    _need(k.dim() == 3, "k must be (tokens, kv_heads, head_dim)")
+    if q.dim() != 3 or q.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("q must be (tokens, heads, head_dim), fp16 or bf16")
+    if k.dim() != 3:
+        raise ValueError("k must be (tokens, kv_heads, head_dim)")
     tokens, nh, hd = q.shape
-    tokens_k, nkv = k.shape[0], k.shape[1]
-    _need(hd in (64, 128), f"head_dim must be 64 or 128, not {hd}")
-    _rows(q, "q", (tokens, nh, hd), q.dtype)
-    _rows(k, "k", (tokens_k, nkv, hd), q.dtype)
-    _rows(v, "v", (tokens_k, nkv, hd), q.dtype)
-    _need(nkv > 0 and nh > 0 and nh % nkv == 0, f"{nh} query heads are not a multiple of {nkv} key heads")
+    tokens_k, nkv, _ = k.shape
+    if hd not in (64, 128):
+        raise ValueError(f"head_dim must be 64 or 128, not {hd}")
+    dtype, shape, shape_k = q.dtype, (tokens, nh, hd), (tokens_k, nkv, hd)
+    strides = [_rows(q, "q", shape, dtype), _rows(k, "k", shape_k, dtype), _rows(v, "v", shape_k, dtype)]
+    if nkv == 0 or nh == 0 or nh % nkv:
+        raise ValueError(f"{nh} query heads are not a multiple of {nkv} key heads")
     if cu_k is None:
         cu_k = cu_q
-    _need(cu_q.dim() == 1 and cu_q.shape[0] >= 1, "cu_q must hold batch + 1 ends")
+    if cu_q.dim() != 1 or cu_q.shape[0] < 1:
+        raise ValueError("cu_q must hold batch + 1 ends")
     _index(cu_q, "cu_q", torch.int32, cu_q.shape)
     _index(cu_k, "cu_k", torch.int32, cu_q.shape)
     if out is None:
-        out = torch.zeros((tokens, nh, hd), dtype=q.dtype, device=q.device)
-    else:
-        _rows(out, "out", (tokens, nh, hd), q.dtype)
-    for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
-        _need(t.numel() == 0 or (t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0),
-              f"{name} must be 16-byte aligned, with row and head strides that are multiples of 8")
-    device = _same_cuda_device((q, k, v, cu_q, cu_k, out))
-    _launch(device, _lib.load().frc_attention_prefill, _TYPE[q.dtype], q.data_ptr(), q.stride(0), q.stride(1),
-            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), cu_q.data_ptr(),
-            cu_k.data_ptr(), cu_q.shape[0] - 1, tokens, tokens_k, nh, nkv, hd, hd ** -0.5 if scale is None else scale,
-            1 if causal else 0, out.data_ptr(), out.stride(0), out.stride(1))
+        out = torch.zeros(shape, dtype=dtype, device=q.device)
+    strides.append(_rows(out, "out", shape, dtype))
+    at = [q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()]
+    for t, (row, head), p, name in zip((q, k, v, out), strides, at, ("q", "k", "v", "out")):
+        if (p % 16 or row % 8 or head % 8) and t.numel():
+            raise ValueError(f"{name} must be 16-byte aligned, with row and head strides that are multiples of 8")
+    if tokens and (strides[3][0] <= 0 < tokens - 1 or strides[3][1] <= 0 < nh - 1):
+        raise ValueError("the rows or heads of out overlap")
+    device = _same_cuda_device(q, k, v, cu_q, cu_k, out)
+    _launch(device, _PREFILL, _TYPE[dtype], at[0], *strides[0], at[1], *strides[1], at[2],
+            *strides[2], cu_q.data_ptr(), cu_k.data_ptr(), cu_q.shape[0] - 1, tokens, tokens_k, nh, nkv, hd,
+            hd ** -0.5 if scale is None else scale, 1 if causal else 0, at[3], *strides[3])
     return out
 
 

@@ -290,10 +290,12 @@ struct PfWork {
     const int span = kPfTiles * p.queries;
     for (int top = p.batch; top > 0; top -= 32) {
       const int b = top - 1 - lane;
-      int a0 = 0, a1 = 0;
+      int a0 = 0, a1 = 0, k0 = 0, k1 = 0;
       if (b >= 0) {
         a0 = min(max(p.cu_q[b], 0), p.tokens_q);
         a1 = min(max(p.cu_q[b + 1], a0), p.tokens_q);
+        k0 = min(max(p.cu_k[b], 0), p.tokens_k);
+        k1 = min(max(p.cu_k[b + 1], k0), p.tokens_k);
       }
       const int n = (a1 - a0 + span - 1) / span;
       int incl = n;
@@ -313,9 +315,8 @@ struct PfWork {
       const int blocks = __shfl_sync(0xffffffffu, n, l);
       const int in_seq = rank - (__shfl_sync(0xffffffffu, incl, l) - blocks);
       q0 = (blocks - 1 - in_seq) * span;
-      const int s = top - 1 - l;
-      k_start = min(max(p.cu_k[s], 0), p.tokens_k);
-      k_len = min(max(p.cu_k[s + 1], k_start), p.tokens_k) - k_start;
+      k_start = __shfl_sync(0xffffffffu, k0, l);
+      k_len = __shfl_sync(0xffffffffu, k1, l) - k_start;
       return true;
     }
     return false;
@@ -373,6 +374,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     attn_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap vmap, const PrefillParams p) {
   griddep_wait();
+  griddep_launch_dependents();
   using SM = PfSmem<HD>;
   constexpr int NS = SM::kStages, H = HD / 64;
   extern __shared__ __align__(1024) uint8_t pf_smem[];
@@ -412,6 +414,12 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh->tmem)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  if (warp == 9 && lane == 0)
+    for (const CUtensorMap* map : {&qmap, &kmap, &vmap}) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+  // Item `i` of this CTA: the block it was launched as, then those it took over.
+  PfWork w;
+  int block = blockIdx.x;
+  bool any = w.find(p, block, lane);  // false: there is none, nor any behind it
   pf_fence_before();
   __syncthreads();
   pf_fence_after();
@@ -420,10 +428,6 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   auto wait = [&](uint64_t* bar, uint32_t parity) {  // a warp's bounded wait
     return __all_sync(0xffffffffu, wait_phase(bar, parity & 1, abort));
   };
-  // Item `i` of this CTA: the block it was launched as, then those it took over.
-  PfWork w;
-  int block = blockIdx.x;
-  auto open = [&] { return w.find(p, block, lane); };
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPfRegsOther));
@@ -436,7 +440,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         if (i >= 2) ok = wait(&sh->next_empty[i & 1], (i >> 1) - 1) && ok;
         if (!ok) break;
         if (lane == 0) pf_ask(&sh->next[i & 1], &sh->next_full[i & 1]);
-        const bool any = open();
+        if (i > 0) any = w.find(p, block, lane);
         const int n = any ? max(w.tiles(p, 0), w.tiles(p, 1)) : 0;
         if (n > 0) {
           if (items > 0) ok = wait(&sh->q_empty, items - 1);
@@ -506,7 +510,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       int used = 0, items = 0;                           // K and V tiles, items that had queries
       int done[kPfTiles] = {0, 0}, outs[kPfTiles] = {0, 0};  // key tiles and items of each query tile
       for (int i = 0; ok; ++i) {
-        const bool any = open();
+        if (i > 0) any = w.find(p, block, lane);
         const int nt[kPfTiles] = {any ? w.tiles(p, 0) : 0, any ? w.tiles(p, 1) : 0};
         const int n = max(nt[0], nt[1]);
         if (n > 0) {
@@ -595,7 +599,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     bool ok = true;
     int done = 0;  // key tiles
     for (int i = 0; ok; ++i) {
-      const bool any = open();
+      if (i > 0) any = w.find(p, block, lane);
       const int nt = any ? w.tiles(p, t) : 0, row = w.q0 + p.queries * t + my_query;
       const bool live = any && my_query < w.queries(p, t);
       const int seen = live ? w.seen(p, row) : w.k_len;  // rows without a query: nothing to mask

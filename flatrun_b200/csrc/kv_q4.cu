@@ -7,17 +7,15 @@
 //       0 .. 15 (0 where d = 0)
 // and a group with a value that is not finite gets m = NaN, so that it reads
 // back as NaN.  The quotients are formed in fp32; where one lies so near a
-// border between two results that fp32 could fall on the wrong side, that
-// lane forms it in fp64 (exact for these operands: an fp32 difference and a
-// quotient by at most 11 bits that is nowhere within 2^-53 of a border without
-// being on it), so the cache's bits follow from the definition alone.
+// border between two results that fp32 could fall on the wrong side, the side is
+// found exactly, so the cache's bits follow from the definition alone.
 //
 // Bound by HBM: 2 or 4 bytes a value in, 5/8 of a byte out (append), and the
-// reverse (read).  A warp takes eight tokens of one head, four lanes a token
-// and eight channels a lane, one group at a time: a group's minimum and maximum
-// are two shuffles, a lane's eight nibbles are one word, a token's K words one
-// 4 NG byte store, and the V words of eight consecutive tokens a full 32-byte
-// sector.
+// reverse (read), if a value takes few instructions: 7 to 10 here.  A warp takes
+// eight tokens of one head, four lanes a token and eight channels a lane, one
+// group at a time: a group's minimum and maximum are two shuffles, a lane's eight
+// nibbles are one word, a token's K words one 4 NG byte store, and the V words of
+// eight consecutive tokens a full 32-byte sector.
 #include <cuda_runtime.h>
 
 #include <cstdio>
@@ -39,57 +37,92 @@ struct KvQ4Params {
 
 constexpr int kQ4Threads = 256;
 
-// fp16 of v / 15, v >= 0, rounded once.  The fp32 quotient is within 3 ulp
-// (three roundings); 13 of its bits are dropped, so only within 4 ulp of their
-// middle can the rounding fall on the wrong side (below fp16's normal range
-// more bits are dropped: there the quotient is formed in fp64).
-FRC_DEVICE_INLINE __half half_fifteenth(double v) {
-  const float f = static_cast<float>(v) * (1.0f / 15.0f);
+// The least and the largest of three, NaN if one is.
+FRC_DEVICE_INLINE float min_nan(float a, float b, float c) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+FRC_DEVICE_INLINE float max_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
+// fp16 of (hi - m) / 15, held within 0 .. 65504, rounded once.  The fp32 quotient
+// is within 3 ulp (three roundings); 13 of its bits are dropped, so only within
+// 4 ulp of their middle can the rounding fall on the wrong side (below fp16's
+// normal range more bits are dropped: there, and there alone, the quotient is
+// formed in fp64 too).
+FRC_DEVICE_INLINE __half step_of(float hi, float m) {
+  const float f = fminf(fmaxf((hi - m) * (1.0f / 15.0f), 0.f), 65504.f);
   const uint32_t low = __float_as_uint(f) & 0x1fffu;
-  if (f < 6.2e-5f || (low >= 0x1000u - 4u && low <= 0x1000u + 4u)) return __double2half(v / 15.0);
-  return __float2half_rn(f);
+  if (f > 6.2e-5f && (low < 0x1000u - 4u || low > 0x1000u + 4u)) return __float2half_rn(f);
+  return __double2half(fmin(fmax((static_cast<double>(hi) - static_cast<double>(m)) / 15.0, 0.0), 65504.0));
 }
 
 // The lane's eight values of a group shared by the four lanes of its quad:
 // its nibbles as one word, and the group's step and offset.
 FRC_DEVICE_INLINE uint32_t quantise8(const float (&x)[8], __half& step, __half& offset) {
   float lo = x[0], hi = x[0];
-  bool finite = true;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    finite = finite && fabsf(x[i]) <= 3.402823466e38f;  // false for NaN too
+  for (int i = 0; i < 8; i += 2) {
+    lo = min_nan(lo, x[i], x[i + 1]);
+    hi = max_nan(hi, x[i], x[i + 1]);
   }
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    finite = __shfl_xor_sync(0xffffffffu, finite ? 1 : 0, o) && finite;
+    const float l = __shfl_xor_sync(0xffffffffu, lo, o), h = __shfl_xor_sync(0xffffffffu, hi, o);
+    lo = min_nan(lo, l, l);
+    hi = max_nan(hi, h, h);
   }
-  offset = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f));
-  const float m = __half2float(offset);
-  const double range = static_cast<double>(hi) - static_cast<double>(m);
-  step = range >= 15.0 * 65504.0 ? __ushort_as_half(0x7bff) : half_fifteenth(range > 0.0 ? range : 0.0);
-  const float d = __half2float(step);
-  if (!finite) {
+  if (!(lo >= -3.402823466e38f && hi <= 3.402823466e38f)) {  // a NaN or an infinity
     offset = __ushort_as_half(0x7fff);
     step = __ushort_as_half(0);
     return 0u;
   }
-  if (d == 0.f) return 0u;
-  const float inv = 1.0f / d;
+  offset = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f));
+  const float m = __half2float(offset);
+  step = step_of(hi, m);
+  const float d = __half2float(step);
+  float inv;  // of 15 d, which is exact; within an ulp
+  asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(15.f * d));
+  if (d == 0.f) inv = 0.f;
+  // t = (x - m) / (15 d) held within 0 .. 1, n = round(15 t) in the low bits of
+  // the sum with 1.5 * 2^23.  t is off by 2^-24 (difference), 2^-23 (reciprocal) and
+  // 2^-24 (product) of itself, so 15 t by less than 4e-6.
+  constexpr float kMagic = 12582912.f;
   uint32_t w = 0;
+  float far = 0.f;  // the largest distance from a whole number
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    // relative error of t: 2^-24 each of the difference, the reciprocal and
-    // the product: below 3e-6 at 15.5
-    const float t = fminf(fmaxf((x[i] - m) * inv, 0.f), 15.f);
-    float r = rintf(t);
-    if (fabsf(fabsf(t - r) - 0.5f) < 4e-6f)
-      r = static_cast<float>(fmin(fmax(rint((static_cast<double>(x[i]) - static_cast<double>(m)) /
-                                            static_cast<double>(d)), 0.0), 15.0));
-    w |= static_cast<uint32_t>(r) << (4 * i);
+  for (int i = 0; i < 8; i += 2) {
+    float off[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float t = __saturatef((x[i + e] - m) * inv);
+      const float u = fmaf(t, 15.f, kMagic);
+      off[e] = fabsf(fmaf(t, 15.f, kMagic - u));
+      w += __float_as_uint(u) << (4 * (i + e));
+    }
+    far = max_nan(far, off[0], off[1]);
+  }
+  // the sums' other bits, 0x4B400000 each, add up to this
+  constexpr uint32_t kSum = 0x4B400000u * 0x11111111u;
+  w -= kSum;
+  if (far > 0.5f - 6e-6f) {  // common where 16-bit values meet the border exactly
+    w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      // h: the border nearest to 15 t; e: on which side of it x - m lies.  s + err is
+      // x - m exactly (two-sum), and s - h d is exact near the border
+      const float t = 15.f * __saturatef((x[i] - m) * inv);
+      const float h = fminf(fmaxf(rintf(t - 0.5f), 0.f), 14.f) + 0.5f;
+      const float s = __fsub_rn(x[i], m), v = __fsub_rn(s, x[i]);
+      const float err = __fsub_rn(__fsub_rn(x[i], __fsub_rn(s, v)), __fadd_rn(m, v));
+      const float e = __fadd_rn(__fmaf_rn(-h, d, s), err);
+      const float n = e > 0.f ? h + 0.5f : (e < 0.f ? h - 0.5f : 2.f * rintf(0.5f * h));  // on it: the even one
+      w |= static_cast<uint32_t>(n) << (4 * i);
+    }
   }
   return w;
 }
@@ -106,13 +139,13 @@ FRC_DEVICE_INLINE void store_words(uint8_t* p, const uint32_t (&w)[NG]) {
 // warp -> (eight tokens, K or V, head); lane -> (token, q)
 FRC_DEVICE_INLINE bool q4_warp_item(const KvQ4Params& p, int64_t& tok, int& is_v, int& h, int& q, int64_t& block,
                                     int& t) {
-  const int64_t warp = (static_cast<int64_t>(blockIdx.x) * kQ4Threads + threadIdx.x) >> 5;
+  const uint32_t warp = blockIdx.x * (kQ4Threads / 32) + (threadIdx.x >> 5);  // below 2^31: checked by the host
   const int lane = threadIdx.x & 31;
-  const int64_t tg = warp / (2 * p.nkv);
-  const int rest = static_cast<int>(warp - tg * (2 * p.nkv));
+  const uint32_t tg = warp / static_cast<uint32_t>(2 * p.nkv);
+  const int rest = static_cast<int>(warp - tg * static_cast<uint32_t>(2 * p.nkv));
   is_v = rest >= p.nkv;
   h = is_v ? rest - p.nkv : rest;
-  tok = tg * 8 + (lane >> 2);
+  tok = static_cast<int64_t>(tg) * 8 + (lane >> 2);
   q = lane & 3;
   block = -1;
   t = 0;
@@ -121,11 +154,11 @@ FRC_DEVICE_INLINE bool q4_warp_item(const KvQ4Params& p, int64_t& tok, int& is_v
     block = q4_block_of_slot(slot, h, p.pages, p.nkv, p.blocks_per_page);
     t = static_cast<int>(slot) & (kQ4Tokens - 1);
   }
-  return tg * 8 < p.tokens;  // the same in all lanes
+  return static_cast<int64_t>(tg) * 8 < p.tokens;  // the same in all lanes
 }
 
 template <typename T, int HD, bool VEC>
-__global__ void __launch_bounds__(kQ4Threads) kv_append_q4_kernel(KvQ4Params p) {
+__global__ void __launch_bounds__(kQ4Threads, 4) kv_append_q4_kernel(KvQ4Params p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" :::);
   constexpr Q4Layout lay(HD);
@@ -145,18 +178,23 @@ __global__ void __launch_bounds__(kQ4Threads) kv_append_q4_kernel(KvQ4Params p) 
     if (live) load_run<8, VEC>(src + kQ4Group * j + 8 * q, x[j]);
   }
   uint32_t w[NG];
+  __half step = __ushort_as_half(0), offset = step;  // of group q: the lanes of a quad share them
 #pragma unroll
   for (int j = 0; j < NG; ++j) {
     __half d, m;
     w[j] = quantise8(x[j], d, m);
-    if (!live) continue;
-    if (is_v) *reinterpret_cast<uint32_t*>(blk + lay.v_word(4 * j + q, t)) = w[j];
-    if (q == (j & 3)) {  // the lanes of a quad share the group's scales
-      *reinterpret_cast<__half*>(blk + (is_v ? lay.v_step(j, t) : lay.k_step(j, t))) = d;
-      *reinterpret_cast<__half*>(blk + (is_v ? lay.v_offset(j, t) : lay.k_offset(t, j))) = m;
+    if (q == j) {
+      step = d;
+      offset = m;
     }
+    if (live && is_v) *reinterpret_cast<uint32_t*>(blk + lay.v_word(4 * j + q, t)) = w[j];
   }
-  if (live && !is_v) store_words(blk + lay.k_word(t, q, 0), w);
+  if (!live) return;
+  if (!is_v) store_words(blk + lay.k_word(t, q, 0), w);
+  if (q < NG) {
+    *reinterpret_cast<__half*>(blk + (is_v ? lay.v_step(q, t) : lay.k_step(q, t))) = step;
+    *reinterpret_cast<__half*>(blk + (is_v ? lay.v_offset(q, t) : lay.k_offset(t, q))) = offset;
+  }
 }
 
 template <typename T, int HD, bool VEC>
@@ -183,7 +221,12 @@ __global__ void __launch_bounds__(kQ4Threads) kv_read_q4_kernel(KvQ4Params p) {
   for (int j = 0; j < NG; ++j) {
     float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = fmaf(static_cast<float>((w[j] >> (4 * i)) & 15u), d[j], m[j]);
+    for (int i = 0; i < 4; ++i) {  // nibbles i and i + 4 as halves: 1024 + n, less 1024
+      const uint32_t b = ((w[j] >> (4 * i)) & 0x000f000fu) | 0x64006400u;
+      const float2 n = __half22float2(__hadd2(*reinterpret_cast<const __half2*>(&b), __float2half2_rn(-1024.f)));
+      x[i] = fmaf(n.x, d[j], m[j]);
+      x[i + 4] = fmaf(n.y, d[j], m[j]);
+    }
     store_run<8, VEC>(dst + kQ4Group * j + 8 * q, x);
   }
 }

@@ -316,6 +316,17 @@ int frc_attention_prefill(int type, const void* q, int64_t q_tok_stride, int64_t
                           int64_t tokens_k, int nh, int nkv, int hd, float scale, int causal, void* out,
                           int64_t out_tok_stride, int64_t out_head_stride, void* stream);
 
+/* The serving operators with their arguments in a record, for callers whose
+ * foreign-function layer charges by the argument: `record` holds the
+ * arguments of operator `op` before `stream`, in their order, eight bytes each
+ * (integers as int64_t, pointers as they are, float as double). */
+#define FRC_OP_QK_NORM_ROPE        0
+#define FRC_OP_KV_APPEND_Q4        1
+#define FRC_OP_KV_READ_Q4          2
+#define FRC_OP_ATTENTION_DECODE_Q4 3
+#define FRC_OP_ATTENTION_PREFILL   4
+int frc_serving_call(int op, const void* record, size_t bytes, void* stream);
+
 /* ---- row-sharded projections: all-gather fused into the GEMV ----------- *
  * No reference counterpart: the reference runs on one CPU.  One process per
  * GPU; rank r owns a contiguous row range of every projection and computes
