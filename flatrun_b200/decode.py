@@ -20,7 +20,19 @@ This is the reference forwarder's decode step (flatrun/model/qwen2.py
 ``make_qwen2_forwarder``: :1510-1646 attention, :1648-1751 MLP, :2238-2297
 head) with the NumPy work moved onto the device; the projections are the
 same B200 kernels the ``cuda`` backend slot calls.  PyTorch is used only to
-allocate device memory and for the stream and graph plumbing.
+allocate device memory and for the stream and graph plumbing (and, in
+``prefill``, for the elementwise steps between the kernels).
+
+``kv_bits=4`` keeps the cache in 4 bits (5 with its scales, against 32): the
+attention steps are then ``flatrun_b200.attention``'s:
+
+    bias + RoPE                         frc_qk_norm_rope (in place)
+    quantise and append                 frc_kv_append_q4
+    attention over the 4-bit cache      frc_attention_decode_q4
+
+``prefill`` takes a whole prompt at once: batched projections, rotation,
+``frc_attention_prefill`` in fp16, and the prompt's keys and values into the
+cache of either kind.
 """
 
 from __future__ import annotations
@@ -47,6 +59,7 @@ class DecoderConfig:
     eps: float
     rope_theta: float
     max_pos: int
+    rope_scaling: dict | None = None  # of attention.rope_tables_scaled; None: the reference's fp32 tables
 
     @property
     def head_dim(self) -> int:
@@ -70,12 +83,16 @@ class DecodeEngine:
     quant)) for the projections and the head, fp32 arrays for norms, biases
     and an fp32 embedding table (or raw bytes with its quant).  `kv_prefill` optionally
     maps a layer to (keys, values) of shape (positions, kv_heads, head_dim)
-    already in the cache before the first token.
+    already in the cache before the first token.  `kv_bits` is 32 or 4 (pages
+    of `kv_page` tokens, a multiple of 16).
     """
 
     def __init__(self, cfg: DecoderConfig, weights: dict, quant_of, device: int = 0, kv_prefill=None,
-                 attn_splits: int = 0):
+                 attn_splits: int = 0, kv_bits: int = 32, kv_page: int = 64):
         import torch
+
+        if kv_bits not in (32, 4):
+            raise ValueError(f"kv_bits must be 32 or 4, not {kv_bits}")
 
         self.torch = torch
         self.cfg = cfg
@@ -113,17 +130,31 @@ class DecodeEngine:
         eq = quant_of("model.embed_tokens.weight")
         self._emb_quant = 0 if eq is None else _lib.QUANT_IDS[eq[2]]
         self._emb = up(emb, np.float32 if eq is None else np.uint8)
-        cos, sin = rope_tables(hd, c.rope_theta, c.max_pos)
+        if c.rope_scaling is None:
+            cos, sin = rope_tables(hd, c.rope_theta, c.max_pos)
+        else:
+            from .attention import rope_tables_scaled
+            cos, sin = rope_tables_scaled(hd, c.rope_theta, c.max_pos, c.rope_scaling)
         self._cos, self._sin = up(cos, np.float32), up(sin, np.float32)
-        self.k_cache = [torch.zeros((c.max_pos, c.kv_heads, hd), dtype=f32, device=self._dev) for _ in range(c.layers)]
-        self.v_cache = [torch.zeros((c.max_pos, c.kv_heads, hd), dtype=f32, device=self._dev) for _ in range(c.layers)]
+        self.kv_bits = kv_bits
+        if kv_bits == 4:
+            from . import attention
+            self._attn = attention
+            pages = -(-c.max_pos // kv_page)
+            self.q4_cache = [attention.kv_cache_q4(pages, kv_page, c.kv_heads, hd, self._dev) for _ in range(c.layers)]
+            self._table = torch.arange(pages, dtype=torch.int32, device=self._dev).reshape(1, -1)
+        else:
+            self.k_cache, self.v_cache = (
+                [torch.zeros((c.max_pos, c.kv_heads, hd), dtype=f32, device=self._dev) for _ in range(c.layers)]
+                for _ in range(2))
         start = 0
         for i, (kp, vp) in (kv_prefill or {}).items():
-            t = kp.shape[0]
-            self.k_cache[i][:t] = up(kp, np.float32).reshape(kp.shape)
-            self.v_cache[i][:t] = up(vp, np.float32).reshape(vp.shape)
-            start = t
+            start = kp.shape[0]
+            self._store(i, 0, up(kp, np.float32).reshape(kp.shape), up(vp, np.float32).reshape(vp.shape))
         self.pos = torch.tensor([start], dtype=torch.int32, device=self._dev)
+        if kv_bits == 4:  # the token's slot, and the number of tokens with it
+            self._slot = torch.tensor([start], dtype=torch.int64, device=self._dev)
+            self._length = torch.tensor([start + 1], dtype=torch.int32, device=self._dev)
         self.tok_in = torch.zeros(1, dtype=torch.int32, device=self._dev)
         self.tok_out = torch.zeros(1, dtype=torch.int32, device=self._dev)
         self.h = torch.zeros(c.hidden, dtype=f32, device=self._dev)
@@ -144,6 +175,16 @@ class DecodeEngine:
         self.argmax_ws = torch.zeros(int(ws.value), dtype=torch.uint8, device=self._dev)
         self._graph = None
         self.launches_per_token = 0
+
+    def _store(self, layer: int, start: int, k, v) -> None:
+        """Keys and values (tokens, kv_heads, head_dim) into the layer's cache from position `start` on."""
+        end = start + k.shape[0]
+        if self.kv_bits == 4:
+            slots = self.torch.arange(start, end, dtype=self.torch.int64, device=self._dev)
+            self._attn.kv_append_q4(self.q4_cache[layer], k, v, slots)
+        else:
+            self.k_cache[layer][start:end] = k
+            self.v_cache[layer][start:end] = v
 
     # ---- launches ------------------------------------------------------------
     def _gemv(self, names, x, ys, x_mul=None, norm=None, accumulate=False):
@@ -169,6 +210,25 @@ class DecodeEngine:
                 out.append([nm])
         return out
 
+    def _mlp(self, p: str) -> None:
+        ln2 = self._norm[f"{p}.post_attention_layernorm.weight"]
+        gu = [f"{p}.mlp.gate_proj.weight", f"{p}.mlp.up_proj.weight"]
+        for grp in self._groups(gu):
+            self._gemv(grp, self.h, [self.gate if g.endswith("gate_proj.weight") else self.upb for g in grp],
+                       norm=ln2)
+        self._gemv([f"{p}.mlp.down_proj.weight"], self.gate, [self.h], x_mul=self.upb, accumulate=True)
+
+    def _attention_q4(self, layer: int, bias) -> None:
+        """The token's attention over the 4-bit cache (on the current stream, which is the engine's)."""
+        c, hd, cache = self.cfg, self.cfg.head_dim, self.q4_cache[layer]
+        row = self.qkv.view(1, -1)
+        q, k, v = (part.view(1, -1, hd) for part in row.split((c.heads * hd, c.kv_heads * hd, c.kv_heads * hd), dim=1))
+        self._attn.qk_norm_rope(row, c.heads, c.kv_heads, self._cos, self._sin, self.pos, bias=bias, out=(q, k, v))
+        self._attn.kv_append_q4(cache, k, v, self._slot)
+        self._attn.attention_decode_q4(q, cache, self._table, self._length, scale=float(np.float32(1.0 / np.sqrt(hd))),
+                                       out=self.ctx.view(1, c.heads, hd))
+        self.launches_per_token += 4
+
     def _token(self) -> None:
         """Enqueue one decode token (the graph body)."""
         c, lib, st = self.cfg, self.lib, self._st
@@ -192,6 +252,11 @@ class DecodeEngine:
             for grp in self._groups([f"{p}.{nm}.weight" for nm in _PROJ[:3]]):
                 self._gemv(grp, self.h, [outs[g[len(p) + 1:-len(".weight")]] for g in grp], norm=ln1)
             bias = self._bias.get(i)
+            if self.kv_bits == 4:
+                self._attention_q4(i, bias)
+                self._gemv([f"{p}.self_attn.o_proj.weight"], self.ctx, [self.h], accumulate=True)
+                self._mlp(p)
+                continue
             chk(lib.frc_rope_append(self.qkv.data_ptr(), bias.data_ptr() if bias is not None else None, c.heads,
                                     c.kv_heads, hd, self._cos.data_ptr(), self._sin.data_ptr(), self.pos.data_ptr(),
                                     self.k_cache[i].data_ptr(), self.v_cache[i].data_ptr(), st))
@@ -199,15 +264,13 @@ class DecodeEngine:
                                          self.pos.data_ptr(), c.heads, c.kv_heads, hd, scale, self.splits,
                                          self.part.data_ptr(), self.ctx.data_ptr(), st), kernels=2)
             self._gemv([f"{p}.self_attn.o_proj.weight"], self.ctx, [self.h], accumulate=True)
-            ln2 = self._norm[f"{p}.post_attention_layernorm.weight"]
-            gu = [f"{p}.mlp.gate_proj.weight", f"{p}.mlp.up_proj.weight"]
-            for grp in self._groups(gu):
-                self._gemv(grp, self.h, [self.gate if g.endswith("gate_proj.weight") else self.upb for g in grp],
-                           norm=ln2)
-            self._gemv([f"{p}.mlp.down_proj.weight"], self.gate, [self.h], x_mul=self.upb, accumulate=True)
+            self._mlp(p)
         self._gemv(["lm_head.weight"], self.h, [self.logits], norm=self._norm["model.norm.weight"])
         chk(lib.frc_argmax(self.logits.data_ptr(), c.vocab, self.tok_out.data_ptr(), self.argmax_ws.data_ptr(), st))
         chk(lib.frc_pos_advance(self.pos.data_ptr(), st))
+        if self.kv_bits == 4:  # (the slot is below 2^31: its low word)
+            chk(lib.frc_pos_advance(self._length.data_ptr(), st))
+            chk(lib.frc_pos_advance(self._slot.data_ptr(), st))
         # the greedy pick is the next token's input unless step() overrides it
         self.tok_in.copy_(self.tok_out)
         self.launches_per_token += 1
@@ -222,11 +285,12 @@ class DecodeEngine:
         with torch.cuda.stream(self.stream):
             # one eager token first: lazy module loading and launch
             # configuration happen outside the capture; then undo its effects
-            pos0, tok0 = self.pos.clone(), self.tok_in.clone()
+            state = [self.pos, self.tok_in] + ([self._slot, self._length] if self.kv_bits == 4 else [])
+            before = [t.clone() for t in state]
             self._token()
             self.stream.synchronize()
-            self.pos.copy_(pos0)
-            self.tok_in.copy_(tok0)
+            for t, b in zip(state, before):
+                t.copy_(b)
             self._graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(self._graph, stream=self.stream):
                 self._token()
@@ -243,6 +307,79 @@ class DecodeEngine:
                 self._token()
             else:
                 self._graph.replay()
+
+    def prefill(self, tokens) -> None:
+        """Feed a prompt at once, behind what the cache holds: afterwards `logits`
+        and `argmax_host()` are those of its last token, and `step()` goes on.
+        The projections run batched (above 16 tokens with fp16 operands, as
+        frc_gemv's), the attention on fp16 queries, keys and values;
+        asynchronous on the engine's stream but for reading the position."""
+        from . import attention
+
+        torch, c, lib, f32 = self.torch, self.cfg, self.lib, self.torch.float32
+        ids = np.asarray(tokens, np.int32).reshape(-1)
+        n, hd = ids.size, c.head_dim
+        kvd = c.kv_heads * hd
+        if n == 0:
+            raise ValueError("an empty prompt")
+        with torch.cuda.stream(self.stream):
+            start = int(self.pos.item())
+            if start + n > c.max_pos:
+                raise ValueError(f"{n} tokens from position {start} on pass max_pos {c.max_pos}")
+            ids_dev = torch.from_numpy(ids).to(self._dev)
+            h = torch.empty((n, c.hidden), dtype=f32, device=self._dev)
+            for t in range(n):
+                _lib.check(lib.frc_embed_row(self._emb_quant, self._emb.data_ptr(), c.hidden, ids_dev[t:].data_ptr(),
+                                             h[t].data_ptr(), self._st), lib)
+
+            def norm(x, w):
+                y = torch.empty_like(x)
+                _lib.check(lib.frc_rmsnorm(x.data_ptr(), w.data_ptr(), n, x.shape[1], c.eps, y.data_ptr(), self._st),
+                           lib)
+                return y
+
+            def project(name, x):
+                # rows scaled by powers of two to below 2, so that none leaves fp16's range in the GEMM
+                w, quant, rows, k = self._w[name]
+                up = torch.exp2(torch.floor(torch.log2(x.abs().amax(dim=1, keepdim=True).clamp(min=1e-30))))
+                x = x / up
+                y = torch.empty((n, rows), dtype=f32, device=self._dev)
+                _lib.check(lib.frc_gemv(quant, w.data_ptr(), w.numel(), rows, k, x.data_ptr(), n, y.data_ptr(), self._st),
+                           lib)
+                return y.mul_(up)
+
+            pos = torch.arange(start, start + n, dtype=torch.int32, device=self._dev)
+            cu_q, cu_k = (torch.tensor([0, m], dtype=torch.int32, device=self._dev) for m in (n, start + n))
+            for i in range(c.layers):
+                p = f"model.layers.{i}"
+                x = norm(h, self._norm[f"{p}.input_layernorm.weight"])
+                qkv = torch.cat([project(f"{p}.{m}.weight", x) for m in _PROJ[:3]], dim=1)
+                parts = tuple(t.unflatten(1, (-1, hd)) for t in qkv.split((c.hidden, kvd, kvd), dim=1))
+                q, k, v = attention.qk_norm_rope(qkv, c.heads, c.kv_heads, self._cos, self._sin, pos,
+                                                 bias=self._bias.get(i), out=parts)
+                self._store(i, start, k, v)
+                k, v = k.half(), v.half()
+                if start:
+                    if self.kv_bits == 4:
+                        slots = torch.arange(start, dtype=torch.int64, device=self._dev)
+                        past = attention.kv_read_q4(self.q4_cache[i], slots, dtype=torch.float16)
+                    else:
+                        past = (self.k_cache[i][:start].half(), self.v_cache[i][:start].half())
+                    k, v = (torch.cat(t) for t in zip(past, (k, v)))
+                ctx = attention.attention_prefill(q.half(), k, v, cu_q, cu_k, scale=float(np.float32(1.0 / np.sqrt(hd))))
+                h += project(f"{p}.self_attn.o_proj.weight", ctx.reshape(n, c.hidden).float())
+                x = norm(h, self._norm[f"{p}.post_attention_layernorm.weight"])
+                gate = torch.nn.functional.silu(project(f"{p}.mlp.gate_proj.weight", x))
+                h += project(f"{p}.mlp.down_proj.weight", gate * project(f"{p}.mlp.up_proj.weight", x))
+            self.h.copy_(h[-1])
+            self._gemv(["lm_head.weight"], self.h, [self.logits], norm=self._norm["model.norm.weight"])
+            _lib.check(lib.frc_argmax(self.logits.data_ptr(), c.vocab, self.tok_out.data_ptr(), self.argmax_ws.data_ptr(),
+                                      self._st), lib)
+            self.tok_in.copy_(self.tok_out)
+            self.pos += n
+            if self.kv_bits == 4:
+                self._slot += n
+                self._length += n
 
     def logits_host(self) -> np.ndarray:
         self.stream.synchronize()

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from flatrun_b200 import attention as A
-from tests import q4_restated as R
+import q4_restated as R
 
 pytestmark = pytest.mark.gpu
 
@@ -473,3 +473,100 @@ def test_calls_on_two_streams_at_once():
     torch.cuda.synchronize()
     for i in (0, 1):
         assert all(torch.equal(g, alone[i]) for g in got[i])
+
+
+# ---- the decode engine's paths ---------------------------------------------------------------
+def _engine(**kw):
+    import qwen2_restated as Q
+    from flatrun_b200.decode import DecodeEngine, DecoderConfig
+
+    s = Q.TINY
+    scaling = kw.pop("rope_scaling", None)
+    cfg = DecoderConfig(s.H, s.F, s.V, s.L, s.NH, s.NKV, s.EPS, s.THETA, 100, scaling)
+    return DecodeEngine(cfg, Q.build(s), lambda name: Q.quant_of(s, name), **kw)
+
+
+def _run(eng, tokens):
+    out = []
+    for t in tokens:
+        eng.step(int(t))
+        out.append(eng.logits_host())
+    return np.stack(out)
+
+
+def test_engine_with_a_4_bit_cache():
+    """The 4-bit engine runs eagerly and captured with the same logits, and its first layer's cache holds what the
+    fp32 engine's does, to half a step."""
+    tokens = np.random.default_rng(5).integers(0, 320, 40)
+    full = _engine()
+    _run(full, tokens)
+    eager, graph = _engine(kv_bits=4, kv_page=16), _engine(kv_bits=4, kv_page=16)
+    graph.capture()
+    got = _run(eager, tokens)
+    assert np.array_equal(got, _run(graph, tokens))
+    assert np.isfinite(got).all() and int(graph.pos.item()) == 40 and int(graph._slot.item()) == 40
+    k, v = A.kv_read_q4(eager.q4_cache[0], torch.arange(40, device="cuda"))
+    for x, y in ((full.k_cache[0][:40], k), (full.v_cache[0][:40], v)):
+        x = _np(x)
+        _, d, _ = R.quantise(x)
+        # half a step, the roundings of d and m to fp16 (as in the round trip of the oracle), and the engines' own
+        # differences before the cache (rotation in fp32: 8 roundings)
+        bound = np.repeat(d, 32, -1) * (0.5 + 15 * 2.0 ** -11) + np.abs(x).max() * (2.0 ** -11 + 16 * E32)
+        _close(y, x, bound)
+    # the last layer's attention of the last token, from the queries and the cache that the engine holds
+    q = eager.qkv[:eager.cfg.hidden].view(1, -1, 64)
+    o, bound = _decode_ref(eager.q4_cache[-1], eager._table, torch.tensor([40]), _np(q), 0.125, "fp32", 16)
+    _close(eager.ctx.view(1, -1, 64), o, bound)
+
+
+@pytest.mark.parametrize("bits", [32, 4])
+@pytest.mark.parametrize("parts", [(33,), (1, 5), (20, 17)])
+def test_engine_prefill(bits, parts):
+    """A prompt at once (and a second one behind it), then single tokens, against the same tokens one by one.
+
+    The first layer's keys and values differ by the fp16 roundings of the batched projection's operands: 2 * 2^-11 of the
+    sum of |x w| over 256 products, which is below three times the largest key (for products of one size with random
+    signs it is 0.8 * 16 times the spread of the keys), and in 4 bits by a step more (a rounding can fall the other way).
+    Later layers of this random model have scores of thousands, where a near tie between two keys can go either way
+    anywhere, so beyond the first layer only the last token's logits are compared, loosely."""
+    rng = np.random.default_rng(sum(parts))
+    prompts = [rng.integers(0, 320, n) for n in parts]
+    one, eng = _engine(kv_bits=bits), _engine(kv_bits=bits)
+    for t in np.concatenate(prompts):
+        one.step(int(t))
+    ref = one.logits_host().copy()
+    for p in prompts:
+        eng.prefill(p)
+    n = sum(parts)
+    got = eng.logits_host().copy()
+    assert eng.argmax_host() == int(np.argmax(got)) and int(eng.pos.item()) == n
+    if bits == 32:
+        pairs = [(c[0][:n], d[0][:n]) for c, d in ((one.k_cache, eng.k_cache), (one.v_cache, eng.v_cache))]
+        assert np.abs(got - ref).max() <= 2e-2 * np.abs(ref).max()
+    else:
+        slots = torch.arange(n, device="cuda")
+        pairs = zip(A.kv_read_q4(one.q4_cache[0], slots), A.kv_read_q4(eng.q4_cache[0], slots))
+    for x, y in pairs:
+        x = _np(x)
+        _, d, _ = R.quantise(x)
+        step = 0 if bits == 32 else np.repeat(d, 32, -1) * (1 + 2.0 ** -10 * 15)
+        _close(y, x, 2 * 2.0 ** -11 * 3 * np.abs(x).max() + step)
+    tail = _run(eng, rng.integers(0, 320, 3))
+    assert np.isfinite(tail).all() and int(eng.pos.item()) == n + 3
+
+
+def test_engine_options_and_refusals():
+    with pytest.raises(ValueError, match="kv_bits"):
+        _engine(kv_bits=8)
+    eng = _engine(rope_scaling={"type": "linear", "factor": 2.0})
+    with pytest.raises(ValueError, match="empty"):
+        eng.prefill([])
+    with pytest.raises(ValueError, match="max_pos"):
+        eng.prefill(np.zeros(101, np.int32))
+    eng.step(3)
+    eng.step(5)
+    plain = _engine()
+    plain.step(3)
+    plain.step(5)
+    eng.logits_host(), plain.logits_host()  # (waits for the engines' streams)
+    assert torch.equal(eng.k_cache[0][0], plain.k_cache[0][0]) and not torch.equal(eng.k_cache[0][1], plain.k_cache[0][1])

@@ -11,7 +11,7 @@ import pytest
 import torch
 
 from flatrun_b200 import _lib, attention as A
-from tests import q4_restated as R
+import q4_restated as R
 
 
 @pytest.fixture(scope="module")
