@@ -69,11 +69,73 @@ constexpr int kPfTiles = 2;      // query tiles of a CTA
 constexpr int kPfThreads = 384;
 // Registers: the CTA is launched with 168 a thread; the softmax warps, which
 // hold a row of scores, take over what the other four warps leave (two of
-// them are there for that alone): 2 * 216 + 72 = 3 * 168.
-constexpr int kPfRegsSoftmax = 216, kPfRegsOther = 72;
+// them are there for that alone): 2 * 224 + 56 = 3 * 168.
+constexpr int kPfRegsSoftmax = 224, kPfRegsOther = 56;
 constexpr int kPfFirst = 64;     // keys whose P is handed over before the rest
 static_assert(kPfFirst % 32 == 0 && kPfFirst >= 64 && kPfFirst < kPfRows, "a multiple of 32 behind the first 32");
 constexpr float kPfSlack = 8.f;  // powers of two that the reference may stay behind
+
+// A work item.
+struct PfWork {
+  int head, kvh;                       // first query head, KV head
+  int q_start, q_len, k_start, k_len;  // the sequence
+  int q0;                              // first query of the item in it
+  // Item `block`: of its heads, block `block / units` of the queries, from the last
+  // one on (the longest first where there is one sequence).  All lanes of a warp
+  // call it.  False: there is none, nor any behind it.
+  FRC_DEVICE_INLINE bool find(const PrefillParams& p, int block, int lane) {
+    const int units = p.nh / p.heads;
+    int rank = block / units;
+    head = (block - rank * units) * p.heads;
+    kvh = head / (p.nh / p.nkv);
+    const int span = kPfTiles * p.queries;
+    for (int top = p.batch; top > 0; top -= 32) {
+      const int b = top - 1 - lane;
+      int a0 = 0, a1 = 0, k0 = 0, k1 = 0;
+      if (b >= 0) {
+        a0 = min(max(p.cu_q[b], 0), p.tokens_q);
+        a1 = min(max(p.cu_q[b + 1], a0), p.tokens_q);
+        k0 = min(max(p.cu_k[b], 0), p.tokens_k);
+        k1 = min(max(p.cu_k[b + 1], k0), p.tokens_k);
+      }
+      const int n = (a1 - a0 + span - 1) / span;
+      int incl = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, rank < incl);
+      if (!hit) {
+        rank -= __shfl_sync(0xffffffffu, incl, 31);
+        continue;
+      }
+      const int l = __ffs(hit) - 1;
+      q_start = __shfl_sync(0xffffffffu, a0, l);
+      q_len = __shfl_sync(0xffffffffu, a1, l) - q_start;
+      const int blocks = __shfl_sync(0xffffffffu, n, l);
+      const int in_seq = rank - (__shfl_sync(0xffffffffu, incl, l) - blocks);
+      q0 = (blocks - 1 - in_seq) * span;
+      k_start = __shfl_sync(0xffffffffu, k0, l);
+      k_len = __shfl_sync(0xffffffffu, k1, l) - k_start;
+      return true;
+    }
+    return false;
+  }
+  // Queries of a tile.
+  FRC_DEVICE_INLINE int queries(const PrefillParams& p, int tile) const {
+    return min(max(q_len - q0 - tile * p.queries, 0), p.queries);
+  }
+  // Keys that query `i` of the sequence sees.
+  FRC_DEVICE_INLINE int seen(const PrefillParams& p, int i) const {
+    return p.causal ? min(max(i + 1 + k_len - q_len, 0), k_len) : k_len;
+  }
+  // Key tiles of a query tile.
+  FRC_DEVICE_INLINE int tiles(const PrefillParams& p, int tile) const {
+    const int n = queries(p, tile);
+    return n == 0 ? 0 : (seen(p, q0 + tile * p.queries + n - 1) + kPfRows - 1) / kPfRows;
+  }
+};
 
 template <int HD>
 struct PfSmem {
@@ -84,8 +146,11 @@ struct PfSmem {
   alignas(1024) uint8_t ring[kStages][kTile];
   uint64_t q_full, q_empty, full[kStages], empty[kStages];
   uint64_t s_full[kPfTiles], p_ready[kPfTiles][2], o_done[kPfTiles], o_free[kPfTiles], drain;
-  alignas(16) uint4 next[2];  // answers to the requests for the next item, by turns
-  uint64_t next_full[2], next_empty[2];
+  alignas(16) uint4 answer;  // to the request for the next block
+  uint64_t answered;
+  PfWork work[2];            // items 1, 2, ... by turns
+  int any[2];                // whether there is one
+  uint64_t work_full[2], work_empty[2];
   uint32_t tmem;
   int abort;
 };
@@ -274,68 +339,6 @@ FRC_DEVICE_INLINE int pf_answer(const uint4* answer) {
   return block;
 }
 
-// A work item.
-struct PfWork {
-  int head, kvh;                       // first query head, KV head
-  int q_start, q_len, k_start, k_len;  // the sequence
-  int q0;                              // first query of the item in it
-  // Item `block`: of its heads, block `block / units` of the queries, from the last
-  // one on (the longest first where there is one sequence).  All lanes of a warp
-  // call it.  False: there is none, nor any behind it.
-  FRC_DEVICE_INLINE bool find(const PrefillParams& p, int block, int lane) {
-    const int units = p.nh / p.heads;
-    int rank = block / units;
-    head = (block - rank * units) * p.heads;
-    kvh = head / (p.nh / p.nkv);
-    const int span = kPfTiles * p.queries;
-    for (int top = p.batch; top > 0; top -= 32) {
-      const int b = top - 1 - lane;
-      int a0 = 0, a1 = 0, k0 = 0, k1 = 0;
-      if (b >= 0) {
-        a0 = min(max(p.cu_q[b], 0), p.tokens_q);
-        a1 = min(max(p.cu_q[b + 1], a0), p.tokens_q);
-        k0 = min(max(p.cu_k[b], 0), p.tokens_k);
-        k1 = min(max(p.cu_k[b + 1], k0), p.tokens_k);
-      }
-      const int n = (a1 - a0 + span - 1) / span;
-      int incl = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-      }
-      const uint32_t hit = __ballot_sync(0xffffffffu, rank < incl);
-      if (!hit) {
-        rank -= __shfl_sync(0xffffffffu, incl, 31);
-        continue;
-      }
-      const int l = __ffs(hit) - 1;
-      q_start = __shfl_sync(0xffffffffu, a0, l);
-      q_len = __shfl_sync(0xffffffffu, a1, l) - q_start;
-      const int blocks = __shfl_sync(0xffffffffu, n, l);
-      const int in_seq = rank - (__shfl_sync(0xffffffffu, incl, l) - blocks);
-      q0 = (blocks - 1 - in_seq) * span;
-      k_start = __shfl_sync(0xffffffffu, k0, l);
-      k_len = __shfl_sync(0xffffffffu, k1, l) - k_start;
-      return true;
-    }
-    return false;
-  }
-  // Queries of a tile.
-  FRC_DEVICE_INLINE int queries(const PrefillParams& p, int tile) const {
-    return min(max(q_len - q0 - tile * p.queries, 0), p.queries);
-  }
-  // Keys that query `i` of the sequence sees.
-  FRC_DEVICE_INLINE int seen(const PrefillParams& p, int i) const {
-    return p.causal ? min(max(i + 1 + k_len - q_len, 0), k_len) : k_len;
-  }
-  // Key tiles of a query tile.
-  FRC_DEVICE_INLINE int tiles(const PrefillParams& p, int tile) const {
-    const int n = queries(p, tile);
-    return n == 0 ? 0 : (seen(p, q0 + tile * p.queries + n - 1) + kPfRows - 1) / kPfRows;
-  }
-};
-
 // Query `row` of head h from the keys it sees alone: a warp, HD / 32 channels a lane.
 template <typename T, int HD>
 __device__ __noinline__ void pf_row_again(const PrefillParams& p, const PfWork& w, int h, int row, int lane) {
@@ -397,9 +400,10 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       mbar_init(&sh->p_ready[t][1], 4);
       mbar_init(&sh->o_done[t], 1);
       mbar_init(&sh->o_free[t], 4);
-      mbar_init(&sh->next_full[t], 1);
-      mbar_init(&sh->next_empty[t], 9);  // the softmax warps and the product warp
+      mbar_init(&sh->work_full[t], 1);
+      mbar_init(&sh->work_empty[t], 9);  // the softmax warps and the product warp
     }
+    mbar_init(&sh->answered, 1);
     mbar_init(&sh->drain, 1);
     sh->abort = 0;
     fence_barrier_init();
@@ -416,10 +420,10 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   }
   if (warp == 9 && lane == 0)
     for (const CUtensorMap* map : {&qmap, &kmap, &vmap}) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
-  // Item `i` of this CTA: the block it was launched as, then those it took over.
+  // Item 0 of this CTA is the block it was launched as; the others are blocks it
+  // took over, found by the loading warp an item ahead.
   PfWork w;
-  int block = blockIdx.x;
-  bool any = w.find(p, block, lane);  // false: there is none, nor any behind it
+  bool any = w.find(p, blockIdx.x, lane);  // false: there is none, nor any behind it
   pf_fence_before();
   __syncthreads();
   pf_fence_after();
@@ -429,19 +433,25 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     return __all_sync(0xffffffffu, wait_phase(bar, parity & 1, abort));
   };
 
+  auto follow = [&](int i) {  // item i + 1 into w and any
+    const int slot = (i + 1) & 1;
+    if (!wait(&sh->work_full[slot], i >> 1)) return false;
+    w = sh->work[slot];
+    any = sh->any[slot] != 0;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh->work_empty[slot]);
+    return true;
+  };
+
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPfRegsOther));
     if (warp == 9) {
       // ---- loads -----------------------------------------------------------------------
       int issued = 0, items = 0;  // K and V tiles, items that had queries
       bool ok = true;
-      for (int i = 0;; ++i) {
-        // the request for item i + 1, when the answer before the last has been read
-        if (i >= 2) ok = wait(&sh->next_empty[i & 1], (i >> 1) - 1) && ok;
-        if (!ok) break;
-        if (lane == 0) pf_ask(&sh->next[i & 1], &sh->next_full[i & 1]);
-        if (i > 0) any = w.find(p, block, lane);
-        const int n = any ? max(w.tiles(p, 0), w.tiles(p, 1)) : 0;
+      for (int i = 0; any; ++i) {
+        if (lane == 0) pf_ask(&sh->answer, &sh->answered);
+        const int n = max(w.tiles(p, 0), w.tiles(p, 1));
         if (n > 0) {
           if (items > 0) ok = wait(&sh->q_empty, items - 1);
           if (ok && lane == 0) {
@@ -469,9 +479,17 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         }
         // the answer is waited for in any case: it must not land after the CTA
         int zero = 0;
-        ok = __all_sync(0xffffffffu, wait_phase(&sh->next_full[i & 1], (i >> 1) & 1, &zero)) && ok;
-        block = pf_answer(&sh->next[i & 1]);
-        if (!ok || !any || block < 0) break;
+        ok = __all_sync(0xffffffffu, wait_phase(&sh->answered, i & 1, &zero)) && ok;
+        const int block = pf_answer(&sh->answer), slot = (i + 1) & 1;
+        any = ok && block >= 0 && w.find(p, block, lane);
+        if (i >= 2) ok = ok && wait(&sh->work_empty[slot], (i >> 1) - 1);
+        if (!ok) break;
+        if (lane == 0) {
+          sh->work[slot] = w;
+          sh->any[slot] = any;
+          mbar_arrive(&sh->work_full[slot]);
+        }
+        __syncwarp();
       }
       if (!ok) {
         *abort = 1;
@@ -509,9 +527,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       bool ok = true;
       int used = 0, items = 0;                           // K and V tiles, items that had queries
       int done[kPfTiles] = {0, 0}, outs[kPfTiles] = {0, 0};  // key tiles and items of each query tile
-      for (int i = 0; ok; ++i) {
-        if (i > 0) any = w.find(p, block, lane);
-        const int nt[kPfTiles] = {any ? w.tiles(p, 0) : 0, any ? w.tiles(p, 1) : 0};
+      for (int i = 0; ok && any; ++i) {
+        const int nt[kPfTiles] = {w.tiles(p, 0), w.tiles(p, 1)};
         const int n = max(nt[0], nt[1]);
         if (n > 0) {
           ok = wait(&sh->q_full, items) && wait(&sh->full[used % NS], used / NS);
@@ -571,12 +588,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           }
           for (int t = 0; t < kPfTiles; ++t) outs[t] += nt[t] > 0;
         }
-        ok = ok && wait(&sh->next_full[i & 1], i >> 1);
-        if (!ok) break;
-        block = pf_answer(&sh->next[i & 1]);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->next_empty[i & 1]);
-        if (!any || block < 0) break;
+        ok = ok && follow(i);
       }
       if (!ok) {
         *abort = 1;
@@ -598,10 +610,9 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     const uint64_t scale2 = pf_two(scale, scale);
     bool ok = true;
     int done = 0;  // key tiles
-    for (int i = 0; ok; ++i) {
-      if (i > 0) any = w.find(p, block, lane);
-      const int nt = any ? w.tiles(p, t) : 0, row = w.q0 + p.queries * t + my_query;
-      const bool live = any && my_query < w.queries(p, t);
+    for (int i = 0; ok && any; ++i) {
+      const int nt = w.tiles(p, t), row = w.q0 + p.queries * t + my_query;
+      const bool live = my_query < w.queries(p, t);
       const int seen = live ? w.seen(p, row) : w.k_len;  // rows without a query: nothing to mask
       float m_ref = -INFINITY, base = 0.f, sum = 0.f;  // reference in units of the unscaled score, and scaled
       for (int j = 0; j < nt; ++j, ++done) {
@@ -707,12 +718,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       for (uint32_t again = __ballot_sync(0xffffffffu, live && !finite); again; again &= again - 1)
         pf_row_again<T, HD>(p, w, w.head + __shfl_sync(0xffffffffu, my_head, __ffs(again) - 1),
                             __shfl_sync(0xffffffffu, row, __ffs(again) - 1), lane);
-      ok = wait(&sh->next_full[i & 1], i >> 1);
-      if (!ok) break;
-      block = pf_answer(&sh->next[i & 1]);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->next_empty[i & 1]);
-      if (!any || block < 0) break;
+      ok = follow(i);
     }
     if (!ok && lane == 0) atomicOr(p.status, kStatusFullWaitTimeout);
   }
