@@ -35,7 +35,7 @@ struct KvQ4Params {
   int64_t k_tok, k_head, v_tok, v_head;  // strides in elements
 };
 
-constexpr int kQ4Threads = 256;
+constexpr int kQ4Threads = 128;
 
 // The least and the largest of three, NaN if one is.
 FRC_DEVICE_INLINE float min_nan(float a, float b, float c) {
@@ -59,6 +59,29 @@ FRC_DEVICE_INLINE __half step_of(float hi, float m) {
   const uint32_t low = __float_as_uint(f) & 0x1fffu;
   if (f > 6.2e-5f && (low < 0x1000u - 4u || low > 0x1000u + 4u)) return __float2half_rn(f);
   return __double2half(fmin(fmax((static_cast<double>(hi) - static_cast<double>(m)) / 15.0, 0.0), 65504.0));
+}
+
+// The nibbles of eight values by the side of the border that each lies on: where
+// a lane has one that is too near for fp32's quotient, as 16-bit values often
+// are (they meet borders exactly).  Out of line, so that the callers' code stays
+// in the instruction cache.
+__device__ __noinline__ uint32_t border8(float x0, float x1, float x2, float x3, float x4, float x5, float x6, float x7,
+                                         float m, float d, float inv) {
+  const float x[8] = {x0, x1, x2, x3, x4, x5, x6, x7};
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    // h: the border nearest to 15 t; e: on which side of it x - m lies.  s + err is
+    // x - m exactly (two-sum), and s - h d is exact near the border
+    const float t = 15.f * __saturatef((x[i] - m) * inv);
+    const float h = fminf(fmaxf(rintf(t - 0.5f), 0.f), 14.f) + 0.5f;
+    const float s = __fsub_rn(x[i], m), v = __fsub_rn(s, x[i]);
+    const float err = __fsub_rn(__fsub_rn(x[i], __fsub_rn(s, v)), __fadd_rn(m, v));
+    const float e = __fadd_rn(__fmaf_rn(-h, d, s), err);
+    const float n = e > 0.f ? h + 0.5f : (e < 0.f ? h - 0.5f : 2.f * rintf(0.5f * h));  // on it: the even one
+    w |= static_cast<uint32_t>(n) << (4 * i);
+  }
+  return w;
 }
 
 // The lane's eight values of a group shared by the four lanes of its quad:
@@ -109,21 +132,7 @@ FRC_DEVICE_INLINE uint32_t quantise8(const float (&x)[8], __half& step, __half& 
   // the sums' other bits, 0x4B400000 each, add up to this
   constexpr uint32_t kSum = 0x4B400000u * 0x11111111u;
   w -= kSum;
-  if (far > 0.5f - 6e-6f) {  // common where 16-bit values meet the border exactly
-    w = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      // h: the border nearest to 15 t; e: on which side of it x - m lies.  s + err is
-      // x - m exactly (two-sum), and s - h d is exact near the border
-      const float t = 15.f * __saturatef((x[i] - m) * inv);
-      const float h = fminf(fmaxf(rintf(t - 0.5f), 0.f), 14.f) + 0.5f;
-      const float s = __fsub_rn(x[i], m), v = __fsub_rn(s, x[i]);
-      const float err = __fsub_rn(__fsub_rn(x[i], __fsub_rn(s, v)), __fadd_rn(m, v));
-      const float e = __fadd_rn(__fmaf_rn(-h, d, s), err);
-      const float n = e > 0.f ? h + 0.5f : (e < 0.f ? h - 0.5f : 2.f * rintf(0.5f * h));  // on it: the even one
-      w |= static_cast<uint32_t>(n) << (4 * i);
-    }
-  }
+  if (far > 0.5f - 6e-6f) w = border8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], m, d, inv);
   return w;
 }
 
@@ -158,7 +167,7 @@ FRC_DEVICE_INLINE bool q4_warp_item(const KvQ4Params& p, int64_t& tok, int& is_v
 }
 
 template <typename T, int HD, bool VEC>
-__global__ void __launch_bounds__(kQ4Threads, 4) kv_append_q4_kernel(KvQ4Params p) {
+__global__ void __launch_bounds__(kQ4Threads, 8) kv_append_q4_kernel(KvQ4Params p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" :::);
   constexpr Q4Layout lay(HD);
