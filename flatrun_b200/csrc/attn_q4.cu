@@ -101,7 +101,7 @@ struct AqSmem {
   static constexpr int kRow = HD + 4;  // floats of a head in a piece
   static constexpr int kPieces = 2 * kAqWarps;  // of each warp: the unit that ends in its range, the one that goes on
   alignas(128) uint8_t ring[kAqWarps][kStages][2][kBlock];
-  float m[kPieces][kAqHeads], l[kPieces][kAqHeads];
+  alignas(16) float m[kAqHeads][kPieces], l[kAqHeads][kPieces];
   int4 piece[kPieces];  // (sequence or -1, unit, start, end) in places of the CTA's range
   uint64_t full[kAqWarps][kStages];
   int64_t scan[kAqWarps];
@@ -234,9 +234,11 @@ struct AqWarp {
       for (int i = 0; i < 8; ++i) {
         y[i] = x[j][i] * up;
         sum[j] += y[i];
-        const float h = __half2float(__float2half_rn(y[i]));
-        lo[i] = (y[i] - h) * 2048.f;
-        y[i] = h;
+        if constexpr (SPLIT) {
+          const float h = __half2float(__float2half_rn(y[i]));
+          lo[i] = (y[i] - h) * 2048.f;
+          y[i] = h;
+        }
       }
       sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
       sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
@@ -246,8 +248,13 @@ struct AqWarp {
       for (int s = 0; s < 2; ++s) {
         a[j][s][0] = pack_half2(y[2 * s], y[2 * s + 4]);
         a[j][s][1] = pack_half2(y[2 * s + 1], y[2 * s + 5]);
-        a[j][s][2] = pack_half2(lo[2 * s], lo[2 * s + 4]);  // zeros for 16-bit types
-        a[j][s][3] = pack_half2(lo[2 * s + 1], lo[2 * s + 5]);
+        if constexpr (SPLIT) {
+          a[j][s][2] = pack_half2(lo[2 * s], lo[2 * s + 4]);
+          a[j][s][3] = pack_half2(lo[2 * s + 1], lo[2 * s + 5]);
+        } else {  // zeros that the compiler keeps in place: the fragment is four neighbouring registers
+          asm volatile("mov.b32 %0, 0;" : "=r"(a[j][s][2]));
+          asm volatile("mov.b32 %0, 0;" : "=r"(a[j][s][3]));
+        }
       }
     }
     // contraction index 2 q, 2 q + 1: the sums of two groups, high parts first, then low parts
@@ -699,8 +706,8 @@ __global__ void __launch_bounds__(kAqThreads, 2) attn_q4_kernel(const AttnQ4Para
           *reinterpret_cast<float4*>(rows + h * SM::kRow + c) = make_float4(v[0], v[1], v[2], v[3]);
         });
         if ((lane & 3) == 0) {
-          sh->m[k][lane >> 2] = st.m_run;
-          sh->l[k][lane >> 2] = st.l_run;
+          sh->m[lane >> 2][k] = st.m_run;
+          sh->l[lane >> 2][k] = st.l_run;
         }
         if (lane == 0) sh->piece[k] = make_int4(walk.seq, walk.unit, walk.u0, walk.end());
       }
@@ -724,28 +731,33 @@ __global__ void __launch_bounds__(kAqThreads, 2) attn_q4_kernel(const AttnQ4Para
     left &= ~same;
     const AqHeads heads(p, unit);
     if (warp < heads.count) {
-      constexpr int C = HD / 32;
-      const bool mine = same >> lane & 1u;
-      float M = mine ? sh->m[lane][warp] : -INFINITY;
-      const float m = M;
+      constexpr int C = HD / 32, N = SM::kPieces;
+      float m[N], l[N];
+      load_run<N, true>(sh->m[warp], m);
+      load_run<N, true>(sh->l[warp], l);
+      float M = -INFINITY, L = 0.f, acc[C];
 #pragma unroll
-      for (int o = 1; o < SM::kPieces; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-      M = __shfl_sync(0xffffffffu, M, 0);
-      const float f = mine ? ex2(m - (M == -INFINITY ? 0.f : M)) : 0.f;
-      float L = mine ? sh->l[lane][warp] * f : 0.f, acc[C];
-#pragma unroll
-      for (int o = 1; o < SM::kPieces; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-      L = __shfl_sync(0xffffffffu, L, 0);
+      for (int j = 0; j < N; ++j) M = fmaxf(M, same >> j & 1u ? m[j] : -INFINITY);
+      const float base = M == -INFINITY ? 0.f : M;
 #pragma unroll
       for (int e = 0; e < C; ++e) acc[e] = 0.f;
-#pragma unroll 4
-      for (uint32_t todo = same; todo; todo &= todo - 1) {
-        const int j = __ffs(todo) - 1;
-        const float fj = __shfl_sync(0xffffffffu, f, j);
-        float v[C];
-        load_run<C, true>(piece_rows(j) + warp * SM::kRow + C * lane, v);
 #pragma unroll
-        for (int e = 0; e < C; ++e) acc[e] = fmaf(v[e], fj, acc[e]);
+      for (int j0 = 0; j0 < N; j0 += 8) {  // eight pieces' loads at a time
+        float v[8][C];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+#pragma unroll
+          for (int e = 0; e < C; ++e) v[j][e] = 0.f;
+          if (same >> (j0 + j) & 1u) load_run<C, true>(piece_rows(j0 + j) + warp * SM::kRow + C * lane, v[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool in = same >> (j0 + j) & 1u;
+          const float f = in ? ex2(m[j0 + j] - base) : 0.f;
+          L = fmaf(in ? l[j0 + j] : 0.f, f, L);
+#pragma unroll
+          for (int e = 0; e < C; ++e) acc[e] = fmaf(v[j][e], f, acc[e]);
+        }
       }
       if (u0 >= 0 && u1 <= count) {
         aq_store<C, T>(p, seq, heads.first + warp, C * lane, acc, L);
@@ -763,63 +775,71 @@ __global__ void __launch_bounds__(kAqThreads, 2) attn_q4_kernel(const AttnQ4Para
   }
 }
 
-// Joins the pieces of a unit that the CTAs' ranges cut, in their order: block
-// (i, h) the head h of the unit that is cut at the end of CTA i's range.
-constexpr int kAqJoin = 256;
+// Joins the pieces of a unit that the CTAs' ranges cut: block (i, h) head h of the
+// unit that is cut at the end of CTA i's range, each warp every fourth piece.
+constexpr int kAqJoinWarps = 4;
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kAqJoin) attn_q4_join_kernel(const AttnQ4Params p) {
+__global__ void __launch_bounds__(kAqJoinWarps * 32) attn_q4_join_kernel(const AttnQ4Params p) {
   griddep_wait();
   griddep_launch_dependents();
-  constexpr int ROW = AqSmem<HD>::kRow, L4 = HD / 4, G = kAqJoin / L4;  // lanes of four channels, G ranges at a time
+  constexpr int ROW = AqSmem<HD>::kRow, C = HD / 32;
   const int4 d = p.desc[blockIdx.x];
   if (d.x < 0) return;
-  const int h = blockIdx.y;
+  const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const AqHeads heads(p, d.y);
   if (h >= heads.count) return;
-  const int np = d.z + 1, tid = threadIdx.x;
-  __shared__ float f[kAqGrid];
-  __shared__ float red[kAqJoin / 32];
-  __shared__ __align__(16) float acc[G][HD];
-  auto row = [&](int k) {  // the cut unit starts in CTA i (its second part) and goes on as the others' first
+  const int np = d.z + 1;
+  auto row = [&](int k) {  // the cut unit starts in CTA i (its second piece) and goes on as the others' first
     return p.part + (static_cast<int64_t>(k == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + k)) * kAqHeads + h) * ROW;
   };
-  float M = -INFINITY;
-  for (int k = tid; k < np; k += kAqJoin) M = fmaxf(M, row(k)[0]);
+  float M = -INFINITY;  // of all pieces, in every warp
+  for (int k = lane; k < np; k += 32) M = fmaxf(M, row(k)[0]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  if ((tid & 31) == 0) red[tid >> 5] = M;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kAqJoin / 32; ++w) M = fmaxf(M, red[w]);
   const float base = M == -INFINITY ? 0.f : M;
-  for (int k = tid; k < np; k += kAqJoin) f[k] = ex2(row(k)[0] - base);
-  __syncthreads();
-  const int g = tid / L4, c = 4 * (tid % L4);
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  float L = 0.f;
-#pragma unroll 4
-  for (int k = g; k < np; k += G) {
-    const float4 v = *reinterpret_cast<const float4*>(row(k) + 4 + c);
-    L = fmaf(row(k)[1], f[k], L);
-    a.x = fmaf(v.x, f[k], a.x);
-    a.y = fmaf(v.y, f[k], a.y);
-    a.z = fmaf(v.z, f[k], a.z);
-    a.w = fmaf(v.w, f[k], a.w);
-  }
-  *reinterpret_cast<float4*>(&acc[g][c]) = a;
-  __shared__ float ls[G];
-  if (c == 0) ls[g] = L;
-  __syncthreads();
-  if (tid < L4) {
-    float v[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+  float L = 0.f, acc[C];
 #pragma unroll
-    for (int k = 0; k < G; ++k) {
-      sum += ls[k];
+  for (int e = 0; e < C; ++e) acc[e] = 0.f;
+  for (int k = warp; k < np; k += 8 * kAqJoinWarps) {  // eight pieces' loads at a time
+    float v[8][C], m[8], l[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += acc[k][c + e];
+    for (int j = 0; j < 8; ++j) {
+      const int kj = k + j * kAqJoinWarps;
+      m[j] = -INFINITY;
+      l[j] = 0.f;
+#pragma unroll
+      for (int e = 0; e < C; ++e) v[j][e] = 0.f;
+      if (kj < np) {
+        const float* r = row(kj);
+        m[j] = r[0];
+        l[j] = r[1];
+        load_run<C, true>(r + 4 + C * lane, v[j]);
+      }
     }
-    aq_store<4, T>(p, d.x, heads.first + h, c, v, sum);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float f = ex2(m[j] - base);
+      L = fmaf(l[j], f, L);
+#pragma unroll
+      for (int e = 0; e < C; ++e) acc[e] = fmaf(v[j][e], f, acc[e]);
+    }
+  }
+  __shared__ __align__(16) float sums[kAqJoinWarps][HD];
+  __shared__ float ls[kAqJoinWarps];
+  store_run<C, true>(&sums[warp][C * lane], acc);
+  if (lane == 0) ls[warp] = L;
+  __syncthreads();
+  if (warp == 0) {
+#pragma unroll
+    for (int w = 1; w < kAqJoinWarps; ++w) {
+      float v[C];
+      load_run<C, true>(&sums[w][C * lane], v);
+      L += ls[w];
+#pragma unroll
+      for (int e = 0; e < C; ++e) acc[e] += v[e];
+    }
+    aq_store<C, T>(p, d.x, heads.first + h, C * lane, acc, L);
   }
 }
 
@@ -844,7 +864,8 @@ cudaError_t launch_attn_q4(AttnQ4Params p, int grid, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   e = launch_pdl(attn_q4_kernel<T, HD>, dim3(grid), dim3(kAqThreads), sizeof(AqSmem<HD>), st, p);
   if (e != cudaSuccess || grid == 1) return e;
-  return launch_pdl(attn_q4_join_kernel<T, HD>, dim3(grid, min(kAqHeads, p.nh / p.nkv)), dim3(kAqJoin), 0, st, p);
+  return launch_pdl(attn_q4_join_kernel<T, HD>, dim3(grid, min(kAqHeads, p.nh / p.nkv)), dim3(kAqJoinWarps * 32), 0,
+                    st, p);
 }
 
 }  // namespace frc
