@@ -268,26 +268,6 @@ FRC_DEVICE_INLINE uint32_t pf_pack(float lo, float hi) {
   }
 }
 
-// Two fp32 operations in one instruction.
-FRC_DEVICE_INLINE uint64_t pf_two(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-FRC_DEVICE_INLINE void pf_split(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-FRC_DEVICE_INLINE uint64_t pf_fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-FRC_DEVICE_INLINE uint64_t pf_add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
 FRC_DEVICE_INLINE float pf_max3(float a, float b, float c) {
   float y;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
@@ -300,15 +280,15 @@ FRC_DEVICE_INLINE float pf_max3(float a, float b, float c) {
 // for 64 heads of 8192 tokens.)
 template <typename T>
 FRC_DEVICE_INLINE void pf_exps(const uint32_t* x, uint64_t scale2, float base, uint64_t (&part)[4], uint32_t (&y)[16]) {
-  const uint64_t base2 = pf_two(base, base);
+  const uint64_t base2 = f32x2_two(base, base);
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
-    const uint64_t v = pf_fma2(pf_two(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), scale2, base2);
+    const uint64_t v = f32x2_fma(f32x2_two(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), scale2, base2);
     float a, b;
-    pf_split(v, a, b);
+    f32x2_split(v, a, b);
     a = pf_ex2(a);
     b = pf_ex2(b);
-    part[e & 3] = pf_add2(part[e & 3], pf_two(a, b));
+    part[e & 3] = f32x2_add(part[e & 3], f32x2_two(a, b));
     y[e] = pf_pack<T>(a, b);
   }
 }
@@ -607,7 +587,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     const uint32_t s_at = tmem + lanes + 128 * t, o_at = tmem + lanes + 256 + HD * t;
     const int r = 32 * (warp & 3) + lane, my_query = r / p.heads, my_head = r - my_query * p.heads;
     const float scale = p.scale;
-    const uint64_t scale2 = pf_two(scale, scale);
+    const uint64_t scale2 = f32x2_two(scale, scale);
     bool ok = true;
     int done = 0;  // key tiles
     for (int i = 0; ok && any; ++i) {
@@ -681,7 +661,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->p_ready[t][1]);
         float a0, a1;
-        pf_split(pf_add2(pf_add2(part[0], part[1]), pf_add2(part[2], part[3])), a0, a1);
+        f32x2_split(f32x2_add(f32x2_add(part[0], part[1]), f32x2_add(part[2], part[3])), a0, a1);
         sum += a0 + a1;
       }
       // ---- O / sum ---------------------------------------------------------------------

@@ -305,7 +305,8 @@ struct AqWarp {
         const uint2 v = *reinterpret_cast<const uint2*>(blk + lay.k_word(tok, q, 0));
         w[0] = v.x; w[1] = v.y;
       }
-      float cm[4], x0 = 0.f, x1 = 0.f;
+      float cm[4];
+      uint64_t x = 0;  // the scores of tokens 4 q + 2 t and the next, of head r
       mma16816_new(cm, am, 0u, 0u, 0u, *reinterpret_cast<const uint32_t*>(blk + lay.k_offset(tok, 2 * (q % (NG / 2)))),
                    0u);
 #pragma unroll
@@ -321,9 +322,11 @@ struct AqWarp {
           c[1] = fmaf(c[3], 1.f / 2048.f, c[1]);
         }
         const float2 d = __half22float2(bits_h2(t ? kd[j].y : kd[j].x));
-        x0 = j ? fmaf(d.x, c[0], x0) : d.x * c[0];
-        x1 = j ? fmaf(d.y, c[1], x1) : d.y * c[1];
+        const uint64_t d2 = f32x2_two(d.x, d.y), c2 = f32x2_two(c[0], c[1]);
+        x = j ? f32x2_fma(d2, c2, x) : f32x2_mul(d2, c2);
       }
+      float x0, x1;
+      f32x2_split(x, x0, x1);
       s[2 * t] = fmaf(x0, f_n, cm[0] * f_m);
       s[2 * t + 1] = fmaf(x1, f_n, cm[1] * f_m);
     }
@@ -424,7 +427,7 @@ struct AqWarp {
     // rows of a tile: 16 channels of group j: word 4 j + r % 4, of it the nibbles
     // of its low half (r < 4) or high half: 2 t in row r, 2 t + 1 in row r + 8
     const uint32_t sel = r < 4 ? 0x5410u : 0x7632u;
-    const float r0 = p0 * kUp, r1 = p1 * kUp, r2 = p2 * kUp, r3 = p3 * kUp;
+    const uint64_t r01 = f32x2_two(p0 * kUp, p1 * kUp), r23 = f32x2_two(p2 * kUp, p3 * kUp);
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
       const uint4 v = *reinterpret_cast<const uint4*>(blk + lay.v_word(4 * j + (r & 3), 4 * q));
@@ -435,7 +438,9 @@ struct AqWarp {
         b1 = h2_bits(__hmul2(bits_h2(h23), bits_h2(vd[j].y)));
       } else {
         const float2 e0 = __half22float2(bits_h2(vd[j].x)), e1 = __half22float2(bits_h2(vd[j].y));
-        const float y0 = r0 * e0.x, y1 = r1 * e0.y, y2 = r2 * e1.x, y3 = r3 * e1.y;
+        float y0, y1, y2, y3;
+        f32x2_split(f32x2_mul(r01, f32x2_two(e0.x, e0.y)), y0, y1);
+        f32x2_split(f32x2_mul(r23, f32x2_two(e1.x, e1.y)), y2, y3);
         b0 = pack_half2(y0, y1);
         b1 = pack_half2(y2, y3);
         if constexpr (SPLIT) {
@@ -598,8 +603,8 @@ __global__ void __launch_bounds__(kAqThreads, 2) attn_q4_kernel(const AttnQ4Para
                  : p.first + (static_cast<int64_t>(blockIdx.x) * kAqWarps + (k >> 1)) * kAqHeads * SM::kRow;
   };
   // ---- this warp's range [w0, w1) of it ------------------------------------------------
-  const int share = (count + kAqWarps - 1) / kAqWarps;
-  const int w0 = min(warp * share, count), w1 = min(w0 + share, count);
+  const int w0 = static_cast<int>(static_cast<int64_t>(count) * warp / kAqWarps);
+  const int w1 = static_cast<int>(static_cast<int64_t>(count) * (warp + 1) / kAqWarps);
   if (w0 < w1) {
     AqWalk walk;
     {

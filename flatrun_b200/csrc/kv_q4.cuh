@@ -66,6 +66,32 @@ FRC_DEVICE_INLINE void from_f32(float v, float& o) { o = v; }
 FRC_DEVICE_INLINE void from_f32(float v, __half& o) { o = __float2half_rn(v); }
 FRC_DEVICE_INLINE void from_f32(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
 
+// Pairs of fp32 values: two operations in one instruction.
+FRC_DEVICE_INLINE uint64_t f32x2_two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+FRC_DEVICE_INLINE void f32x2_split(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+FRC_DEVICE_INLINE uint64_t f32x2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+FRC_DEVICE_INLINE uint64_t f32x2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+FRC_DEVICE_INLINE uint64_t f32x2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // N consecutive elements at p as fp32, and back.  VEC: p is aligned to the
 // run (at most 16 bytes); otherwise one element at a time.
 template <int N, bool VEC, typename T>
