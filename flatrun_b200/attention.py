@@ -300,16 +300,15 @@ def kv_read_q4(cache, slots, *, dtype=None, out=None):
 
 
 # ---- attention ----------------------------------------------------------------------------
-_workspace_bytes: dict = {}
+_workspace_bytes: dict = {}  # by head_dim
 
 
 def _decode_q4_workspace(batch: int, nh: int, nkv: int, hd: int) -> int:
-    key = (batch, nh, nkv, hd)
-    if key not in _workspace_bytes:
+    if hd not in _workspace_bytes:
         ws = ctypes.c_size_t()
         _lib.check(_lib.load().frc_attention_decode_q4_workspace(batch, nh, nkv, hd, ctypes.byref(ws)))
-        _workspace_bytes[key] = int(ws.value)
-    return _workspace_bytes[key]
+        _workspace_bytes[hd] = int(ws.value)
+    return _workspace_bytes[hd]
 
 
 def attention_decode_q4(q, cache, block_table, lengths, *, scale: float | None = None, out=None):

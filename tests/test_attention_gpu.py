@@ -247,6 +247,8 @@ def _decode_ref(cache, table, lens, qx, scale, dtype, page):
     ([40, 300], 32, 2, 128, 16),   # 16 query heads a KV head
     ([90], 11, 1, 64, 16),          # 11: two parts of unequal heads
     ([3000, 1, 1, 900], 6, 2, 64, 16),
+    ([20000], 2, 1, 64, 64),                       # cut into more than 32 pieces
+    ([5, 0, 40] * 100 + [700], 3, 1, 64, 16),     # more sequences than threads of a CTA
 ])
 def test_decode_q4(dtype, lens, nh, nkv, hd, page):
     cache, table, n, q, qx = _decode_case(len(lens) + nh, lens, nh, nkv, hd, page, dtype)
@@ -284,6 +286,12 @@ def test_decode_q4_bad_tables_lengths_and_strides():
     _close(out, ref, bound)
     assert not out[2].any()
     assert bool((wide[:, 8] == 5).all() and (wide[:, :, :8] == 5).all() and (wide[:, :, 72:] == 5).all())
+    # queries and outputs that allow no vector access
+    odd = torch.full((4, 8 * 65 + 1), 3.0, device="cuda")
+    q_odd, o_odd = (t[:, 1:].view(4, 8, 65)[..., :64] for t in (odd.clone(), odd))
+    q_odd.copy_(q)
+    A.attention_decode_q4(q_odd, cache, table, n, out=o_odd)
+    assert torch.equal(o_odd, out) and bool((odd[:, 0] == 3).all())
     n.fill_(-3)
     assert not A.attention_decode_q4(q, cache, table, n).any()
     assert A.attention_decode_q4(q, cache, table[:, :0], n.fill_(9)).abs().sum() == 0
@@ -351,6 +359,9 @@ def _prefill_case(seed, qs, ks, nh, nkv, hd, dtype, pad=0, std=1.0):
     ([200, 30], [60, 0], 2, 2, 64),                       # more queries than keys: rows that see nothing
     ([700], [900], 6, 1, 128),
     ([1, 1, 1, 2, 1, 3] * 9, [4, 1, 9, 2, 130, 3] * 9, 2, 1, 64),
+    ([100, 37], [100, 50], 14, 2, 64),                     # seven heads a tile, 126 rows of it
+    ([40], [40], 11, 1, 128),                              # eleven: one a tile
+    ([9, 3], [9, 300], 96, 1, 64),                         # 96 = 32 * 3: 32 heads a tile
 ])
 def test_prefill(dtype, causal, qs, ks, nh, nkv, hd):
     q, k, v, cu_q, cu_k, x = _prefill_case(len(qs) + hd + nh, qs, ks, nh, nkv, hd, dtype, pad=3)
@@ -398,6 +409,66 @@ def test_prefill_hidden_values_have_no_part(dtype):
     _close(got[seen], ref[seen], bound[seen])
     assert bool(torch.isnan(got[100:150]).all()) and bool(torch.isnan(got[219]).all())
     assert not got[220:].any()
+
+
+def test_no_tokens():
+    """Calls without a token launch nothing and return what has the right shape."""
+    z = lambda *s, d=torch.float32: torch.zeros(*s, dtype=d, device="cuda")  # noqa: E731
+    q, k, v = A.qk_norm_rope(z(0, 8 * 64), 4, 2, z(5, 32), z(5, 32), z(0, d=torch.int32))
+    assert q.shape == (0, 4, 64) and k.shape == v.shape == (0, 2, 64)
+    cache, slots = A.kv_cache_q4(1, 16, 2, 64), z(0, d=torch.int64)
+    A.kv_append_q4(cache, k, v, slots)
+    assert not cache.any() and A.kv_read_q4(cache, slots)[0].shape == (0, 2, 64)
+    h = torch.float16
+    out = A.attention_prefill(z(0, 4, 64, d=h), z(3, 2, 64, d=h), z(3, 2, 64, d=h), z(2, d=torch.int32))
+    assert out.shape == (0, 4, 64)
+    cu = torch.tensor([0, 2], dtype=torch.int32, device="cuda")
+    out = A.attention_prefill(z(2, 4, 64, d=h) + 1, z(0, 2, 64, d=h), z(0, 2, 64, d=h), cu, z(2, d=torch.int32))
+    assert not out.any()
+
+
+def test_bad_ends_stay_inside():
+    """Ends that fall, or lie outside the rows, are held to them: nothing outside is touched."""
+    q, k, v, _, _, _ = _prefill_case(4, [64], [64], 2, 1, 64, "bf16")
+    for ends in ([5, 3, 70], [-9, 1 << 30, 2], [64, 0, 0]):
+        cu = torch.tensor(ends, dtype=torch.int32, device="cuda")
+        guard = torch.full((68, 2, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+        A.attention_prefill(q, k, v, cu, out=guard[2:66])
+        torch.cuda.synchronize()
+        assert bool((guard[:2] == 7).all() and (guard[66:] == 7).all())
+
+
+def test_first_calls_inside_a_capture():
+    """In a fresh process: every operator's first call is captured, and the replay gives what an eager call gives."""
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from flatrun_b200 import attention as A
+z = lambda *s, d=torch.float32: torch.randn(*s, device="cuda").to(d)
+qkv, pos = z(3, 8 * 64), torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+cos, sin = (torch.from_numpy(t).cuda() for t in A.rope_tables_scaled(64, 1e4, 9))
+cache, slots = A.kv_cache_q4(1, 16, 2, 64), torch.arange(3, device="cuda")
+table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+n, cu = torch.tensor([3], dtype=torch.int32, device="cuda"), torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+def step():
+    q, k, v = A.qk_norm_rope(qkv, 4, 2, cos, sin, pos, out_dtype=torch.float16)
+    A.kv_append_q4(cache, k, v, slots)
+    return A.attention_prefill(q, k, v, cu), A.attention_decode_q4(q[2:], cache, table, n), A.kv_read_q4(cache, slots)[0]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = step()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, step())) and all(bool(t.any()) for t in got)
+print("captured")
+"""
+    import os
+    repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=repo, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
 
 
 # ---- as they are used together ---------------------------------------------------------------
@@ -570,3 +641,14 @@ def test_engine_options_and_refusals():
     plain.step(5)
     eng.logits_host(), plain.logits_host()  # (waits for the engines' streams)
     assert torch.equal(eng.k_cache[0][0], plain.k_cache[0][0]) and not torch.equal(eng.k_cache[0][1], plain.k_cache[0][1])
+
+
+def test_no_wait_ran_out():
+    """The status word that bounded waits report to is clear after the calls above."""
+    import ctypes
+
+    from flatrun_b200 import _lib
+
+    flags = ctypes.c_uint32(1)
+    _lib.check(_lib.load().frc_device_status(0, ctypes.byref(flags)))
+    assert flags.value == 0
