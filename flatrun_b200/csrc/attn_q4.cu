@@ -418,11 +418,16 @@ struct AqWarp {
     const float p0 = ex2(s[0] - base), p1 = ex2(s[1] - base), p2 = ex2(s[2] - base), p3 = ex2(s[3] - base);
     l_run += (p0 + p1) + (p2 + p3);
     const uint32_t h01 = pack_half2(p0, p1), h23 = pack_half2(p2, p3);
-    mma16816(om, vm.x, 0u, vm.y, 0u, h01, h23);
     if constexpr (SPLIT) {
       const float2 g01 = __half22float2(bits_h2(h01)), g23 = __half22float2(bits_h2(h23));
-      mma16816(om, vm.x, 0u, vm.y, 0u, pack_half2(p0 - g01.x, p1 - g01.y), pack_half2(p2 - g23.x, p3 - g23.y));
-      mma16816(om, vml.x, 0u, vml.y, 0u, h01, h23);
+      float c[4];
+      mma16816_new(c, vm.x, 0u, vm.y, 0u, pack_half2(p0 - g01.x, p1 - g01.y), pack_half2(p2 - g23.x, p3 - g23.y));
+      mma16816(c, vml.x, 0u, vml.y, 0u, h01, h23);
+      mma16816(c, vm.x, 0u, vm.y, 0u, h01, h23);
+      om[0] += c[0];
+      om[1] += c[1];
+    } else {
+      mma16816(om, vm.x, 0u, vm.y, 0u, h01, h23);
     }
     // rows of a tile: 16 channels of group j: word 4 j + r % 4, of it the nibbles
     // of its low half (r < 4) or high half: 2 t in row r, 2 t + 1 in row r + 8
@@ -454,8 +459,17 @@ struct AqWarp {
         const uint32_t u0 = t ? w0 >> 8 : w0, u1 = t ? w1 >> 8 : w1;
         const uint32_t n0 = nibbles<true, 8>(u0, bias), n1 = nibbles<false, 8>(u0, bias);
         const uint32_t n2 = nibbles<true, 8>(u1, bias), n3 = nibbles<false, 8>(u1, bias);
-        mma16816(o[j][t], n0, n1, n2, n3, b0, b1);
-        if constexpr (SPLIT) mma16816(o[j][t], n0, n1, n2, n3, c0, c1);
+        if constexpr (SPLIT) {
+          // into a fresh accumulator: the tensor cores cut their sums (towards zero),
+          // which over thousands of tokens takes 2e-6 off a running one
+          float c[4];
+          mma16816_new(c, n0, n1, n2, n3, c0, c1);
+          mma16816(c, n0, n1, n2, n3, b0, b1);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[j][t][i] += c[i];
+        } else {
+          mma16816(o[j][t], n0, n1, n2, n3, b0, b1);
+        }
       }
     }
   }

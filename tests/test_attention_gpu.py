@@ -268,6 +268,16 @@ def test_decode_q4_sizes_of_values(dtype):
         _close(got, ref, bound + 1e-30)
 
 
+def test_decode_q4_long_sums_keep_fp32():
+    """Over tens of thousands of tokens fp32 results stay fp32: what roundings of either sign leave of 16 a term, 16 * E32
+    of the result's norm.  (Sums that are cut towards zero, as the tensor cores' are, lose half a step each time: 1e-5
+    over 60000 tokens if they ran through.)"""
+    cache, table, n, q, qx = _decode_case(6, [60000], 4, 1, 64, 128, "fp32")
+    got = _np(A.attention_decode_q4(q, cache, table, n))
+    ref, _ = _decode_ref(cache, table, n, qx, 0.125, "fp32", 128)
+    assert np.linalg.norm(got - ref) <= 16 * E32 * np.linalg.norm(ref)
+
+
 def test_decode_q4_bad_tables_lengths_and_strides():
     """Page numbers outside the cache hide their tokens, lengths are held to the table, strided queries and outputs,
     and what lies beside the output stays."""
