@@ -74,18 +74,21 @@ def _launch(device: int, op, *args) -> None:
         _lib.check(rc)
 
 
-def _same_cuda_device(*tensors) -> int:
-    grad = torch.is_grad_enabled()
-    first = tensors[0]
+def _device(first, *others) -> int:
+    """The CUDA device that all tensors are on."""
     i = first.get_device()
-    for t in tensors:
-        if grad and t.requires_grad:
-            raise ValueError("the operator has no backward pass: call it under torch.no_grad()")
+    for t in others:
         if t.get_device() != i:
             raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
-    if not first.is_cuda:
+    if i < 0 or not first.is_cuda:
         raise ValueError(f"tensors must be on a CUDA device, not {first.device}")
     return i
+
+
+def _no_grad(*tensors) -> None:
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("the operator has no backward pass: call it under torch.no_grad()")
 
 
 def _index(t: torch.Tensor, name: str, dtype: torch.dtype, shape) -> None:
@@ -195,41 +198,57 @@ def qk_norm_rope(qkv, heads: int, kv_heads: int, cos, sin, positions, *, bias=No
     if 2 * pairs > hd:
         raise ValueError(f"the tables rotate {2 * pairs} of {hd} channels")
     _index(positions, "positions", torch.int32, (tokens,))
-    used = [qkv, cos, sin, positions]
-    weights = []
-    for t, name, size in ((bias, "bias", n), (q_norm, "q_norm", hd), (k_norm, "k_norm", hd)):
-        if t is None:
-            weights.append(0)
-        else:
-            _index(t, name, torch.float32, (size,))
-            used.append(t)
-            weights.append(t.data_ptr())
+    _no_grad(qkv, cos, sin)
+    p_bias = p_q = p_k = 0
+    if bias is not None:
+        p_bias = _weight(bias, "bias", n, qkv)
+    if q_norm is not None:
+        p_q = _weight(q_norm, "q_norm", hd, qkv)
+    if k_norm is not None:
+        p_k = _weight(k_norm, "k_norm", hd, qkv)
     if out is None:
         dtype = out_dtype or qkv.dtype
         if dtype not in _TYPE:
             raise ValueError(f"out_dtype must be fp32, fp16 or bf16, not {dtype}")
         out = tuple(torch.zeros((tokens, h, hd), dtype=dtype, device=qkv.device) for h in (heads, kv_heads, kv_heads))
-    else:
-        if len(out) != 3:
-            raise ValueError("out must be (q, k, v)")
-        dtype = out[0].dtype
-        if dtype not in _TYPE or out_dtype not in (None, dtype):
-            raise ValueError("out has another type than out_dtype, or not fp32, fp16 or bf16")
-    strides = []
-    for t, name, h in zip(out, ("out q", "out k", "out v"), (heads, kv_heads, kv_heads)):
-        r, s = _rows(t, name, (tokens, h, hd), dtype)
-        if s != hd and h > 1 and tokens:
-            raise ValueError(f"the heads of {name} must be contiguous")
-        if r < h * hd and tokens > 1:
-            raise ValueError(f"the rows of {name} overlap")
-        strides.append(r if tokens > 1 else h * hd)
+    elif len(out) != 3:
+        raise ValueError("out must be (q, k, v)")
     q, k, v = out
-    device = _same_cuda_device(*used, q, k, v)
-    _launch(device, _ROPE, in_type, _TYPE[dtype], qkv.data_ptr(), row if tokens > 1 else n, tokens,
-            heads, kv_heads, hd, weights[0], weights[1], weights[2], eps, cos.data_ptr(), sin.data_ptr(), max_pos,
-            2 * pairs, 1 if interleaved else 0, positions.data_ptr(), q.data_ptr(), strides[0], k.data_ptr(), strides[1],
-            v.data_ptr(), strides[2])
+    dtype = q.dtype
+    if dtype not in _TYPE or (out_dtype is not None and out_dtype != dtype):
+        raise ValueError("out has another type than out_dtype, or not fp32, fp16 or bf16")
+    shape = (tokens, kv_heads, hd)
+    q_row = _packed(q, "out q", (tokens, heads, hd), dtype)
+    k_row = _packed(k, "out k", shape, dtype)
+    v_row = _packed(v, "out v", shape, dtype)
+    _launch(_device(qkv, cos, sin, positions, q, k, v), _ROPE, in_type, _TYPE[dtype], qkv.data_ptr(),
+            row if tokens > 1 else n, tokens, heads, kv_heads, hd, p_bias, p_q, p_k, eps, cos.data_ptr(), sin.data_ptr(),
+            max_pos, 2 * pairs, 1 if interleaved else 0, positions.data_ptr(), q.data_ptr(), q_row, k.data_ptr(), k_row,
+            v.data_ptr(), v_row)
     return out
+
+
+def _weight(t, name: str, size: int, beside) -> int:
+    _index(t, name, torch.float32, (size,))
+    _no_grad(t)
+    if t.get_device() != beside.get_device():
+        raise ValueError(f"tensors on different devices: {beside.device} and {t.device}")
+    return t.data_ptr()
+
+
+def _packed(t, name: str, shape, dtype) -> int:
+    """Row stride of a (rows, heads, head_dim) output with contiguous heads."""
+    row, head = _rows(t, name, shape, dtype)
+    rows, heads, hd = shape
+    if rows == 0:
+        return heads * hd
+    if head != hd and heads > 1:
+        raise ValueError(f"the heads of {name} must be contiguous")
+    if rows == 1:
+        return heads * hd
+    if row < heads * hd:
+        raise ValueError(f"the rows of {name} overlap")
+    return row
 
 
 # ---- the cache ------------------------------------------------------------------------
@@ -244,12 +263,13 @@ def kv_cache_q4(pages: int, page_size: int, kv_heads: int, head_dim: int, device
 
 
 def _cache(cache) -> tuple[int, int, int, int]:
-    if cache.dim() != 4 or cache.dtype != torch.uint8 or not cache.is_contiguous() or cache.numel() == 0 or \
-            cache.shape[3] not in (20 * 64, 20 * 128):
-        raise ValueError("the cache must be a contiguous uint8 tensor (pages, kv_heads, page_size / 16, 20 * head_dim), "
-                         "head_dim 64 or 128")
-    pages, kv_heads, blocks, nbytes = cache.shape
-    return pages, kv_heads, blocks * _BLOCK, nbytes // 20
+    shape = cache.shape
+    if len(shape) == 4 and cache.dtype == torch.uint8 and cache.is_contiguous():
+        pages, kv_heads, blocks, nbytes = shape
+        if pages and kv_heads and blocks and (nbytes == 20 * 128 or nbytes == 20 * 64):
+            return pages, kv_heads, blocks * _BLOCK, nbytes // 20
+    raise ValueError("the cache must be a contiguous uint8 tensor (pages, kv_heads, page_size / 16, 20 * head_dim), "
+                     "head_dim 64 or 128")
 
 
 def kv_append_q4(cache, k, v, slots) -> None:
@@ -265,8 +285,8 @@ def kv_append_q4(cache, k, v, slots) -> None:
     k_row, k_head = _rows(k, "k", shape, k.dtype)
     v_row, v_head = _rows(v, "v", shape, k.dtype)
     _index(slots, "slots", torch.int64, (tokens,))
-    device = _same_cuda_device(cache, k, v, slots)
-    _launch(device, _APPEND, dtype, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
+    _no_grad(k, v)
+    _launch(_device(cache, k, v, slots), _APPEND, dtype, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
             tokens, slots.data_ptr(), nkv, hd, pages, page, cache.data_ptr())
 
 
@@ -293,8 +313,7 @@ def kv_read_q4(cache, slots, *, dtype=None, out=None):
     v_row, v_head = _rows(v, "out v", shape, k.dtype)
     if tokens and (min(k_row, v_row) <= 0 < tokens - 1 or min(k_head, v_head) <= 0 < nkv - 1):
         raise ValueError("the rows or heads of out overlap")
-    device = _same_cuda_device(cache, slots, k, v)
-    _launch(device, _READ, _TYPE[k.dtype], cache.data_ptr(), slots.data_ptr(), tokens, nkv, hd,
+    _launch(_device(cache, slots, k, v), _READ, _TYPE[k.dtype], cache.data_ptr(), slots.data_ptr(), tokens, nkv, hd,
             pages, page, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head)
     return out
 
@@ -341,7 +360,8 @@ def attention_decode_q4(q, cache, block_table, lengths, *, scale: float | None =
     o_seq, o_head = _rows(out, "out", shape, q.dtype)
     if batch and (o_seq <= 0 < batch - 1 or o_head <= 0 < nh - 1):
         raise ValueError("the rows or heads of out overlap")
-    device = _same_cuda_device(q, cache, block_table, lengths, out)
+    _no_grad(q)
+    device = _device(q, cache, block_table, lengths, out)
     nbytes = _decode_q4_workspace(batch, nh, nkv, hd)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     _launch(device, _DECODE, dtype, q.data_ptr(), q_seq, q_head, cache.data_ptr(), pages,
@@ -384,15 +404,17 @@ def attention_prefill(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: f
         out = torch.zeros(shape, dtype=dtype, device=q.device)
     strides.append(_rows(out, "out", shape, dtype))
     at = [q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()]
-    for t, (row, head), p, name in zip((q, k, v, out), strides, at, ("q", "k", "v", "out")):
-        if (p % 16 or row % 8 or head % 8) and t.numel():
-            raise ValueError(f"{name} must be 16-byte aligned, with row and head strides that are multiples of 8")
-    if tokens and (strides[3][0] <= 0 < tokens - 1 or strides[3][1] <= 0 < nh - 1):
+    (q_row, q_head), (k_row, k_head), (v_row, v_head), (o_row, o_head) = strides
+    if (at[0] | at[1] | at[2] | at[3]) & 15 or (q_row | q_head | k_row | k_head | v_row | v_head | o_row | o_head) & 7:
+        for t, (row, head), p, name in zip((q, k, v, out), strides, at, ("q", "k", "v", "out")):
+            if (p % 16 or row % 8 or head % 8) and t.numel():
+                raise ValueError(f"{name} must be 16-byte aligned, with row and head strides that are multiples of 8")
+    if tokens and (o_row <= 0 < tokens - 1 or o_head <= 0 < nh - 1):
         raise ValueError("the rows or heads of out overlap")
-    device = _same_cuda_device(q, k, v, cu_q, cu_k, out)
-    _launch(device, _PREFILL, _TYPE[dtype], at[0], *strides[0], at[1], *strides[1], at[2],
-            *strides[2], cu_q.data_ptr(), cu_k.data_ptr(), cu_q.shape[0] - 1, tokens, tokens_k, nh, nkv, hd,
-            hd ** -0.5 if scale is None else scale, 1 if causal else 0, at[3], *strides[3])
+    _no_grad(q, k, v)
+    _launch(_device(q, k, v, cu_q, cu_k, out), _PREFILL, _TYPE[dtype], at[0], q_row, q_head, at[1], k_row, k_head,
+            at[2], v_row, v_head, cu_q.data_ptr(), cu_k.data_ptr(), cu_q.shape[0] - 1, tokens, tokens_k, nh, nkv, hd,
+            hd ** -0.5 if scale is None else scale, 1 if causal else 0, at[3], o_row, o_head)
     return out
 
 
