@@ -143,6 +143,7 @@ def rope_tables_scaled(rot: int, theta: float, max_pos: int, scaling: dict | Non
             if kind == "yarn":
                 fast, slow = float(scaling.get("beta_fast", 32)), float(scaling.get("beta_slow", 1))
                 _need(fast > slow > 0, "yarn scaling needs beta_fast > beta_slow > 0")
+                _need(theta > 1, "yarn scaling needs theta above 1")
 
                 def pair(r):  # the (fractional) pair that turns r times in n positions
                     return rot * math.log(n / (r * 2 * math.pi)) / (2 * math.log(theta))
@@ -380,7 +381,8 @@ def attention_prefill(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: f
     Causal: the last query of a sequence sees all its keys, each earlier one a
     key less, so a prompt may go on behind tokens that came before.  A query that
     sees no key gives zeros; rows of no sequence are left as they are (zeros
-    where this call makes the output).  `scale` defaults to head_dim^-1/2.
+    where this call makes the output).  `scale` defaults to head_dim^-1/2.  `out`
+    shares no memory with q, k and v.
     """
     if q.dim() != 3 or q.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError("q must be (tokens, heads, head_dim), fp16 or bf16")
@@ -411,6 +413,8 @@ def attention_prefill(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: f
                 raise ValueError(f"{name} must be 16-byte aligned, with row and head strides that are multiples of 8")
     if tokens and (o_row <= 0 < tokens - 1 or o_head <= 0 < nh - 1):
         raise ValueError("the rows or heads of out overlap")
+    if at[3] in at[:3] and tokens:
+        raise ValueError("out must not be q, k or v: their rows are read again where a result is not finite")
     _no_grad(q, k, v)
     _launch(_device(q, k, v, cu_q, cu_k, out), _PREFILL, _TYPE[dtype], at[0], q_row, q_head, at[1], k_row, k_head,
             at[2], v_row, v_head, cu_q.data_ptr(), cu_k.data_ptr(), cu_q.shape[0] - 1, tokens, tokens_k, nh, nkv, hd,

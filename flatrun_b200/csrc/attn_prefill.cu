@@ -692,7 +692,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       pf_fence_after();
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       T* op = static_cast<T*>(p.out) + static_cast<int64_t>(w.q_start + row) * p.o_tok + (w.head + my_head) * p.o_head;
-      bool finite = true;
+      bool finite = sum != 0.f || seen == 0;  // all scores -inf: 0 / 0
 #pragma unroll
       for (int c = 0; c < HD; c += 32) {
         float v[32];

@@ -41,8 +41,9 @@
 //    parts for fp32, rounded to fp16 for 16-bit types as the stored m is.
 //
 // The softmax's reference is not the largest s but the largest s + log2 d (d
-// the token's largest V step, at least 2^-10): so p d stays within one power of
-// two of 1 whatever the size of the values, and p below 2^10.
+// the token's largest V step, at least 2^-7): so p d stays below 2^8 whatever the
+// size of the values, p below 2^15, and both well above fp16's least for
+// steps from 2^-24 to 65504.
 //
 // Split: all sequences' tokens, 32 (two blocks) a place, for each KV head (and
 // part of eight query heads: a unit), form one line, with one empty place before
@@ -208,9 +209,10 @@ struct AqWarp {
   static constexpr int NG = HD / kQ4Group;
   static constexpr bool SPLIT = sizeof(T) == 4;  // operands in two parts
   static constexpr bool TWICE = std::is_same<T, __nv_bfloat16>::value;  // p rounded to 11 bits before p d is
-  // p at the reference is 2^kLift, and may be 2^(kLift + kSlack), times d up to
-  // kUp times that: p (at most 2^10 / d more) and p d stay below fp16's 65504
-  static constexpr float kLift = 1.f, kSlack = 4.f, kUp = TWICE ? 1.f : 512.f;
+  // p d at the reference is 2^kLift (p where d is below 2^-7 2^7 times that), and may
+  // be 2^kSlack times that: p and kUp p d stay below fp16's 65504
+  static constexpr float kLift = 4.f, kSlack = 4.f, kUp = TWICE ? 1.f : 64.f;
+  static constexpr float kLow = 2048.f;  // of the low parts of fp32 weights and offsets
   uint32_t a[NG][2][4];  // query fragments: (group, k step): rows 0-7 of both k halves, rows 8-15 (low parts) of both
   uint32_t am;                       // groups' query sums
   float f_n, f_m;                    // scale of the two score products, with log2 e
@@ -232,6 +234,7 @@ struct AqWarp {
     const float down = __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
     f_n = scale * 1.44269504088896341f * down;
     f_m = scale * 1.44269504088896341f * down * 64.f;
+    if (mx == INFINITY) f_n = f_m = NAN;  // every score is infinite or NaN: so is the softmax
     float sum[NG];
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
@@ -425,14 +428,44 @@ struct AqWarp {
     const float p0 = ex2(s[0] - base), p1 = ex2(s[1] - base), p2 = ex2(s[2] - base), p3 = ex2(s[3] - base);
     l_run += (p0 + p1) + (p2 + p3);
     const uint32_t h01 = pack_half2(p0, p1), h23 = pack_half2(p2, p3);
+    uint32_t l01 = 0u, l23 = 0u;  // fp32: 2^11 times the rest of p, so that it stays above fp16's subnormals
     if constexpr (SPLIT) {
       const float2 g01 = __half22float2(bits_h2(h01)), g23 = __half22float2(bits_h2(h23));
+      l01 = pack_half2((p0 - g01.x) * kLow, (p1 - g01.y) * kLow);
+      l23 = pack_half2((p2 - g23.x) * kLow, (p3 - g23.y) * kLow);
+    }
+    const __half2 most = __hmax2(__habs2(bits_h2(vm.x)), __habs2(bits_h2(vm.y)));
+    if (__any_sync(0xffffffffu, !__hblt2(most, bits_h2(0x7c007c00u)))) {
+      // a sum m + 8 d beyond fp16 (values above 65504): m and d as rows of their own
+      uint2 m = make_uint2(0u, 0u), d = m;
+      if (r < NG) {
+        m = *reinterpret_cast<const uint2*>(blk + lay.v_offset(r, 4 * q));
+        d = *reinterpret_cast<const uint2*>(blk + lay.v_step(r, 4 * q));
+      }
+      if constexpr (TAIL) {
+        uint32_t k0, k1;
+        own_tokens(left - 4 * q, k0, k1);
+        m.x &= k0;
+        m.y &= k1;
+        d.x &= k0;
+        d.y &= k1;
+      }
       float c[4];
-      mma16816_new(c, vm.x, 0u, vm.y, 0u, pack_half2(p0 - g01.x, p1 - g01.y), pack_half2(p2 - g23.x, p3 - g23.y));
-      mma16816(c, vml.x, 0u, vml.y, 0u, h01, h23);
-      mma16816(c, vm.x, 0u, vm.y, 0u, h01, h23);
-      om[0] += c[0];
-      om[1] += c[1];
+      if constexpr (SPLIT) {
+        mma16816_new(c, m.x, d.x, m.y, d.y, l01, l23);
+        om[0] += fmaf(c[2], 8.f, c[0]) * (1.f / kLow);
+        om[1] += fmaf(c[3], 8.f, c[1]) * (1.f / kLow);
+      }
+      mma16816_new(c, m.x, d.x, m.y, d.y, h01, h23);
+      om[0] += fmaf(c[2], 8.f, c[0]);
+      om[1] += fmaf(c[3], 8.f, c[1]);
+    } else if constexpr (SPLIT) {
+      float c[4], low[4];
+      mma16816_new(low, vm.x, 0u, vm.y, 0u, l01, l23);
+      mma16816(low, vml.x, 0u, vml.y, 0u, h01, h23);
+      mma16816_new(c, vm.x, 0u, vm.y, 0u, h01, h23);
+      om[0] += fmaf(low[0], 1.f / kLow, c[0]);
+      om[1] += fmaf(low[1], 1.f / kLow, c[1]);
     } else {
       mma16816(om, vm.x, 0u, vm.y, 0u, h01, h23);
     }
@@ -492,7 +525,7 @@ struct AqWarp {
   // The blocks of a place (bit e of `seen`: block e is there), of which `left`
   // tokens belong to the sequence.
   FRC_DEVICE_INLINE void place(const uint8_t (*blk)[20 * HD], uint32_t seen, int left, int lane, uint32_t bias) {
-    const __half2 least = __float2half2_rn(1.f / 1024.f);
+    const __half2 least = __float2half2_rn(1.f / 128.f);
     if (left >= 2 * kQ4Tokens && seen == 3u) {
       float s0[4], s1[4];
       __half2 dx = least;
@@ -514,13 +547,14 @@ struct AqWarp {
     }
   }
 
-  // Two tokens' m + 8 d as the sum of two halves each: m becomes the high part.
+  // Two tokens' m + 8 d as the sum of two halves each, the second times kLow: m
+  // becomes the high part.
   static FRC_DEVICE_INLINE void offset_parts(uint32_t d, uint32_t& m, uint32_t& low) {
     const float2 df = __half22float2(bits_h2(d)), mf = __half22float2(bits_h2(m));
     const float x = fmaf(df.x, 8.f, mf.x), y = fmaf(df.y, 8.f, mf.y);
     m = pack_half2(x, y);
     const float2 h = __half22float2(bits_h2(m));
-    low = pack_half2(x - h.x, y - h.y);
+    low = pack_half2((x - h.x) * kLow, (y - h.y) * kLow);
   }
 
   // The warp's sums: f(head, channel, o[4]) for this lane's channels of its two
@@ -924,6 +958,7 @@ int frc_attention_decode_q4(int type, const void* q, int64_t q_seq_stride, int64
               "frc_attention_decode_q4: bad batch or block table");
   FRC_REQUIRE(q_seq_stride >= 0 && q_head_stride >= 0 && out_seq_stride >= 0 && out_head_stride >= 0,
               "frc_attention_decode_q4: negative stride");
+  FRC_REQUIRE(scale - scale == 0.f, "frc_attention_decode_q4: scale must be finite");
   if (batch == 0) return FRC_OK;
   FRC_REQUIRE(q && cache && (block_table || max_pages == 0) && lengths && out && workspace,
               "frc_attention_decode_q4: null pointer");

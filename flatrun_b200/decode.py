@@ -322,6 +322,8 @@ class DecodeEngine:
         kvd = c.kv_heads * hd
         if n == 0:
             raise ValueError("an empty prompt")
+        if ids.min() < 0 or ids.max() >= c.vocab:
+            raise ValueError(f"token ids must lie in 0 .. {c.vocab - 1}")
         with torch.cuda.stream(self.stream):
             start = int(self.pos.item())
             if start + n > c.max_pos:

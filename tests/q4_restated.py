@@ -66,6 +66,18 @@ def unpack(cache):
     return out[0], out[2], out[1], out[3]
 
 
+def middle_sizes(cache):
+    """|d (n - 8)| + |m + 8 d| of V (pages, heads, page_size, hd): the terms of a value taken from its group's middle."""
+    pages, heads, blocks, nbytes = cache.shape
+    hd = nbytes // 20
+    _, at, odd, scales = _places(hd)
+    flat = cache.reshape(-1, nbytes)
+    d, m = ((flat[:, s].astype(np.uint16) | (flat[:, s + 1].astype(np.uint16) << 8)).view(np.float16)
+            .astype(np.float64).repeat(32, axis=-1) for s in scales[2:])
+    n = ((flat[:, at] >> (4 * odd)) & 15).astype(np.float64)
+    return (np.abs(d * (n - 8)) + np.abs(m + 8 * d)).reshape(pages, heads, blocks * 16, hd)
+
+
 def write(cache, k, v, slots):
     """Quantise rows into a cache (uint8, changed in place); slots outside it are skipped."""
     pages, heads, blocks, nbytes = cache.shape

@@ -216,9 +216,11 @@ def _decode_case(seed, lens, nh, nkv, hd, page, dtype, extra_pages=2, std=1.0, q
     return cache, torch.from_numpy(table).cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), q, qx
 
 
-def _decode_ref(cache, table, lens, qx, scale, dtype, page):
+def _decode_ref(cache, table, lens, qx, scale, dtype, page, skewed=False):
     with np.errstate(all="ignore"):
         kk, vv, ks, vs = R.unpack(cache.cpu().numpy())
+        if skewed:
+            vs = np.maximum(vs, R.middle_sizes(cache.cpu().numpy()))
     table, lens = table.cpu().numpy(), lens.cpu().numpy()
     out, bound = np.zeros_like(qx), np.zeros_like(qx)
     group = qx.shape[1] // kk.shape[1]
@@ -324,6 +326,58 @@ def test_decode_q4_not_finite():
     _close(got, ref, bound)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+def test_decode_q4_values_beyond_fp16(dtype):
+    """Groups whose middle m + 8 d lies above 65504, in whole blocks and in a sequence's last one (in fp16 few and with
+    small weights, so that the results stay inside the type).  Weights are applied to n - 8 and m + 8 d, so in a
+    group that lies to one side of its offset their roundings count by |d (n - 8)| + |m + 8 d|, which at n = 0 is more
+    than |m| = |d n| + |m|."""
+    cache, table, n, q, qx = _decode_case(9, [100, 37, 64], 8, 2, 128, 16, dtype)
+    rng = np.random.default_rng(10)
+    at = [(0, 20), (0, 99), (1, 5), (1, 36), (2, 63)]
+    slots = torch.tensor([int(table[b, t // 16]) * 16 + t % 16 for b, t in at]).cuda()
+    k, v = (np.asarray(rng.standard_normal((5, 2, 128)) * s, np.float32) for s in (1.0, 2e5))
+    if dtype == "fp16":
+        v *= 1e-2
+        v[:, 0, 40:72] = 6e4
+        v[:, 0, 50] = 4e5
+    A.kv_append_q4(cache, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), slots)
+    got = A.attention_decode_q4(q, cache, table, n, scale=0.01)
+    ref, bound = _decode_ref(cache, table, n, qx, float(np.float32(0.01)), dtype, 16, skewed=True)
+    assert np.abs(ref).max() < 65000
+    _close(got, ref, bound)
+
+
+@pytest.mark.parametrize("std", [1e-5, 1e-3, 1e-2, 1.0, 1e3, 1e4, 1e5])
+def test_decode_q4_fp32_at_any_size_of_values(std):
+    """Equal weights (queries of zero), so that only the values' way counts.  Weights times steps and offsets m + 8 d are
+    in two halves each: 2^-22, 4 * E32; the rest of an offset's weight another 4 * E32; four sums of 16 terms that may
+    cut, 8 * E32; sums over blocks and warps and the division, 8 * E32: 24 * E32 of the terms' sizes."""
+    cache, table, n, q, qx = _decode_case(12, [90, 17], 4, 2, 128, 16, "fp32", std=std, q_std=0.0)
+    with np.errstate(all="ignore"):
+        _, vv, _, vs = R.unpack(cache.cpu().numpy())
+    got = _np(A.attention_decode_q4(q, cache, table, n))
+    for b, tokens in enumerate(n.tolist()):
+        t = np.arange(tokens)
+        pg = table[b].cpu().numpy()[t // 16]
+        for h in range(2):
+            v, size = vv[pg, h, t % 16], vs[pg, h, t % 16]
+            assert np.all(np.abs(got[b, 2 * h:2 * h + 2] - v.mean(0)) <= 24 * E32 * size.mean(0))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+def test_decode_q4_queries_not_finite(dtype):
+    """An infinity or a NaN in a query makes its head's results NaN, as it makes every score, and no other's."""
+    cache, table, n, q, qx = _decode_case(13, [40, 3, 0], 4, 2, 64, 16, dtype)
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        x = q.clone()
+        x[:, 1, 7] = bad
+        got = A.attention_decode_q4(x, cache, table, n)
+        ref, bound = _decode_ref(cache, table, n, qx, 0.125, dtype, 16)
+        assert bool(torch.isnan(got[:2, 1]).all()) and not got[2].any()
+        _close(got[:, [0, 2, 3]], ref[:, [0, 2, 3]], bound[:, [0, 2, 3]])
+
+
 # ---- prompt attention ------------------------------------------------------------------------
 def _prefill_ref(qx, kx, vx, cu_q, cu_k, causal, scale, dtype):
     nh, nkv = qx.shape[1], kx.shape[1]
@@ -419,6 +473,24 @@ def test_prefill_hidden_values_have_no_part(dtype):
     _close(got[seen], ref[seen], bound[seen])
     assert bool(torch.isnan(got[100:150]).all()) and bool(torch.isnan(got[219]).all())
     assert not got[220:].any()
+
+
+def test_prefill_scores_of_minus_infinity():
+    """A key of score -inf has no weight, and a query that sees no other gets 0 / 0."""
+    q, k, v, cu_q, cu_k, x = _prefill_case(7, [140], [140], 2, 1, 64, "bf16")
+    qx, kx, vx, *cu = x
+    q[..., 3], qx[..., 3] = 1.0, 1.0
+    k[0, 0, 3], kx[0, 0, 3] = float("-inf"), -np.inf
+    got = A.attention_prefill(q, k, v, cu_q, cu_k)
+    kx[0] = 0.0  # (for the reference: the key is left out)
+    for h in range(2):
+        seen = np.tril(np.ones((140, 140), bool))
+        seen[:, 0] = False
+        ref, p_abs = R.attend(qx[:, h], kx[:, 0], vx[:, 0], 0.125, seen)
+        size = (np.abs(qx[:, h]) @ np.abs(kx[:, 0]).T * 0.125).max(-1)
+        step = R.HALF["bf16"] + 73 * E32 + np.expm1(2 * 72 * E32 * size)
+        _close(got[1:, h], ref[1:], step[1:, None] * p_abs[1:] + R.HALF["bf16"] * np.abs(ref[1:]) + 2.0 ** -25)
+    assert bool(torch.isnan(got[0]).all())
 
 
 def test_no_tokens():
@@ -644,6 +716,9 @@ def test_engine_options_and_refusals():
         eng.prefill([])
     with pytest.raises(ValueError, match="max_pos"):
         eng.prefill(np.zeros(101, np.int32))
+    for bad in (-1, 320):
+        with pytest.raises(ValueError, match="token ids"):
+            eng.prefill([3, bad])
     eng.step(3)
     eng.step(5)
     plain = _engine()

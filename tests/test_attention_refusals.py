@@ -105,6 +105,8 @@ def test_prefill_refusals():
                    ((q, k, k, cu), "CUDA device")):
         with pytest.raises(ValueError, match=msg):
             A.attention_prefill(*a)
+    with pytest.raises(ValueError, match="out must not be"):
+        A.attention_prefill(q, k, k, cu, out=q)
 
 
 def test_c_abi_refusals(lib):
@@ -132,12 +134,12 @@ def test_c_abi_refusals(lib):
                dict(qkv=None), dict(max_pos=0)):
         assert rope(**kw) == _lib.FRC_ERR_INVALID, kw
 
-    def decode(hd=64, nh=4, page=32, ws=1 << 30, q=p16, cache=p16, batch=2, table=p16):
-        return lib.frc_attention_decode_q4(0, q, 256, 64, cache, 3, page, table, 2, 2, p16, batch, nh, 2, hd, 0.1, p16,
+    def decode(hd=64, nh=4, page=32, ws=1 << 30, q=p16, cache=p16, batch=2, table=p16, scale=0.1):
+        return lib.frc_attention_decode_q4(0, q, 256, 64, cache, 3, page, table, 2, 2, p16, batch, nh, 2, hd, scale, p16,
                                            ws, p16, 256, 64, None)
 
     for kw in (dict(hd=96), dict(nh=5), dict(page=20), dict(ws=0), dict(q=None), dict(cache=ctypes.c_void_p(24)),
-               dict(batch=-1), dict(table=None)):
+               dict(batch=-1), dict(table=None), dict(scale=math.inf), dict(scale=math.nan)):
         assert decode(**kw) == _lib.FRC_ERR_INVALID, kw
     assert decode(batch=0, q=None) == 0
 
@@ -182,6 +184,8 @@ def test_rope_tables():
                 {"type": "llama3", "factor": 2, "original_max_position": 0}):
         with pytest.raises(ValueError):
             A.rope_tables_scaled(64, 1e4, 4, bad)
+    with pytest.raises(ValueError, match="theta"):
+        A.rope_tables_scaled(64, 1.0, 4, {"type": "yarn", "factor": 2, "original_max_position": 64})
 
 
 def test_oracle_of_the_cache_round_trips():
