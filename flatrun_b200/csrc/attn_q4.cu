@@ -38,7 +38,8 @@
 //    large as the result, where sum p d n grows with the tokens and cancels
 //    with sum p m (fp32: 2e-6 off at 4097 tokens), and roundings of p d count
 //    relative to a value's distance from its group's middle.  m + 8 d is in two
-//    parts for fp32, rounded to fp16 for 16-bit types as the stored m is.
+//    parts for fp32, rounded to fp16 for 16-bit types as the stored m is; where it
+//    lies beyond fp16 (values above 65504) m and d take a row each.
 //
 // The softmax's reference is not the largest s but the largest s + log2 d (d
 // the token's largest V step, at least 2^-7): so p d stays below 2^8 whatever the
@@ -54,13 +55,13 @@
 // places are looked up at once, a block a lane, a batch ahead) and writes the
 // units that lie wholly in its range.  (Whole CTAs on one unit with their warps
 // taking blocks in turn spent 3 us on each short sequence's head: 404 us for a
-// batch of 128 that takes 68 now.)  A unit that a boundary cuts is joined from its
+// batch of 128 that takes 69 now.)  A unit that a boundary cuts is joined from its
 // pieces, by the CTA where the CTA has all of them, otherwise from pieces that
 // the CTAs leave in the workspace, by a second kernel.
 //
-// Measured: 128 sequences of 1 to 8192 tokens, 64 / 8 heads of 128, bf16: 68 us
+// Measured: 128 sequences of 1 to 8192 tokens, 64 / 8 heads of 128, bf16: 69 us
 // (190 MB of cache: 2.8 TB/s, 0.43 of a plain copy); 131071 tokens, 32 / 8 heads,
-// fp16: 59 us.  About 440 warp instructions a block of 16 tokens and KV head
+// fp16: 60 us.  About 440 warp instructions a block of 16 tokens and KV head
 // keep the issue slots 68 % busy in the main loop, which is what binds.
 #include <cuda_runtime.h>
 
@@ -365,13 +366,18 @@ struct AqWarp {
     k1 = mine >= 4 ? 0xffffffffu : (mine == 3 ? 0xffffu : 0u);
   }
 
-  // The reference raised, where it has to be, to m (of the lane's tokens) and
-  // the other lanes' of the head.  It may stay up to kSlack below: the operands
-  // have that room, and most raises of a running maximum are small.
-  FRC_DEVICE_INLINE void refer(float m, int lane) {
+  // The reference raised, where it has to be, to m + d (of the lane's tokens: the
+  // largest score and the log2 of the largest V step) and the other lanes' of the
+  // head.  It may stay up to kSlack below: the operands have that room, and
+  // most raises of a running maximum are small.  True: a step is so large that
+  // m + 8 d may lie beyond fp16 (at m = 65504 a step of 2 rounds to it).
+  FRC_DEVICE_INLINE bool refer(float m, float d, int lane) {
+    m += d;
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    if (__any_sync(0xffffffffu, m > m_run + kSlack)) {
+    const bool up = m > m_run + kSlack, wide = d >= 1.f;
+    if (!__any_sync(0xffffffffu, up || wide)) return false;
+    if (__any_sync(0xffffffffu, up)) {
       const int q = lane & 3;
       const float m_new = fmaxf(m, m_run);
       const float keep = m_new == -INFINITY ? 1.f : ex2(m_run - m_new);
@@ -391,9 +397,11 @@ struct AqWarp {
       m_run = m_new;
       base = m_new == -INFINITY ? 0.f : m_new - kLift;
     }
+    return __any_sync(0xffffffffu, wide);
   }
 
-  // The block's values, weighted by its scores.
+  // The block's values, weighted by its scores; not TAIL: no sum m + 8 d lies
+  // beyond fp16.
   template <bool TAIL>
   FRC_DEVICE_INLINE void values(const uint8_t* blk, int left, int lane, uint32_t bias, const float (&s)[4]) {
     constexpr Q4Layout lay(HD);
@@ -434,17 +442,15 @@ struct AqWarp {
       l01 = pack_half2((p0 - g01.x) * kLow, (p1 - g01.y) * kLow);
       l23 = pack_half2((p2 - g23.x) * kLow, (p3 - g23.y) * kLow);
     }
-    const __half2 most = __hmax2(__habs2(bits_h2(vm.x)), __habs2(bits_h2(vm.y)));
-    if (__any_sync(0xffffffffu, !__hblt2(most, bits_h2(0x7c007c00u)))) {
-      // a sum m + 8 d beyond fp16 (values above 65504): m and d as rows of their own
+    bool apart = false;
+    if constexpr (TAIL) apart = beyond(bits_h2(vm.x), bits_h2(vm.y));
+    if (apart) {  // a sum m + 8 d beyond fp16 (values above 65504): m and d as rows of their own
       uint2 m = make_uint2(0u, 0u), d = m;
       if (r < NG) {
-        m = *reinterpret_cast<const uint2*>(blk + lay.v_offset(r, 4 * q));
-        d = *reinterpret_cast<const uint2*>(blk + lay.v_step(r, 4 * q));
-      }
-      if constexpr (TAIL) {
         uint32_t k0, k1;
         own_tokens(left - 4 * q, k0, k1);
+        m = *reinterpret_cast<const uint2*>(blk + lay.v_offset(r, 4 * q));
+        d = *reinterpret_cast<const uint2*>(blk + lay.v_step(r, 4 * q));
         m.x &= k0;
         m.y &= k1;
         d.x &= k0;
@@ -514,6 +520,22 @@ struct AqWarp {
     }
   }
 
+  // Whether one of a whole block's sums m + 8 d lies beyond fp16.
+  static FRC_DEVICE_INLINE bool beyond(const uint8_t* blk, int lane) {
+    constexpr Q4Layout lay(HD);
+    const int r = lane >> 2, q = lane & 3;
+    uint2 m = make_uint2(0u, 0u), d = m;
+    if (r < NG) {
+      m = *reinterpret_cast<const uint2*>(blk + lay.v_offset(r, 4 * q));
+      d = *reinterpret_cast<const uint2*>(blk + lay.v_step(r, 4 * q));
+    }
+    const __half2 eight = __float2half2_rn(8.f);
+    return beyond(__hfma2(bits_h2(d.x), eight, bits_h2(m.x)), __hfma2(bits_h2(d.y), eight, bits_h2(m.y)));
+  }
+  static FRC_DEVICE_INLINE bool beyond(__half2 a, __half2 b) {
+    return __any_sync(0xffffffffu, !__hblt2(__hmax2(__habs2(a), __habs2(b)), bits_h2(0x7c007c00u)));
+  }
+
   // What the reference has to cover of a lane's scores: the largest s + log2
   // of the largest V step of its tokens, taken apart: no less than the largest
   // s + log2 d.
@@ -531,19 +553,20 @@ struct AqWarp {
       __half2 dx = least;
       scores<false>(blk[0], 0, lane, bias, s0, dx);
       scores<false>(blk[1], 0, lane, bias, s1, dx);
-      refer(largest(s0, largest(s1, -INFINITY)) + log2_of(dx), lane);
-      values<false>(blk[0], 0, lane, bias, s0);
-      values<false>(blk[1], 0, lane, bias, s1);
-    } else {
-#pragma unroll 1
-      for (int e = 0; e < 2; ++e) {
-        if (!(seen >> e & 1u)) continue;
-        float s[4];
-        __half2 dx = least;
-        scores<true>(blk[e], left - e * kQ4Tokens, lane, bias, s, dx);
-        refer(largest(s, -INFINITY) + log2_of(dx), lane);
-        values<true>(blk[e], left - e * kQ4Tokens, lane, bias, s);
+      if (!refer(largest(s0, largest(s1, -INFINITY)), log2_of(dx), lane) || !(beyond(blk[0], lane) || beyond(blk[1], lane))) {
+        values<false>(blk[0], 0, lane, bias, s0);
+        values<false>(blk[1], 0, lane, bias, s1);
+        return;
       }
+    }
+#pragma unroll 1
+    for (int e = 0; e < 2; ++e) {
+      if (!(seen >> e & 1u)) continue;
+      float s[4];
+      __half2 dx = least;
+      scores<true>(blk[e], left - e * kQ4Tokens, lane, bias, s, dx);
+      refer(largest(s, -INFINITY), log2_of(dx), lane);
+      values<true>(blk[e], left - e * kQ4Tokens, lane, bias, s);
     }
   }
 
