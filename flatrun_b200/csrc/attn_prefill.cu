@@ -315,6 +315,24 @@ FRC_DEVICE_INLINE void pf_exps(const uint32_t* x, uint64_t scale2, float base, u
   }
 }
 
+// Lane l of a quad has w of its row, four units of four words: afterwards unit k
+// of lane l is unit l of lane k's row.
+FRC_DEVICE_INLINE void pf_quad_transpose(uint32_t (&w)[16], int lane) {
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (u & o) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t &a = w[4 * u + e], &b = w[4 * (u + o) + e];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, lane & o ? a : b, o);
+        if (lane & o) a = got;
+        else b = got;
+      }
+    }
+}
+
 // Asks for a block of the grid that has not started; the answer (16 bytes)
 // arrives on `bar`.
 FRC_DEVICE_INLINE void pf_ask(uint4* answer, uint64_t* bar) {
@@ -691,11 +709,16 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       if (!ok) break;
       pf_fence_after();
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      T* op = static_cast<T*>(p.out) + static_cast<int64_t>(w.q_start + row) * p.o_tok + (w.head + my_head) * p.o_head;
-      bool finite = sum != 0.f || seen == 0;  // all scores -inf: 0 / 0
+      const int64_t at = static_cast<int64_t>(w.q_start + row) * p.o_tok + (w.head + my_head) * p.o_head;
+      T* quad[4];  // the rows of the quad's lanes, from this lane's unit on
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        quad[k] = static_cast<T*>(p.out) + __shfl_sync(0xffffffffu, at, (lane & ~3) + k) + 8 * (lane & 3);
+      const uint32_t rows = __ballot_sync(0xffffffffu, live) >> (lane & ~3);
+      bool finite = sum != 0.f;  // all scores -inf: 0 / 0
 #pragma unroll
       for (int c = 0; c < HD; c += 32) {
-        float v[32];
+        uint32_t y[16];
         if (nt > 0) {
           uint32_t o[32];
           tmem_ld32(o_at + c, o);
@@ -706,16 +729,23 @@ __global__ void __launch_bounds__(kPfThreads, 1)
             if (lane == 0) mbar_arrive(&sh->o_free[t]);
           }
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            v[e] = seen == 0 ? 0.f : __uint_as_float(o[e]) * inv;
-            finite = finite && fabsf(v[e]) <= 3.402823466e38f;
+          for (int e = 0; e < 32; e += 2) {
+            const float v0 = __uint_as_float(o[e]) * inv, v1 = __uint_as_float(o[e + 1]) * inv;
+            finite = finite && fabsf(v0) <= 3.402823466e38f && fabsf(v1) <= 3.402823466e38f;
+            y[e / 2] = seen == 0 ? 0u : pf_pack<T>(v0, v1);
           }
         } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = 0.f;
+          for (int e = 0; e < 16; ++e) y[e] = 0u;
         }
-        if (live) store_run<32, true>(op + c, v);
+        // 64 bytes of a row in one store, not of 32 rows 16 each
+        pf_quad_transpose(y, lane);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (rows >> k & 1u)
+            *reinterpret_cast<uint4*>(quad[k] + c) = make_uint4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
       }
+      finite = finite || seen == 0;
       __syncwarp();
       for (uint32_t again = __ballot_sync(0xffffffffu, live && !finite); again; again &= again - 1)
         pf_row_again<T, HD>(p, w, w.head + __shfl_sync(0xffffffffu, my_head, __ffs(again) - 1),
