@@ -633,7 +633,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     for (int i = 0; ok && any; ++i) {
       const int nt = w.tiles(p, t), row = w.q0 + p.queries * t + my_query;
       const bool live = my_query < w.queries(p, t);
-      const int seen = live ? w.seen(p, row) : w.k_len;  // rows without a query: nothing to mask
+      // rows without a query mask as the tile's last one
+      const int seen = w.seen(p, min(row, w.q0 + p.queries * t + w.queries(p, t) - 1));
       float m_ref = -INFINITY, base = 0.f, sum = 0.f;  // reference in units of the unscaled score, and scaled
       for (int j = 0; j < nt; ++j, ++done) {
         ok = wait(&sh->s_full[t], done);
@@ -645,8 +646,13 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         tmem_wait_ld();
         const int mine = seen - j * kPfRows;  // columns that the row sees
         if (!__all_sync(0xffffffffu, mine >= kPfRows)) {
+          const int least = __reduce_min_sync(0xffffffffu, mine);
 #pragma unroll
-          for (int c = 0; c < kPfRows; ++c) x[c] = c < mine ? x[c] : 0xff800000u;
+          for (int c = 0; c < kPfRows; c += 32)
+            if (c + 32 > least) {
+#pragma unroll
+              for (int e = c; e < c + 32; ++e) x[e] = e < mine ? x[e] : 0xff800000u;
+            }
         }
         // the first quarter's exponentials run with the old reference while the
         // maximum is formed, and again in the few tiles that raise it
