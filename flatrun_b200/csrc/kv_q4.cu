@@ -75,9 +75,9 @@ __device__ __noinline__ uint32_t border8(float x0, float x1, float x2, float x3,
   uint32_t w = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    // h: the border nearest to 15 t; e: on which side of it x - m lies.  s + err is
+    // h: the border nearest to t; e: on which side of it x - m lies.  s + err is
     // x - m exactly (two-sum), and s - h d is exact near the border
-    const float t = 15.f * __saturatef((x[i] - m) * inv);
+    const float t = fminf(fmaxf((x[i] - m) * inv, 0.f), 15.f);
     const float h = fminf(fmaxf(rintf(t - 0.5f), 0.f), 14.f) + 0.5f;
     const float s = __fsub_rn(x[i], m), v = __fsub_rn(s, x[i]);
     const float err = __fsub_rn(__fsub_rn(x[i], __fsub_rn(s, v)), __fadd_rn(m, v));
@@ -112,26 +112,27 @@ FRC_DEVICE_INLINE uint32_t quantise8(const float (&x)[8], __half& step, __half& 
   const float m = __half2float(offset);
   step = step_of(hi, m);
   const float d = __half2float(step);
-  float inv;  // of 15 d, which is exact; within an ulp
-  asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(15.f * d));
+  float inv;  // of d, within an ulp
+  asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(d));
   if (d == 0.f) inv = 0.f;
-  // t = (x - m) / (15 d) held within 0 .. 1, n = round(15 t) in the low bits of
-  // the sum with 1.5 * 2^23.  t is off by 2^-24 (difference), 2^-23 (reciprocal) and
-  // 2^-24 (product) of itself, so 15 t by less than 4e-6.
+  // n = round((x - m) / d) in the low bits of the sum with 1.5 * 2^23.  The quotient is
+  // off by 2^-24 (difference) and 2^-23 (reciprocal) of itself, less than 4e-6.
   constexpr float kMagic = 12582912.f;
+  const uint64_t inv2 = f32x2_two(inv, inv), m2 = f32x2_two(-m, -m), magic2 = f32x2_two(kMagic, kMagic);
   uint32_t w = 0;
-  float far = 0.f;  // the largest distance from a whole number
+  // the largest distance from a whole number, or (where m or d was rounded by as much) of
+  // the quotients beyond 0 and 15
+  float far = max_nan((m - lo) * inv, fmaf(hi - m, inv, -15.f), 0.f);
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
-    float off[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float t = __saturatef((x[i + e] - m) * inv);
-      const float u = fmaf(t, 15.f, kMagic);
-      off[e] = fabsf(fmaf(t, 15.f, kMagic - u));
-      w += __float_as_uint(u) << (4 * (i + e));
-    }
-    far = max_nan(far, off[0], off[1]);
+    const uint64_t t = f32x2_add(f32x2_two(x[i], x[i + 1]), m2), u = f32x2_fma(t, inv2, magic2);
+    float u0, u1, off0, off1;
+    f32x2_split(u, u0, u1);
+    // t inv - (u - magic)
+    f32x2_split(f32x2_fma(t, inv2, f32x2_fma(u, f32x2_two(-1.f, -1.f), magic2)), off0, off1);
+    far = max_nan(far, fabsf(off0), fabsf(off1));
+    w += __float_as_uint(u0) << (4 * i);
+    w += __float_as_uint(u1) << (4 * i + 4);
   }
   // the sums' other bits, 0x4B400000 each, add up to this
   constexpr uint32_t kSum = 0x4B400000u * 0x11111111u;
