@@ -876,12 +876,7 @@ __global__ void __launch_bounds__(kAqJoinWarps * 32) attn_q4_join_kernel(const A
   auto row = [&](int k) {  // the cut unit starts in CTA i (its second piece) and goes on as the others' first
     return p.part + (static_cast<int64_t>(k == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + k)) * kAqHeads + h) * ROW;
   };
-  float M = -INFINITY;  // of all pieces, in every warp
-  for (int k = lane; k < np; k += 32) M = fmaxf(M, row(k)[0]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  const float base = M == -INFINITY ? 0.f : M;
-  float L = 0.f, acc[C];
+  float M = -INFINITY, L = 0.f, acc[C];  // of the warp's pieces
 #pragma unroll
   for (int e = 0; e < C; ++e) acc[e] = 0.f;
   for (int k = warp; k < np; k += 8 * kAqJoinWarps) {  // eight pieces' loads at a time
@@ -900,6 +895,14 @@ __global__ void __launch_bounds__(kAqJoinWarps * 32) attn_q4_join_kernel(const A
         load_run<C, true>(r + 4 + C * lane, v[j]);
       }
     }
+    float top = M;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, m[j]);
+    const float base = top == -INFINITY ? 0.f : top, keep = ex2(M - base);
+    M = top;
+    L *= keep;
+#pragma unroll
+    for (int e = 0; e < C; ++e) acc[e] *= keep;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float f = ex2(m[j] - base);
@@ -909,18 +912,28 @@ __global__ void __launch_bounds__(kAqJoinWarps * 32) attn_q4_join_kernel(const A
     }
   }
   __shared__ __align__(16) float sums[kAqJoinWarps][HD];
-  __shared__ float ls[kAqJoinWarps];
+  __shared__ float ms[kAqJoinWarps], ls[kAqJoinWarps];
   store_run<C, true>(&sums[warp][C * lane], acc);
-  if (lane == 0) ls[warp] = L;
+  if (lane == 0) {
+    ms[warp] = M;
+    ls[warp] = L;
+  }
   __syncthreads();
   if (warp == 0) {
 #pragma unroll
-    for (int w = 1; w < kAqJoinWarps; ++w) {
+    for (int w = 1; w < kAqJoinWarps; ++w) M = fmaxf(M, ms[w]);
+    const float base = M == -INFINITY ? 0.f : M;
+    L = 0.f;
+#pragma unroll
+    for (int e = 0; e < C; ++e) acc[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kAqJoinWarps; ++w) {
       float v[C];
       load_run<C, true>(&sums[w][C * lane], v);
-      L += ls[w];
+      const float f = ex2(ms[w] - base);
+      L = fmaf(ls[w], f, L);
 #pragma unroll
-      for (int e = 0; e < C; ++e) acc[e] += v[e];
+      for (int e = 0; e < C; ++e) acc[e] = fmaf(v[e], f, acc[e]);
     }
     aq_store<C, T>(p, d.x, heads.first + h, C * lane, acc, L);
   }
