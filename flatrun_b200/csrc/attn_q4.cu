@@ -718,7 +718,8 @@ __global__ void __launch_bounds__(kAqThreads, 2) attn_q4_kernel(const AttnQ4Para
       const int at = issued & 15;
       if (at == 0) {
         blk = blk_next;
-        look_up(issued + 16);
+      } else if (at == 8) {
+        look_up(issued + 8);
       }
       const uint32_t bits = __ballot_sync(0xffffffffu, blk >= 0) >> (2 * at) & 3u;
       seen = (seen & ~(3u << (2 * s))) | bits << (2 * s);
@@ -806,7 +807,16 @@ __global__ void __launch_bounds__(kAqThreads, 2) attn_q4_kernel(const AttnQ4Para
   static_assert(SM::kPieces <= 32, "a piece a lane");
   const int4 pc = sh->piece[lane & (SM::kPieces - 1)];
   const bool own = lane < SM::kPieces && pc.x >= 0;
-  for (uint32_t left = __ballot_sync(0xffffffffu, own); left;) {
+  const uint32_t present = __ballot_sync(0xffffffffu, own);
+  constexpr int C = HD / 32, N = SM::kPieces;
+  float v[N][C];  // the head's part of all pieces, loaded together
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+#pragma unroll
+    for (int e = 0; e < C; ++e) v[j][e] = 0.f;
+    if (present >> j & 1u) load_run<C, true>(piece_rows(j) + warp * SM::kRow + C * lane, v[j]);
+  }
+  for (uint32_t left = present; left;) {
     const int k = __ffs(left) - 1;
     const int seq = __shfl_sync(0xffffffffu, pc.x, k), unit = __shfl_sync(0xffffffffu, pc.y, k);
     const int u0 = __shfl_sync(0xffffffffu, pc.z, k), u1 = __shfl_sync(0xffffffffu, pc.w, k);
@@ -814,7 +824,6 @@ __global__ void __launch_bounds__(kAqThreads, 2) attn_q4_kernel(const AttnQ4Para
     left &= ~same;
     const AqHeads heads(p, unit);
     if (warp < heads.count) {
-      constexpr int C = HD / 32, N = SM::kPieces;
       float m[N], l[N];
       load_run<N, true>(sh->m[warp], m);
       load_run<N, true>(sh->l[warp], l);
@@ -825,22 +834,12 @@ __global__ void __launch_bounds__(kAqThreads, 2) attn_q4_kernel(const AttnQ4Para
 #pragma unroll
       for (int e = 0; e < C; ++e) acc[e] = 0.f;
 #pragma unroll
-      for (int j0 = 0; j0 < N; j0 += 8) {  // eight pieces' loads at a time
-        float v[8][C];
+      for (int j = 0; j < N; ++j) {
+        if (!(same >> j & 1u)) continue;
+        const float f = ex2(m[j] - base);
+        L = fmaf(l[j], f, L);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-#pragma unroll
-          for (int e = 0; e < C; ++e) v[j][e] = 0.f;
-          if (same >> (j0 + j) & 1u) load_run<C, true>(piece_rows(j0 + j) + warp * SM::kRow + C * lane, v[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool in = same >> (j0 + j) & 1u;
-          const float f = in ? ex2(m[j0 + j] - base) : 0.f;
-          L = fmaf(in ? l[j0 + j] : 0.f, f, L);
-#pragma unroll
-          for (int e = 0; e < C; ++e) acc[e] = fmaf(v[j][e], f, acc[e]);
-        }
+        for (int e = 0; e < C; ++e) acc[e] = fmaf(v[j][e], f, acc[e]);
       }
       if (u0 >= 0 && u1 <= count) {
         aq_store<C, T>(p, seq, heads.first + warp, C * lane, acc, L);
