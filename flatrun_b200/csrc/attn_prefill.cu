@@ -39,10 +39,15 @@
 // that comes out not finite (a NaN or infinity among the keys of its tile that it
 // does not see makes 0 * NaN) is computed again from the keys it sees alone.
 //
-// Measured: 8192 tokens, causal, 64 / 8 heads of 128, bf16: 0.99 ms, 1115 TFLOP/s (0.67
-// of cuBLAS's burst rate, 0.80 of its sustained one; the card is at its power
+// Measured: 8192 tokens, causal, 64 / 8 heads of 128, bf16: 0.98 ms, 1124 TFLOP/s (0.68
+// of cuBLAS's burst rate, 0.81 of its sustained one; the card is at its power
 // limit).  A key tile's chain of scores, softmax and products takes a query tile
-// 3000 cycles; the two tiles in turn keep the tensor pipe two thirds busy.
+// 3000 cycles (1800 in the softmax); the two tiles in turn keep the tensor pipe two
+// thirds busy.  Scores of the next 64 keys formed early, in the half of S's columns
+// that P leaves free, took 9 % longer: products with 64 columns cost as much as
+// with 128.  17 packed prompts of 1 to 1000 queries, 32 / 8 heads of 64, fp16: 48 us.  Code
+// size counts: a second copy of the softmax step for tiles with masks took
+// 52 us, and skipping hidden quarters' exponentials costs the long prompt 3 %.
 #include <cuda.h>
 #include <cuda_runtime.h>
 

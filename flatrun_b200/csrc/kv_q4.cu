@@ -16,10 +16,10 @@
 // group at a time: a group's minimum and maximum are two shuffles, a lane's eight
 // nibbles are one word, a token's K words one 4 NG byte store, and the V words of
 // eight consecutive tokens a full 32-byte sector.  65536 tokens of 8 heads of 128 in
-// bf16: 121 us appended (830 warp instructions for eight tokens of a head: the
-// issue slots bind at 2.9 TB/s), 64 us read (5.5 TB/s).  Two lanes a token
-// with twice the channels took 163 us: fewer instructions, but more code than the
-// instruction cache holds.
+// bf16: 117 us appended (750 warp instructions for eight tokens of a head: the
+// issue slots bind at 3.0 TB/s), 64 us read (5.5 TB/s).  Two lanes a token
+// with twice the channels took 163 us where this took 121: fewer instructions, but
+// more code than the instruction cache holds.
 #include <cuda_runtime.h>
 
 #include <cstdio>
