@@ -44,8 +44,8 @@
 // limit).  A key tile's chain of scores, softmax and products takes a query tile
 // 3000 cycles (1800 in the softmax); the two tiles in turn keep the tensor pipe two
 // thirds busy.  Scores of the next 64 keys formed early, in the half of S's columns
-// that P leaves free, took 9 % longer: products with 64 columns cost as much as
-// with 128.  17 packed prompts of 1 to 1000 queries, 32 / 8 heads of 64, fp16: 48 us.  Code
+// that P leaves free, took 9 % longer (two products of 64 columns in place of one of
+// 128).  17 packed prompts of 1 to 1000 queries, 32 / 8 heads of 64, fp16: 48 us.  Code
 // size counts: a second copy of the softmax step for tiles with masks took
 // 52 us, and skipping hidden quarters' exponentials costs the long prompt 3 %.
 #include <cuda.h>
