@@ -150,8 +150,11 @@ class DecodeEngine:
         start = 0
         for i, (kp, vp) in (kv_prefill or {}).items():
             start = kp.shape[0]
+            if start > c.max_pos:
+                raise ValueError(f"kv_prefill holds {start} positions, max_pos is {c.max_pos}")
             self._store(i, 0, up(kp, np.float32).reshape(kp.shape), up(vp, np.float32).reshape(vp.shape))
         self.pos = torch.tensor([start], dtype=torch.int32, device=self._dev)
+        self._filled = start  # the position, known to the host: a token at max_pos would lie behind tables and caches
         if kv_bits == 4:  # the token's slot, and the number of tokens with it
             self._slot = torch.tensor([start], dtype=torch.int64, device=self._dev)
             self._length = torch.tensor([start + 1], dtype=torch.int32, device=self._dev)
@@ -282,6 +285,7 @@ class DecodeEngine:
     def capture(self) -> None:
         """Record one token as a CUDA graph (replayed by step())."""
         torch = self.torch
+        self._room(1)  # the eager token below writes its cache row
         with torch.cuda.stream(self.stream):
             # one eager token first: lazy module loading and launch
             # configuration happen outside the capture; then undo its effects
@@ -298,8 +302,10 @@ class DecodeEngine:
 
     def step(self, token: int | None = None) -> None:
         """One token: feed `token` (None: the previous step's argmax) and
-        advance the position.  Asynchronous on the engine's stream."""
+        advance the position.  Asynchronous on the engine's stream.  Raises
+        ValueError where max_pos tokens are there already."""
         torch = self.torch
+        self._room(1)
         with torch.cuda.stream(self.stream):
             if token is not None:
                 self.tok_in.fill_(int(token))
@@ -307,13 +313,18 @@ class DecodeEngine:
                 self._token()
             else:
                 self._graph.replay()
+        self._filled += 1
+
+    def _room(self, tokens: int) -> None:
+        if self._filled + tokens > self.cfg.max_pos:
+            raise ValueError(f"{tokens} tokens from position {self._filled} on pass max_pos {self.cfg.max_pos}")
 
     def prefill(self, tokens) -> None:
         """Feed a prompt at once, behind what the cache holds: afterwards `logits`
         and `argmax_host()` are those of its last token, and `step()` goes on.
         The projections run batched (above 16 tokens with fp16 operands, as
         frc_gemv's), the attention on fp16 queries, keys and values;
-        asynchronous on the engine's stream but for reading the position."""
+        asynchronous on the engine's stream."""
         from . import attention
 
         torch, c, lib, f32 = self.torch, self.cfg, self.lib, self.torch.float32
@@ -324,10 +335,9 @@ class DecodeEngine:
             raise ValueError("an empty prompt")
         if ids.min() < 0 or ids.max() >= c.vocab:
             raise ValueError(f"token ids must lie in 0 .. {c.vocab - 1}")
+        self._room(n)
+        start = self._filled
         with torch.cuda.stream(self.stream):
-            start = int(self.pos.item())
-            if start + n > c.max_pos:
-                raise ValueError(f"{n} tokens from position {start} on pass max_pos {c.max_pos}")
             ids_dev = torch.from_numpy(ids).to(self._dev)
             h = torch.empty((n, c.hidden), dtype=f32, device=self._dev)
             for t in range(n):
@@ -382,6 +392,7 @@ class DecodeEngine:
             if self.kv_bits == 4:
                 self._slot += n
                 self._length += n
+        self._filled += n
 
     def logits_host(self) -> np.ndarray:
         self.stream.synchronize()

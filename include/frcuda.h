@@ -220,7 +220,8 @@ int frc_gemv_ex(int quant, int count, const void* const* w_dev, const size_t* w_
  *  frc_rope_append: qkv = [q (nh*hd) | k (nkv*hd) | v (nkv*hd)] of one token;
  *    adds `bias` (same layout, may be NULL), rotates q in place and k at
  *    position *pos_dev with cos/sin tables [max_pos][hd/2], writes k and v to
- *    row *pos_dev of the caches ([max_pos][nkv][hd]).
+ *    row *pos_dev of the caches ([max_pos][nkv][hd]).  It is not told max_pos:
+ *    the caller keeps *pos_dev below it (DecodeEngine counts on the host).
  *  frc_attention_decode: one query token (q, nh*hd, rotated) over cache rows
  *    0..*pos_dev: softmax(q.k * scale) . v per head, query head h reading KV
  *    head h / (nh/nkv); positions split into `splits` ranges (flash
