@@ -414,7 +414,7 @@ def attention_prefill(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: f
     if tokens and (o_row <= 0 < tokens - 1 or o_head <= 0 < nh - 1):
         raise ValueError("the rows or heads of out overlap")
     if at[3] in at[:3] and tokens:
-        raise ValueError("out must not be q, k or v: their rows are read again where a result is not finite")
+        raise ValueError("out must not be q, k or v: they are read while its rows are written")
     _no_grad(q, k, v)
     _launch(_device(q, k, v, cu_q, cu_k, out), _PREFILL, _TYPE[dtype], at[0], q_row, q_head, at[1], k_row, k_head,
             at[2], v_row, v_head, cu_q.data_ptr(), cu_k.data_ptr(), cu_q.shape[0] - 1, tokens, tokens_k, nh, nkv, hd,

@@ -24,6 +24,8 @@
 //   warp 8        issues tcgen05.mma: S = Q K^T (128 x 128 fp32 in tensor
 //                 memory), and O += P V with P read from tensor memory, where
 //                 it takes the place of S; V is the transposed operand as it lies
+//   warp 10       makes V tiles ready: rows behind the last key zeroed, and in tiles
+//                 that some row does not see whole all elements that are not finite
 //   warps 0-3,    softmax of tile 0 and 1, a row a thread: maximum, exponentials,
 //   warps 4-7     P rounded to the type of the inputs, handed over in two parts;
 //                 at the end O / sum.  (Two threads a row took 1134 us where one
@@ -35,9 +37,11 @@
 // must be, and the sum is of the unrounded values.
 //
 // What is masked has no part in the result whatever it holds: scores are
-// replaced, V rows behind the last key are zeroed in shared memory, and a row
-// that comes out not finite (a NaN or infinity among the keys of its tile that it
-// does not see makes 0 * NaN) is computed again from the keys it sees alone.
+// replaced, V rows behind the last key are zeroed in shared memory, and so are NaNs
+// and infinities of V in tiles that some row does not see whole (0 * NaN would reach
+// the rows that do not see them).  Rows that do see one get it added at the end
+// (pf_add_seen), so that an element that is not finite costs the rows beside it
+// nothing and no row is computed twice.
 //
 // Measured: 8192 tokens, causal, 64 / 8 heads of 128, bf16: 0.98 ms, 1124 TFLOP/s (0.68
 // of cuBLAS's burst rate, 0.81 of its sustained one; the card is at its power
@@ -169,14 +173,17 @@ struct PfSmem {
   static constexpr int kHalf = kPfRows * 128;           // 64 channels of 128 rows, swizzled: 16 KB
   static constexpr int kTile = HD / 64 * kHalf;
   static constexpr int kStages = HD == 128 ? 5 : 8;
+  static constexpr int kVTiles = (kStages + 1) / 2;  // V tiles that the ring can hold: every second tile is one
   alignas(1024) uint8_t q[kPfTiles][kTile];
   alignas(1024) uint8_t ring[kStages][kTile];
   uint64_t q_full, q_empty, full[kStages], empty[kStages];
+  uint64_t clean[kVTiles];  // V tile v of the CTA is ready: entry v % kVTiles
   uint64_t s_full[kPfTiles], p_ready[kPfTiles][2], o_done[kPfTiles], o_free[kPfTiles], drain;
   alignas(16) uint4 answer;  // to the request for the next block
   uint64_t answered;
   PfWork work[2];            // items 1, 2, ... by turns
   int any[2];                // whether there is one
+  int taken_out[4];          // of items by turns: elements of V were zeroed
   uint64_t work_full[2], work_empty[2];
   uint32_t tmem;
   int abort;
@@ -364,37 +371,62 @@ FRC_DEVICE_INLINE int pf_answer(const uint4* answer) {
   return block;
 }
 
-// Query `row` of head h from the keys it sees alone: a warp, HD / 32 channels a lane.
+template <typename T>
+constexpr uint32_t kPfInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;  // bits of infinity
+
+// Zeroes the elements of a V tile's first `rows` rows that are not finite.  True:
+// there are some.  A warp.
 template <typename T, int HD>
-__device__ __noinline__ void pf_row_again(const PrefillParams& p, const PfWork& w, int h, int row, int lane) {
+FRC_DEVICE_INLINE bool pf_clean(uint8_t* tile, int rows, int lane) {
+  constexpr uint32_t inf = kPfInf<T>;
+  uint32_t top = 0;
+  for (int h = 0; h < HD / 64; ++h) {
+    const uint4* at = reinterpret_cast<const uint4*>(tile + h * PfSmem<HD>::kHalf);
+#pragma unroll 4
+    for (int e = lane; e < rows * 8; e += 32) {
+      const uint4 v = at[e];
+      top = __vmaxu2(top, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
+                                   __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+    }
+  }
+  if (!__any_sync(0xffffffffu, (top & 0xffffu) >= inf || top >> 16 >= inf)) return false;
+  for (int h = 0; h < HD / 64; ++h) {
+    uint32_t* at = reinterpret_cast<uint32_t*>(tile + h * PfSmem<HD>::kHalf);
+    for (int e = lane; e < rows * 32; e += 32) {
+      const uint32_t v = at[e];
+      const uint32_t keep = ((v & 0x7fffu) < inf ? 0xffffu : 0u) | ((v >> 16 & 0x7fffu) < inf ? 0xffff0000u : 0u);
+      if (keep != 0xffffffffu) at[e] = v & keep;
+    }
+  }
+  return true;
+}
+
+// Adds to the warp's rows what pf_clean took out of the tiles from key `first` on
+// and they see: a value that is not finite makes the sum so whatever its weight.
+// `at`: the lane's row of the output, `seen`: its keys (0: none, or no row).  At
+// most 128 keys more than the item has queries, so the other warps do not wait long.
+template <typename T, int HD>
+__device__ __noinline__ void pf_add_seen(const PrefillParams& p, const PfWork& w, int first, int seen, int64_t at, int lane) {
   constexpr int C = HD / 32;
-  const int g = w.kvh;
-  const T* qp = static_cast<const T*>(p.q) + (w.q_start + row) * p.q_tok + h * p.q_head;
-  float qv[C], acc[C];
+  const int end = __reduce_max_sync(0xffffffffu, seen);
+  for (int j = first; j < end; ++j) {
+    const T* vp = static_cast<const T*>(p.v) + (w.k_start + static_cast<int64_t>(j)) * p.v_tok + w.kvh * p.v_head + C * lane;
+    float v[C];
+    bool some = false;
 #pragma unroll
-  for (int e = 0; e < C; ++e) {
-    qv[e] = to_f32(qp[C * lane + e]);
-    acc[e] = 0.f;
+    for (int e = 0; e < C; ++e) {
+      v[e] = to_f32(vp[e]);
+      if (fabsf(v[e]) <= 3.402823466e38f) v[e] = 0.f;  // finite: the products had it
+      else some = true;
+    }
+    if (!__any_sync(0xffffffffu, some)) continue;
+    for (uint32_t rows = __ballot_sync(0xffffffffu, seen > j); rows; rows &= rows - 1) {
+      T* op = static_cast<T*>(p.out) + __shfl_sync(0xffffffffu, at, __ffs(rows) - 1) + C * lane;
+#pragma unroll
+      for (int e = 0; e < C; ++e)
+        if (!(v[e] == 0.f)) from_f32(to_f32(op[e]) + v[e], op[e]);
+    }
   }
-  float mx = -INFINITY, sum = 0.f;
-  const int n = w.seen(p, row);
-  for (int j = 0; j < n; ++j) {
-    const int64_t t = w.k_start + j;
-    const T* kp = static_cast<const T*>(p.k) + t * p.k_tok + g * p.k_head + C * lane;
-    const T* vp = static_cast<const T*>(p.v) + t * p.v_tok + g * p.v_head + C * lane;
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < C; ++e) s = fmaf(qv[e], to_f32(kp[e]), s);
-    s = warp_sum(s) * p.signed_scale;
-    const float m_new = fmaxf(mx, s), keep = mx == m_new ? 1.f : expf(mx - m_new), x = expf(s - m_new);
-    mx = m_new;
-    sum = fmaf(sum, keep, x);
-#pragma unroll
-    for (int e = 0; e < C; ++e) acc[e] = fmaf(acc[e], keep, x * to_f32(vp[e]));
-  }
-  T* op = static_cast<T*>(p.out) + (w.q_start + row) * p.o_tok + h * p.o_head;
-#pragma unroll
-  for (int e = 0; e < C; ++e) from_f32(acc[e] / sum, op[C * lane + e]);
 }
 
 template <typename T, int HD>
@@ -426,8 +458,9 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       mbar_init(&sh->o_done[t], 1);
       mbar_init(&sh->o_free[t], 4);
       mbar_init(&sh->work_full[t], 1);
-      mbar_init(&sh->work_empty[t], 9);  // the softmax warps and the product warp
+      mbar_init(&sh->work_empty[t], 10);  // the softmax warps, the product warp and warp 10
     }
+    for (int v = 0; v < SM::kVTiles; ++v) mbar_init(&sh->clean[v], 1);
     mbar_init(&sh->answered, 1);
     mbar_init(&sh->drain, 1);
     sh->abort = 0;
@@ -551,6 +584,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       auto release = [&](int stage) { pf_commit(one, &sh->empty[stage]); };
       bool ok = true;
       int used = 0, items = 0;                           // K and V tiles, items that had queries
+      int v_used = 0;                                    // V tiles
       int done[kPfTiles] = {0, 0}, outs[kPfTiles] = {0, 0};  // key tiles and items of each query tile
       for (int i = 0; ok && any; ++i) {
         const int nt[kPfTiles] = {w.tiles(p, 0), w.tiles(p, 1)};
@@ -567,17 +601,9 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           ++used;
           for (int j = 0; ok && j < n; ++j) {
             const int sv = used % NS, sk = (used + 1) % NS;
-            ok = wait(&sh->full[sv], used / NS);
+            ok = wait(&sh->full[sv], used / NS) && wait(&sh->clean[v_used % SM::kVTiles], v_used / SM::kVTiles);
             if (!ok) break;
-            const int left = w.k_len - j * kPfRows;
-            if (left < kPfRows) {  // rows behind the last key: zeros, whatever lies there
-              uint4* row = reinterpret_cast<uint4*>(sh->ring[sv]);
-              for (int h = 0; h < H; ++h)
-                for (int e = left * 8 + lane; e < kPfRows * 8; e += 32)
-                  row[h * (SM::kHalf / 16) + e] = make_uint4(0, 0, 0, 0);
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-              __syncwarp();
-            }
+            ++v_used;
             bool k_there = false;
 #pragma unroll
             for (int t = 0; t < kPfTiles; ++t) {
@@ -623,6 +649,42 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       pf_commit(one, &sh->drain);
       int zero = 0;
       if (!wait_phase(&sh->drain, 0, &zero) && lane == 0) atomicOr(p.status, kStatusDrainTimeout);
+    } else if (warp == 10) {
+      // ---- V tiles made ready ------------------------------------------------------------------
+      // A V tile's stage is not filled again before the product warp has waited for
+      // its entry of `clean`, so this warp misses no phase of `full`; and the ring holds
+      // no more V tiles than `clean` has entries, so the product warp misses none.
+      bool ok = true;
+      int used = 0, v_used = 0;
+      for (int i = 0; ok && any; ++i) {
+        const int n = max(w.tiles(p, 0), w.tiles(p, 1));
+        const int whole = p.causal ? w.seen(p, w.q0) / kPfRows : n;  // tiles that all rows see whole
+        // read by the softmax warps at the end of the item; two items ahead at most, this
+        // warp writes no other's entry
+        volatile int* taken_out = &sh->taken_out[i & 3];
+        if (lane == 0) *taken_out = 0;
+        __syncwarp();
+        for (int j = 0; j < n; ++j, used += 2, ++v_used) {
+          const int s = (used + 1) % NS, left = w.k_len - j * kPfRows;
+          ok = wait(&sh->full[s], (used + 1) / NS);
+          if (!ok) break;
+          if (j >= whole && pf_clean<T, HD>(sh->ring[s], min(left, kPfRows), lane)) *taken_out = 1;
+          if (left < kPfRows) {  // rows behind the last key: zeros, whatever lies there
+            uint4* row = reinterpret_cast<uint4*>(sh->ring[s]);
+            for (int h = 0; h < H; ++h)
+              for (int e = left * 8 + lane; e < kPfRows * 8; e += 32)
+                row[h * (SM::kHalf / 16) + e] = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->clean[v_used % SM::kVTiles]);
+        }
+        ok = ok && follow(i);
+      }
+      if (!ok) {
+        *abort = 1;
+        if (lane == 0) atomicOr(p.status, kStatusFullWaitTimeout);
+      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPfRegsSoftmax));
@@ -719,14 +781,13 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       if (ok && nt > 0) ok = wait(&sh->o_done[t], done - 1);
       if (!ok) break;
       pf_fence_after();
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const float inv = 1.f / sum;  // all scores -inf: 0 / 0
       const int64_t at = static_cast<int64_t>(w.q_start + row) * p.o_tok + (w.head + my_head) * p.o_head;
       T* quad[4];  // the rows of the quad's lanes, from this lane's unit on
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         quad[k] = static_cast<T*>(p.out) + __shfl_sync(0xffffffffu, at, (lane & ~3) + k) + 8 * (lane & 3);
       const uint32_t rows = __ballot_sync(0xffffffffu, live) >> (lane & ~3);
-      bool finite = sum != 0.f;  // all scores -inf: 0 / 0
 #pragma unroll
       for (int c = 0; c < HD; c += 32) {
         uint32_t y[16];
@@ -742,7 +803,6 @@ __global__ void __launch_bounds__(kPfThreads, 1)
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             const float v0 = __uint_as_float(o[e]) * inv, v1 = __uint_as_float(o[e + 1]) * inv;
-            finite = finite && fabsf(v0) <= 3.402823466e38f && fabsf(v1) <= 3.402823466e38f;
             y[e / 2] = seen == 0 ? 0u : pf_pack<T>(v0, v1);
           }
         } else {
@@ -756,11 +816,10 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           if (rows >> k & 1u)
             *reinterpret_cast<uint4*>(quad[k] + c) = make_uint4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
       }
-      finite = finite || seen == 0;
-      __syncwarp();
-      for (uint32_t again = __ballot_sync(0xffffffffu, live && !finite); again; again &= again - 1)
-        pf_row_again<T, HD>(p, w, w.head + __shfl_sync(0xffffffffu, my_head, __ffs(again) - 1),
-                            __shfl_sync(0xffffffffu, row, __ffs(again) - 1), lane);
+      if (nt > 0 && *static_cast<volatile int*>(&sh->taken_out[i & 3])) {
+        __syncwarp();  // the rows were written by the lanes of their quads
+        pf_add_seen<T, HD>(p, w, w.seen(p, w.q0) / kPfRows * kPfRows, live ? seen : 0, at, lane);
+      }
       ok = follow(i);
     }
     if (!ok && lane == 0) atomicOr(p.status, kStatusFullWaitTimeout);

@@ -291,9 +291,10 @@ int frc_pos_advance(int* pos_dev, void* stream);
  *    cu_q[b] .. cu_q[b + 1] of q and out and rows cu_k[b] .. cu_k[b + 1] of k
  *    and v; causal: the last query of a sequence sees all its keys, each
  *    earlier one a key less.  A query that sees no key gives zeros; rows of no
- *    sequence stay as they are.  type FRC_F16 or FRC_BF16, hd 64 or 128;
- *    pointers 16-byte aligned and strides multiples of 8; out apart from q, k
- *    and v (rows whose result is not finite are read again). */
+ *    sequence stay as they are.  A value that is not finite reaches the rows that
+ *    see it, in its channel; masked ones reach none.  type FRC_F16 or
+ *    FRC_BF16, hd 64 or 128; pointers 16-byte aligned and strides multiples of
+ *    8; out apart from q, k and v (they are read while rows are written). */
 int frc_qk_norm_rope(int in_type, int out_type, const void* qkv, int64_t row_stride, int64_t tokens, int nh, int nkv,
                      int hd, const float* bias, const float* q_norm, const float* k_norm, float eps,
                      const float* cos_table, const float* sin_table, int64_t max_pos, int rot, int interleaved,
