@@ -5,7 +5,8 @@
 //
 // query head h reading KV head h / (nh / nkv).  A page number outside the
 // cache hides the page's tokens, and a sequence of no (visible) tokens gives
-// zeros, so no table can lead a read out of the cache.
+// zeros, so no table can lead a read out of the cache.  Scores that all overflow
+// to -inf leave 0 / 0: NaN, as prompt attention gives.
 //
 // Bound: a token and KV head is 5/4 HD bytes, read once for all its query
 // heads, so HBM, if a value costs few instructions.  The products are
@@ -119,6 +120,10 @@ struct AqSmem {
   int abort;
   static_assert(kAqHeads * kRow * 4 <= 2 * kStages * kBlock, "a piece fits the ring");
 };
+
+// The sum of no weights: -0, which stays -0 until a token's weight is added, if only
+// +0 (of a score of -inf), and through products with factors that are not negative.
+constexpr float kNoTokens = -0.f;
 
 FRC_DEVICE_INLINE float ex2(float x) {
   float y;
@@ -291,7 +296,7 @@ struct AqWarp {
     for (int i = 0; i < 4; ++i) om[i] = 0.f;
     m_run = -INFINITY;
     base = 0.f;
-    l_run = 0.f;
+    l_run = kNoTokens;
   }
 
   // Lane (r, q) = (lane / 4, lane % 4) has tokens 4 q .. 4 q + 3 of a block.
@@ -614,7 +619,7 @@ struct AqHeads {
 
 template <int N, typename T>
 FRC_DEVICE_INLINE void aq_store(const AttnQ4Params& p, int seq, int head, int c, float (&v)[N], float l) {
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = __float_as_uint(l) == 0x80000000u ? 0.f : 1.f / l;  // kNoTokens; 0: 0 / 0
 #pragma unroll
   for (int e = 0; e < N; ++e) v[e] *= inv;
   T* op = static_cast<T*>(p.out) + seq * p.o_seq + head * p.o_head + c;
@@ -827,7 +832,7 @@ __global__ void __launch_bounds__(kAqThreads, 2) attn_q4_kernel(const AttnQ4Para
       float m[N], l[N];
       load_run<N, true>(sh->m[warp], m);
       load_run<N, true>(sh->l[warp], l);
-      float M = -INFINITY, L = 0.f, acc[C];
+      float M = -INFINITY, L = kNoTokens, acc[C];
 #pragma unroll
       for (int j = 0; j < N; ++j) M = fmaxf(M, same >> j & 1u ? m[j] : -INFINITY);
       const float base = M == -INFINITY ? 0.f : M;
@@ -875,7 +880,7 @@ __global__ void __launch_bounds__(kAqJoinWarps * 32) attn_q4_join_kernel(const A
   auto row = [&](int k) {  // the cut unit starts in CTA i (its second piece) and goes on as the others' first
     return p.part + (static_cast<int64_t>(k == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + k)) * kAqHeads + h) * ROW;
   };
-  float M = -INFINITY, L = 0.f, acc[C];  // of the warp's pieces
+  float M = -INFINITY, L = kNoTokens, acc[C];  // of the warp's pieces
 #pragma unroll
   for (int e = 0; e < C; ++e) acc[e] = 0.f;
   for (int k = warp; k < np; k += 8 * kAqJoinWarps) {  // eight pieces' loads at a time
@@ -884,7 +889,7 @@ __global__ void __launch_bounds__(kAqJoinWarps * 32) attn_q4_join_kernel(const A
     for (int j = 0; j < 8; ++j) {
       const int kj = k + j * kAqJoinWarps;
       m[j] = -INFINITY;
-      l[j] = 0.f;
+      l[j] = kNoTokens;
 #pragma unroll
       for (int e = 0; e < C; ++e) v[j][e] = 0.f;
       if (kj < np) {
@@ -922,7 +927,7 @@ __global__ void __launch_bounds__(kAqJoinWarps * 32) attn_q4_join_kernel(const A
 #pragma unroll
     for (int w = 1; w < kAqJoinWarps; ++w) M = fmaxf(M, ms[w]);
     const float base = M == -INFINITY ? 0.f : M;
-    L = 0.f;
+    L = kNoTokens;
 #pragma unroll
     for (int e = 0; e < C; ++e) acc[e] = 0.f;
 #pragma unroll
