@@ -30,7 +30,7 @@
 //  * m q: one more product, offsets (fp16 as stored) by the groups' query sums
 //    as two fp16 each.
 //  * p n: 16 channels of one group as rows, the heads as columns, 16 tokens as
-//    the contraction; p d is the fp16 operand, in two parts for fp32, rounded
+//    the contraction; p d 2^-E is the fp16 operand, in two parts for fp32, rounded
 //    once for fp16 (by 2^-11) and twice for bf16 (p and p d, an eighth of the
 //    type's own rounding each).  The fragment of p is the one that the first
 //    product leaves in the same lanes.
@@ -39,13 +39,22 @@
 //    large as the result, where sum p d n grows with the tokens and cancels
 //    with sum p m (fp32: 2e-6 off at 4097 tokens), and roundings of p d count
 //    relative to a value's distance from its group's middle.  m + 8 d is in two
-//    parts for fp32, rounded to fp16 for 16-bit types as the stored m is; where it
-//    lies beyond fp16 (values above 65504) m and d take a row each.
+//    parts for fp32, rounded to fp16 for 16-bit types as the stored m is.
 //
-// The softmax's reference is not the largest s but the largest s + log2 d (d
-// the token's largest V step, at least 2^-7): so p d stays below 2^8 whatever the
-// size of the values, p below 2^15, and both well above fp16's least for
-// steps from 2^-24 to 65504.
+// Range: the softmax's reference, the largest s, has p = 2^11 to 2^15, so p is a
+// normal fp16 number down to 2^-25 of it, and smaller ones are off by 2^-36 of it.  The
+// steps of a place have to lie within a window, 0 or 2^(E-12) to 2^E, and its |m + 8 d|
+// below 2^(E+11) and fp16's largest.  Then what p d 2^-E loses below fp16's normal
+// numbers is 2^-25 at most, against 2^11 2^-12 of the reference's smallest step: 2^-24.
+// E is 2, for values between some hundredths and some tens; where a warp's first block
+// of a unit does not fit that, four to eight times its largest step.  Blocks outside the
+// window (tokens or groups of far larger or smaller values than the rest, groups that
+// are not finite, values above 65504) are added in fp32 on the CUDA cores, whatever they
+// hold: a call of nothing else takes 213 us where ordinary values take 56 (4 sequences of
+// 32768 tokens, 32 / 8 heads of 128, bf16).  Taken from scores and steps together, as it
+// was, the reference let a token of small weight and a large step take the bits of the
+// others' weights; the check of the window costs 2 to 3 % (batch of 128 66.7 -> 68.1 us,
+// 131071 tokens 57.6 -> 59.5 us).
 //
 // Split: all sequences' tokens, 32 (two blocks) a place, for each KV head (and
 // part of eight query heads: a unit), form one line, with one empty place before
@@ -104,6 +113,14 @@ constexpr int kAqHeads = 8;                       // query heads a unit
 constexpr int kAqGrid = 2 * 148;
 constexpr int kAqMinPlaces = kAqWarps;            // places a CTA, at least: one for each warp
 
+// The window of a warp's steps (comment on top), in shared memory: halves in pairs.
+struct alignas(16) AqWindow {
+  float down;  // 2^-E
+  uint32_t hi, lo, mid;
+};
+
+constexpr AqWindow kWindow{0.25f, 0x44004400u, 0x14001400u, 0x70007000u};  // E = 2: 2^-2, 4, 2^-10, 2^13
+
 template <int HD>
 struct AqSmem {
   static constexpr int kStages = HD == 128 ? 2 : 4;  // places in flight for each warp
@@ -113,6 +130,7 @@ struct AqSmem {
   alignas(128) uint8_t ring[kAqWarps][kStages][2][kBlock];
   alignas(16) float m[kAqHeads][kPieces], l[kAqHeads][kPieces];
   int4 piece[kPieces];  // (sequence or -1, unit, start, end) in places of the CTA's range
+  AqWindow window[kAqWarps];
   uint64_t full[kAqWarps][kStages];
   int64_t scan[kAqWarps];
   int64_t first_start;  // place of sequence first_seq in the line
@@ -128,11 +146,6 @@ constexpr float kNoTokens = -0.f;
 FRC_DEVICE_INLINE float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-FRC_DEVICE_INLINE float lg2(float x) {
-  float y;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -215,12 +228,12 @@ struct AqWarp {
   static constexpr int NG = HD / kQ4Group;
   static constexpr bool SPLIT = sizeof(T) == 4;  // operands in two parts
   static constexpr bool TWICE = std::is_same<T, __nv_bfloat16>::value;  // p rounded to 11 bits before p d is
-  // p d at the reference is 2^kLift (p where d is below 2^-7 2^7 times that), and may
-  // be 2^kSlack times that: p and kUp p d stay below fp16's 65504
-  static constexpr float kLift = 4.f, kSlack = 4.f, kUp = TWICE ? 1.f : 64.f;
+  // p at the reference is 2^kLift, and may be 2^kSlack times that: below fp16's 65504
+  static constexpr float kLift = 11.f, kSlack = 4.f;
   static constexpr float kLow = 2048.f;  // of the low parts of fp32 weights and offsets
   uint32_t a[NG][2][4];  // query fragments: (group, k step): rows 0-7 of both k halves, rows 8-15 (low parts) of both
   uint32_t am;                       // groups' query sums
+  AqWindow* win;
   float f_n, f_m;                    // scale of the two score products, with log2 e
   float o[NG][2][4], om[4];
   float m_run, base, l_run;  // the reference, what is taken off the scores, the sum of p
@@ -285,7 +298,10 @@ struct AqWarp {
     am = part == 0 ? pack_half2(h0, h1) : (part == 1 ? pack_half2(s0 - h0, s1 - h1) : 0u);
   }
 
-  FRC_DEVICE_INLINE void reset() {
+  FRC_DEVICE_INLINE void reset(int lane) {
+    __syncwarp();
+    if (lane == 0) *win = kWindow;
+    __syncwarp();
 #pragma unroll
     for (int j = 0; j < NG; ++j)
 #pragma unroll
@@ -302,12 +318,12 @@ struct AqWarp {
   // Lane (r, q) = (lane / 4, lane % 4) has tokens 4 q .. 4 q + 3 of a block.
 
   // Scores of a block in shared memory, of which (TAIL) `left` tokens belong to
-  // the sequence; dx: the larger of dx and the lane's V steps.
+  // the sequence.
   template <bool TAIL>
-  FRC_DEVICE_INLINE void scores(const uint8_t* blk, int left, int lane, uint32_t bias, float (&s)[4], __half2& dx) {
+  FRC_DEVICE_INLINE void scores(const uint8_t* blk, int left, int lane, uint32_t bias, float (&s)[4]) {
     constexpr Q4Layout lay(HD);
     const int r = lane >> 2, q = lane & 3;
-    uint2 kd[NG], vd[NG];
+    uint2 kd[NG];
 #pragma unroll
     for (int j = 0; j < NG; ++j) kd[j] = *reinterpret_cast<const uint2*>(blk + lay.k_step(j, 4 * q));
 #pragma unroll
@@ -346,22 +362,11 @@ struct AqWarp {
       s[2 * t] = fmaf(x0, f_n, cm[0] * f_m);
       s[2 * t + 1] = fmaf(x1, f_n, cm[1] * f_m);
     }
-#pragma unroll
-    for (int j = 0; j < NG; ++j) vd[j] = *reinterpret_cast<const uint2*>(blk + lay.v_step(j, 4 * q));
     if constexpr (TAIL) {
-      uint32_t k0, k1;
-      own_tokens(left - 4 * q, k0, k1);
-#pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        vd[j].x &= k0;
-        vd[j].y &= k1;
-      }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (i >= left - 4 * q) s[i] = -INFINITY;
     }
-#pragma unroll
-    for (int j = 0; j < NG; ++j) dx = __hmax2(dx, __hmax2(bits_h2(vd[j].x), bits_h2(vd[j].y)));
   }
 
   // Masks of the lane's first and second pair of tokens, of which `mine` count:
@@ -371,17 +376,61 @@ struct AqWarp {
     k1 = mine >= 4 ? 0xffffffffu : (mine == 3 ? 0xffffu : 0u);
   }
 
-  // The reference raised, where it has to be, to m + d (of the lane's tokens: the
-  // largest score and the log2 of the largest V step) and the other lanes' of the
-  // head.  It may stay up to kSlack below: the operands have that room, and
-  // most raises of a running maximum are small.  True: a step is so large that
-  // m + 8 d may lie beyond fp16 (at m = 65504 a step of 2 rounds to it).
-  FRC_DEVICE_INLINE bool refer(float m, float d, int lane) {
-    m += d;
+  // The place's steps and middles m + 8 d as one lane sees them: lane (r, q) has group
+  // r % NG and tokens 4 q .. 4 q + 3 of block r / NG, where bit r / NG of `present` is set.
+  struct Extent {
+    __half2 top, mid;  // largest step, largest |m + 8 d|: NaN if one is
+    __half2 d0, d1;
+  };
+  static FRC_DEVICE_INLINE Extent extent(const uint8_t (*blk)[20 * HD], uint32_t present, int left, int lane) {
+    constexpr Q4Layout lay(HD);
+    const int r = lane >> 2, q = lane & 3, e = r / NG, j = r % NG;
+    uint2 m = make_uint2(0u, 0u), d = m;
+    if (present >> e & 1u) {
+      m = *reinterpret_cast<const uint2*>(blk[e] + lay.v_offset(j, 4 * q));
+      d = *reinterpret_cast<const uint2*>(blk[e] + lay.v_step(j, 4 * q));
+      if (left < 2 * kQ4Tokens) {
+        uint32_t k0, k1;
+        own_tokens(left - e * kQ4Tokens - 4 * q, k0, k1);
+        m.x &= k0;
+        d.x &= k0;
+        m.y &= k1;
+        d.y &= k1;
+      }
+    }
+    const __half2 eight = __float2half2_rn(8.f), d0 = bits_h2(d.x), d1 = bits_h2(d.y);
+    return {__hmax2_nan(d0, d1),
+            __hmax2_nan(__habs2(__hfma2(d0, eight, bits_h2(m.x))), __habs2(__hfma2(d1, eight, bits_h2(m.y)))), d0, d1};
+  }
+  static FRC_DEVICE_INLINE bool fits(const Extent& x, const AqWindow& w) {
+    const __half2 lo = bits_h2(w.lo);
+    // steps below the window, but for zeros
+    const __half2 small = __hfma2(__hlt2(x.d0, lo), x.d0, __hmul2(__hlt2(x.d1, lo), x.d1));
+    return __hble2(x.top, bits_h2(w.hi)) && __hble2(x.mid, bits_h2(w.mid)) && __hbeq2(small, bits_h2(0u));
+  }
+  // The window chosen for a block's steps: true if they fit then (if not, it stays as it was).
+  FRC_DEVICE_INLINE bool adopt(const Extent& x, int lane) {
+    const float mine = fmaxf(__low2float(x.top), __high2float(x.top));  // (NaN, or below 0: does not fit)
+    const uint32_t top = __reduce_max_sync(0xffffffffu, mine > 0.f ? __float_as_uint(mine) : 0u);
+    const int e = min(max(static_cast<int>(top >> 23) - 127 + 3, -12), 16);
+    auto power = [](int n) { return __uint_as_float(static_cast<uint32_t>(127 + n) << 23); };
+    auto both = [](float v) { return h2_bits(__float2half2_rn(fminf(v, 65504.f))); };
+    const AqWindow w{power(-e), both(power(e)), both(power(e - 12)), both(power(e + 11))};
+    const bool fit = __all_sync(0xffffffffu, fits(x, w));
+    if (fit && lane == 0) *win = w;
+    __syncwarp();
+    return fit;
+  }
+
+  // The reference raised, where it has to be, to m (the largest score of the lane's
+  // tokens) and the other lanes' of the head.  It may stay up to kSlack below: the
+  // operands have that room, and most raises of a running maximum are small.  True: the
+  // place does not fit the window.
+  FRC_DEVICE_INLINE bool refer(float m, bool fit, int lane) {
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    const bool up = m > m_run + kSlack, wide = d >= 1.f;
-    if (!__any_sync(0xffffffffu, up || wide)) return false;
+    const bool up = m > m_run + kSlack;
+    if (!__any_sync(0xffffffffu, up || !fit)) return false;
     if (__any_sync(0xffffffffu, up)) {
       const int q = lane & 3;
       const float m_new = fmaxf(m, m_run);
@@ -402,11 +451,10 @@ struct AqWarp {
       m_run = m_new;
       base = m_new == -INFINITY ? 0.f : m_new - kLift;
     }
-    return __any_sync(0xffffffffu, wide);
+    return !__all_sync(0xffffffffu, fit);
   }
 
-  // The block's values, weighted by its scores; not TAIL: no sum m + 8 d lies
-  // beyond fp16.
+  // The block's values, weighted by its scores: a block that fits the window.
   template <bool TAIL>
   FRC_DEVICE_INLINE void values(const uint8_t* blk, int left, int lane, uint32_t bias, const float (&s)[4]) {
     constexpr Q4Layout lay(HD);
@@ -447,30 +495,7 @@ struct AqWarp {
       l01 = pack_half2((p0 - g01.x) * kLow, (p1 - g01.y) * kLow);
       l23 = pack_half2((p2 - g23.x) * kLow, (p3 - g23.y) * kLow);
     }
-    bool apart = false;
-    if constexpr (TAIL) apart = beyond(bits_h2(vm.x), bits_h2(vm.y));
-    if (apart) {  // a sum m + 8 d beyond fp16 (values above 65504): m and d as rows of their own
-      uint2 m = make_uint2(0u, 0u), d = m;
-      if (r < NG) {
-        uint32_t k0, k1;
-        own_tokens(left - 4 * q, k0, k1);
-        m = *reinterpret_cast<const uint2*>(blk + lay.v_offset(r, 4 * q));
-        d = *reinterpret_cast<const uint2*>(blk + lay.v_step(r, 4 * q));
-        m.x &= k0;
-        m.y &= k1;
-        d.x &= k0;
-        d.y &= k1;
-      }
-      float c[4];
-      if constexpr (SPLIT) {
-        mma16816_new(c, m.x, d.x, m.y, d.y, l01, l23);
-        om[0] += fmaf(c[2], 8.f, c[0]) * (1.f / kLow);
-        om[1] += fmaf(c[3], 8.f, c[1]) * (1.f / kLow);
-      }
-      mma16816_new(c, m.x, d.x, m.y, d.y, h01, h23);
-      om[0] += fmaf(c[2], 8.f, c[0]);
-      om[1] += fmaf(c[3], 8.f, c[1]);
-    } else if constexpr (SPLIT) {
+    if constexpr (SPLIT) {
       float c[4], low[4];
       mma16816_new(low, vm.x, 0u, vm.y, 0u, l01, l23);
       mma16816(low, vml.x, 0u, vml.y, 0u, h01, h23);
@@ -483,15 +508,17 @@ struct AqWarp {
     // rows of a tile: 16 channels of group j: word 4 j + r % 4, of it the nibbles
     // of its low half (r < 4) or high half: 2 t in row r, 2 t + 1 in row r + 8
     const uint32_t sel = r < 4 ? 0x5410u : 0x7632u;
-    const uint64_t r01 = f32x2_two(p0 * kUp, p1 * kUp), r23 = f32x2_two(p2 * kUp, p3 * kUp);
+    const float down = win->down;
+    const uint64_t r01 = f32x2_two(p0 * down, p1 * down), r23 = f32x2_two(p2 * down, p3 * down);
+    const __half2 down2 = __float2half2_rn(down);  // (a step in the window times it is exact)
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
       const uint4 v = *reinterpret_cast<const uint4*>(blk + lay.v_word(4 * j + (r & 3), 4 * q));
       const uint32_t w0 = __byte_perm(v.x, v.y, sel), w1 = __byte_perm(v.z, v.w, sel);
       uint32_t b0, b1, c0 = 0u, c1 = 0u;
       if constexpr (TWICE) {
-        b0 = h2_bits(__hmul2(bits_h2(h01), bits_h2(vd[j].x)));
-        b1 = h2_bits(__hmul2(bits_h2(h23), bits_h2(vd[j].y)));
+        b0 = h2_bits(__hmul2(bits_h2(h01), __hmul2(bits_h2(vd[j].x), down2)));
+        b1 = h2_bits(__hmul2(bits_h2(h23), __hmul2(bits_h2(vd[j].y), down2)));
       } else {
         const float2 e0 = __half22float2(bits_h2(vd[j].x)), e1 = __half22float2(bits_h2(vd[j].y));
         float y0, y1, y2, y3;
@@ -525,40 +552,49 @@ struct AqWarp {
     }
   }
 
-  // Whether one of a whole block's sums m + 8 d lies beyond fp16.
-  static FRC_DEVICE_INLINE bool beyond(const uint8_t* blk, int lane) {
+  // The same for any block, in fp32: `left` tokens of it, each lane its channels of its
+  // two heads.
+  FRC_DEVICE_INLINE void values_apart(const uint8_t* blk, int left, int lane, const float (&s)[4]) {
     constexpr Q4Layout lay(HD);
     const int r = lane >> 2, q = lane & 3;
-    uint2 m = make_uint2(0u, 0u), d = m;
-    if (r < NG) {
-      m = *reinterpret_cast<const uint2*>(blk + lay.v_offset(r, 4 * q));
-      d = *reinterpret_cast<const uint2*>(blk + lay.v_step(r, 4 * q));
+    const float p0 = ex2(s[0] - base), p1 = ex2(s[1] - base), p2 = ex2(s[2] - base), p3 = ex2(s[3] - base);
+    l_run += (p0 + p1) + (p2 + p3);
+    const float down = win->down;
+#pragma unroll 1
+    for (int tok = 0; tok < min(left, kQ4Tokens); ++tok) {
+      const int i = tok & 3;
+      const float mine = (i & 2 ? (i & 1 ? p3 : p2) : (i & 1 ? p1 : p0)) * down;
+      const float f0 = __shfl_sync(0xffffffffu, mine, 8 * q + (tok >> 2));
+      const float f1 = __shfl_sync(0xffffffffu, mine, 8 * q + 4 + (tok >> 2));
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        const uint32_t w = *reinterpret_cast<const uint16_t*>(blk + lay.v_word(4 * j + (r & 3), tok) + 2 * (r >> 2));
+        const float d = __half2float(*reinterpret_cast<const __half*>(blk + lay.v_step(j, tok)));
+        const float m = __half2float(*reinterpret_cast<const __half*>(blk + lay.v_offset(j, tok)));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float v = fmaf(static_cast<float>(w >> (4 * k) & 15u), d, m);
+          float* at = &o[j][k >> 1][2 * (k & 1)];
+          at[0] = fmaf(f0, v, at[0]);
+          at[1] = fmaf(f1, v, at[1]);
+        }
+      }
     }
-    const __half2 eight = __float2half2_rn(8.f);
-    return beyond(__hfma2(bits_h2(d.x), eight, bits_h2(m.x)), __hfma2(bits_h2(d.y), eight, bits_h2(m.y)));
-  }
-  static FRC_DEVICE_INLINE bool beyond(__half2 a, __half2 b) {
-    return __any_sync(0xffffffffu, !__hblt2(__hmax2(__habs2(a), __habs2(b)), bits_h2(0x7c007c00u)));
   }
 
-  // What the reference has to cover of a lane's scores: the largest s + log2
-  // of the largest V step of its tokens, taken apart: no less than the largest
-  // s + log2 d.
   static FRC_DEVICE_INLINE float largest(const float (&s)[4], float m) {
     return fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), m);
   }
-  static FRC_DEVICE_INLINE float log2_of(__half2 dx) { return lg2(__half2float(__hmax(__low2half(dx), __high2half(dx)))); }
 
   // The blocks of a place (bit e of `seen`: block e is there), of which `left`
   // tokens belong to the sequence.
   FRC_DEVICE_INLINE void place(const uint8_t (*blk)[20 * HD], uint32_t seen, int left, int lane, uint32_t bias) {
-    const __half2 least = __float2half2_rn(1.f / 128.f);
     if (left >= 2 * kQ4Tokens && seen == 3u) {
       float s0[4], s1[4];
-      __half2 dx = least;
-      scores<false>(blk[0], 0, lane, bias, s0, dx);
-      scores<false>(blk[1], 0, lane, bias, s1, dx);
-      if (!refer(largest(s0, largest(s1, -INFINITY)), log2_of(dx), lane) || !(beyond(blk[0], lane) || beyond(blk[1], lane))) {
+      scores<false>(blk[0], 0, lane, bias, s0);
+      scores<false>(blk[1], 0, lane, bias, s1);
+      const bool fit = fits(extent(blk, 3u, 2 * kQ4Tokens, lane), *win);
+      if (!refer(largest(s0, largest(s1, -INFINITY)), fit, lane) ) {
         values<false>(blk[0], 0, lane, bias, s0);
         values<false>(blk[1], 0, lane, bias, s1);
         return;
@@ -568,10 +604,14 @@ struct AqWarp {
     for (int e = 0; e < 2; ++e) {
       if (!(seen >> e & 1u)) continue;
       float s[4];
-      __half2 dx = least;
-      scores<true>(blk[e], left - e * kQ4Tokens, lane, bias, s, dx);
-      refer(largest(s, -INFINITY), log2_of(dx), lane);
-      values<true>(blk[e], left - e * kQ4Tokens, lane, bias, s);
+      scores<true>(blk[e], left - e * kQ4Tokens, lane, bias, s);
+      const Extent x = extent(blk, 1u << e, left, lane);
+      bool fit = __all_sync(0xffffffffu, fits(x, *win));
+      if (!fit && __float_as_uint(l_run) == 0x80000000u) fit = adopt(x, lane);  // (no token yet)
+      if (!refer(largest(s, -INFINITY), fit, lane) )
+        values<true>(blk[e], left - e * kQ4Tokens, lane, bias, s);
+      else
+        values_apart(blk[e], left - e * kQ4Tokens, lane, s);
     }
   }
 
@@ -592,15 +632,15 @@ struct AqWarp {
     const int r = lane >> 2, q = lane & 3;
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
-    constexpr float kStep = 1.f / kUp;
+    const float up = __uint_as_float((254u << 23) - __float_as_uint(win->down));  // 1 / 2^-E
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const float l = __shfl_sync(0xffffffffu, l_run, 4 * (2 * q + e));
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
         const float m = __shfl_sync(0xffffffffu, om[e], 4 * j + q);
-        const float v[4] = {fmaf(o[j][0][e], kStep, m), fmaf(o[j][0][2 + e], kStep, m), fmaf(o[j][1][e], kStep, m),
-                            fmaf(o[j][1][2 + e], kStep, m)};
+        const float v[4] = {fmaf(o[j][0][e], up, m), fmaf(o[j][0][2 + e], up, m), fmaf(o[j][1][e], up, m),
+                            fmaf(o[j][1][2 + e], up, m)};
         f(2 * q + e, kQ4Group * j + 8 * (r & 3) + 4 * (r >> 2), v, l);
       }
     }
@@ -744,6 +784,7 @@ __global__ void __launch_bounds__(kAqThreads, 2) attn_q4_kernel(const AttnQ4Para
     uint32_t parity = 0;
 
     AqWarp<HD, T> st;
+    st.win = &sh->window[warp];
     for (int place = w0; place < w1;) {
       walk.to(p, place, units);
       const AqHeads heads(p, walk.unit);
@@ -763,7 +804,7 @@ __global__ void __launch_bounds__(kAqThreads, 2) attn_q4_kernel(const AttnQ4Para
         }
         st.load_q(x, p.scale, lane);
       }
-      st.reset();
+      st.reset(lane);
       for (; place < end; ++place) {
         bool there = __all_sync(0xffffffffu, mbar_try_wait(&sh->full[warp][s], parity));
         if (!there) there = __all_sync(0xffffffffu, wait_phase(&sh->full[warp][s], parity, abort));
