@@ -75,6 +75,30 @@ def rope_tables(head_dim: int, theta: float, max_pos: int) -> tuple[np.ndarray, 
     return np.cos(freqs).astype(np.float32), np.sin(freqs).astype(np.float32)
 
 
+def _half_operands(q, k, v):
+    """q, the parts of k and the parts of v (fp32, (tokens, heads, head_dim)) as fp16 operands
+    of prompt attention: (q, k, v, up), the result being `up` times what they give.
+
+    Where something lies beyond 2^15 it is taken down by a power of two; v's is `up`, and
+    q and k take over each other's as far as they stay below 2^15 themselves, so that the
+    scores are the same.  (Where both are that large the scores come down with them: by less
+    than what their fp16 roundings leave open, which stays far above one.)  Decided on the
+    device: the factors are 1 for what fp16 holds."""
+    import torch
+
+    def beyond(parts):  # exponent of the largest, and how far it is above 15
+        top = torch.stack([torch.linalg.vector_norm(x, float("inf")) if x.numel() else x.new_zeros(()) for x in parts]).amax()
+        e = torch.frexp(top)[1].float()
+        e = torch.where(torch.isfinite(top), e, torch.zeros_like(e))
+        return e, (e - 15).clamp(min=0)
+
+    (eq, a), (ek, b), (_, c) = beyond([q]), beyond(k), beyond(v)
+    fq = torch.exp2(torch.minimum(b, 15 - eq.clamp(max=15)) - a)
+    fk = torch.exp2(torch.minimum(a, 15 - ek.clamp(max=15)) - b)
+    k, v = (torch.cat([(x * f).half() for x in parts]) for parts, f in ((k, fk), (v, torch.exp2(-c))))
+    return (q * fq).half(), k, v, torch.exp2(c)
+
+
 class DecodeEngine:
     """Greedy decode of one sequence with every weight and the KV cache in HBM.
 
@@ -323,7 +347,8 @@ class DecodeEngine:
         """Feed a prompt at once, behind what the cache holds: afterwards `logits`
         and `argmax_host()` are those of its last token, and `step()` goes on.
         The projections run batched (above 16 tokens with fp16 operands, as
-        frc_gemv's), the attention on fp16 queries, keys and values;
+        frc_gemv's), the attention on fp16 queries, keys and values (scaled
+        by powers of two where they lie beyond fp16's range);
         asynchronous on the engine's stream."""
         from . import attention
 
@@ -370,16 +395,17 @@ class DecodeEngine:
                 q, k, v = attention.qk_norm_rope(qkv, c.heads, c.kv_heads, self._cos, self._sin, pos,
                                                  bias=self._bias.get(i), out=parts)
                 self._store(i, start, k, v)
-                k, v = k.half(), v.half()
+                k, v = [k], [v]
                 if start:
                     if self.kv_bits == 4:
                         slots = torch.arange(start, dtype=torch.int64, device=self._dev)
-                        past = attention.kv_read_q4(self.q4_cache[i], slots, dtype=torch.float16)
+                        past = attention.kv_read_q4(self.q4_cache[i], slots)
                     else:
-                        past = (self.k_cache[i][:start].half(), self.v_cache[i][:start].half())
-                    k, v = (torch.cat(t) for t in zip(past, (k, v)))
-                ctx = attention.attention_prefill(q.half(), k, v, cu_q, cu_k, scale=float(np.float32(1.0 / np.sqrt(hd))))
-                h += project(f"{p}.self_attn.o_proj.weight", ctx.reshape(n, c.hidden).float())
+                        past = (self.k_cache[i][:start], self.v_cache[i][:start])
+                    k, v = ([x] + y for x, y in zip(past, (k, v)))
+                q, k, v, up = _half_operands(q, k, v)
+                ctx = attention.attention_prefill(q, k, v, cu_q, cu_k, scale=float(np.float32(1.0 / np.sqrt(hd))))
+                h += project(f"{p}.self_attn.o_proj.weight", ctx.reshape(n, c.hidden).float().mul_(up))
                 x = norm(h, self._norm[f"{p}.post_attention_layernorm.weight"])
                 gate = torch.nn.functional.silu(project(f"{p}.mlp.gate_proj.weight", x))
                 h += project(f"{p}.mlp.down_proj.weight", gate * project(f"{p}.mlp.up_proj.weight", x))

@@ -36,3 +36,45 @@ def test_no_token_behind_max_pos():
     assert eng.launched == 2
     with pytest.raises(ValueError, match="max_pos"):
         _stand_in(max_pos=5, filled=3).prefill([1, 2, 3])
+
+
+@pytest.mark.parametrize("sizes", [(1.0, 1.0, 1.0), (3e4, 3e4, 6.5e4), (1.0, 1e6, 1.0), (1e5, 2.0, 3e9), (4e-3, 7e5, 1e-6),
+                                   (1e5, 1e5, 1.0), (1e9, 1e9, 1e30), (2e4, 1e6, 0.0)])
+@pytest.mark.parametrize("past", [0, 3])
+def test_half_operands(sizes, past):
+    """Nothing finite becomes infinite; scores and values are those of the fp32 operands to fp16's rounding of their
+    sizes (three of 2^-11: two operands and their product's), except that scores come down by a power of two where
+    queries and keys are both beyond 2^15; operands that fp16 holds are converted as they are."""
+    from flatrun_b200.decode import _half_operands
+
+    g = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(5 + n, 2, 8, generator=g).clamp(-3, 3) / 3 * s for s, n in zip(sizes, (0, past, past)))
+    k, v = ([x[:past], x[past:]] if past else [x] for x in (k, v))
+    hq, hk, hv, up = _half_operands(q, k, v)
+    k, v = torch.cat(k), torch.cat(v)
+    assert all(x.dtype == torch.float16 and bool(torch.isfinite(x).all()) for x in (hq, hk, hv))
+    assert hk.shape == k.shape and hv.shape == v.shape
+    got, ref = (torch.einsum("thc,shc->tsh", x.double(), y.double()) for x, y in ((hq, hk), (q, k)))
+    size = torch.einsum("thc,shc->tsh", q.double().abs(), k.double().abs())
+    if max(sizes[0], sizes[1]) / 32768 * min(sizes[0], sizes[1]) > 32768:
+        down = (ref / got).median().log2().round().exp2()
+        assert down > 1
+        got = got * down
+    # (below 2^-14 fp16's steps are 2^-24: relative to the largest, at least 2^-24 / 2^-14)
+    assert bool(((got - ref).abs() <= 3 * 2.0 ** -11 * size + 2.0 ** -10 * size.max() * 2.0 ** -10).all())
+    assert bool(((hv.double() * up.double() - v.double()).abs() <= 2.0 ** -11 * v.double().abs() +
+                 2.0 ** -25 * max(1.0, up)).all())
+    if max(sizes) < 32768:
+        assert up == 1 and torch.equal(hq, q.half()) and torch.equal(hk, k.half()) and torch.equal(hv, v.half())
+
+
+def test_half_operands_not_finite():
+    """An infinity or a NaN stays one, and changes nothing beside it."""
+    from flatrun_b200.decode import _half_operands
+
+    for bad in (float("inf"), float("nan")):
+        q, k, v = (torch.ones(4, 1, 8) for _ in range(3))
+        v[1, 0, 3] = bad
+        hq, hk, hv, up = _half_operands(q, [k], [v])
+        assert up == 1 and torch.equal(hq, q.half()) and torch.equal(hk, k.half())
+        assert torch.equal(hv.isfinite(), v.isfinite()) and bool((hv[v.isfinite()] == 1).all())

@@ -35,3 +35,40 @@ def test_the_last_position_is_used_and_none_behind_it(bits):
     kv = {0: (np.zeros((22, Q.TINY.NKV, 64), np.float32),) * 2}
     with pytest.raises(ValueError, match="max_pos"):
         _engine(max_pos=21, kv_bits=bits, kv_page=16, kv_prefill=kv)
+
+
+def _large_past(kv_bits):
+    """A layer behind 10 cached positions whose values are around 3e5 and whose keys are 1e6 in two channels that no query
+    has (both beyond fp16).  Queries are the biases alone, 0.02, so that scores are of size one."""
+    from dataclasses import replace
+
+    spec = replace(Q.TINY, L=1)
+    w = Q.build(spec)
+    p, hd = "model.layers.0.self_attn", spec.H // spec.NH
+    w[f"{p}.q_proj.weight"] = np.zeros_like(w[f"{p}.q_proj.weight"])
+    rng = np.random.default_rng(8)
+    bias = (0.02 * rng.standard_normal((spec.NH, hd))).astype(np.float32)
+    bias[:, [31, 63]] = 0.0
+    w[f"{p}.q_proj.bias"] = bias.reshape(-1)
+    for m in ("k", "v"):
+        w[f"{p}.{m}_proj.bias"] = np.zeros(spec.NKV * hd, np.float32)
+    k, v = (rng.standard_normal((10, spec.NKV, hd)).astype(np.float32) for _ in range(2))
+    k[:, :, 31], k[:, :, 63] = 1e6, -1e6
+    v = (3e5 + 1e5 * v).astype(np.float32)
+    return _engine(spec=spec, weights=w, kv_bits=kv_bits, kv_page=16, kv_prefill={0: (k, v)})
+
+
+@pytest.mark.parametrize("bits", [32, 4])
+def test_prefill_behind_values_beyond_fp16(bits):
+    """A prompt at once gives what its tokens give one by one.  fp16 roundings between the two: of queries, keys, weights,
+    values, the attention's result, and two operands of each batched product, 2^-11 each: below 16 * 2^-11 of the logits'
+    size.  (In 4 bits the prompt's own keys differ too, exact in one and quantised in the other: finite is all that is asked.)"""
+    tokens = np.random.default_rng(3).integers(0, 320, 20)
+    one, eng = _large_past(bits), _large_past(bits)
+    for t in tokens:
+        one.step(int(t))
+    eng.prefill(tokens)
+    ref, got = one.logits_host(), eng.logits_host()
+    assert np.isfinite(ref).all() and np.isfinite(got).all()
+    if bits == 32:
+        assert np.abs(got - ref).max() <= 2.0 ** -7 * np.abs(ref).max()
