@@ -307,13 +307,14 @@ class DecodeEngine:
         return ctypes.c_void_p(self.stream.cuda_stream)
 
     def capture(self) -> None:
-        """Record one token as a CUDA graph (replayed by step())."""
+        """Record one token as a CUDA graph (replayed by step()).  The position,
+        the last token's logits and its pick stay as they are."""
         torch = self.torch
         self._room(1)  # the eager token below writes its cache row
         with torch.cuda.stream(self.stream):
             # one eager token first: lazy module loading and launch
             # configuration happen outside the capture; then undo its effects
-            state = [self.pos, self.tok_in] + ([self._slot, self._length] if self.kv_bits == 4 else [])
+            state = [self.pos, self.tok_in, self.tok_out, self.h, self.logits] + ([self._slot, self._length] if self.kv_bits == 4 else [])
             before = [t.clone() for t in state]
             self._token()
             self.stream.synchronize()

@@ -72,3 +72,20 @@ def test_prefill_behind_values_beyond_fp16(bits):
     assert np.isfinite(ref).all() and np.isfinite(got).all()
     if bits == 32:
         assert np.abs(got - ref).max() <= 2.0 ** -7 * np.abs(ref).max()
+
+
+@pytest.mark.parametrize("bits", [32, 4])
+def test_capture_keeps_the_last_token(bits):
+    """prefill, then capture: logits and pick are the prompt's still, and the pick goes in next, as without a capture."""
+    tokens = np.random.default_rng(4).integers(0, 320, 23)
+    plain, eng = _engine(kv_bits=bits), _engine(kv_bits=bits)
+    for e in (plain, eng):
+        e.prefill(tokens)
+    logits, pick = eng.logits_host().copy(), eng.argmax_host()
+    eng.capture()
+    assert np.array_equal(eng.logits_host(), logits) and eng.argmax_host() == pick
+    assert int(eng.pos.item()) == 23
+    for _ in range(3):
+        for e in (plain, eng):
+            e.step()
+        assert np.array_equal(eng.logits_host(), plain.logits_host()) and eng.argmax_host() == plain.argmax_host()
