@@ -357,6 +357,8 @@ class DecodeEngine:
         ids = np.asarray(tokens, np.int32).reshape(-1)
         n, hd = ids.size, c.head_dim
         kvd = c.kv_heads * hd
+        if hd not in (64, 128):
+            raise ValueError(f"prompt attention needs a head_dim of 64 or 128, not {hd}")
         if n == 0:
             raise ValueError("an empty prompt")
         if ids.min() < 0 or ids.max() >= c.vocab:

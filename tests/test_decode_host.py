@@ -78,3 +78,10 @@ def test_half_operands_not_finite():
         hq, hk, hv, up = _half_operands(q, [k], [v])
         assert up == 1 and torch.equal(hq, q.half()) and torch.equal(hk, k.half())
         assert torch.equal(hv.isfinite(), v.isfinite()) and bool((hv[v.isfinite()] == 1).all())
+
+
+def test_prefill_refuses_a_head_dim_before_anything_is_written():
+    eng = _stand_in(max_pos=5, filled=0)
+    eng.cfg = DecoderConfig(80, 64, 16, 1, 1, 1, 1e-6, 1e4, 5)
+    with pytest.raises(ValueError, match="head_dim"):
+        eng.prefill([1, 2])
