@@ -331,6 +331,13 @@ def _decode_q4_workspace(batch: int, nh: int, nkv: int, hd: int) -> int:
     return _workspace_bytes[hd]
 
 
+def _decode_q4_kernels(batch: int, nh: int, nkv: int, room: int) -> int:
+    """Kernels that attention_decode_q4 launches for tables of `room` tokens: the second joins what several CTAs have
+    of a head, and a CTA takes eight places (of 32 tokens, and one more a sequence, KV head and eight query heads)."""
+    units = batch * nkv * -(-nh // nkv // 8)
+    return 1 if batch == 0 or units * (-(-room // 32) + 1) <= 8 else 2
+
+
 def attention_decode_q4(q, cache, block_table, lengths, *, scale: float | None = None, out=None):
     """Attention of one query token a sequence over the 4-bit cache.
 

@@ -167,6 +167,7 @@ class DecodeEngine:
             pages = -(-c.max_pos // kv_page)
             self.q4_cache = [attention.kv_cache_q4(pages, kv_page, c.kv_heads, hd, self._dev) for _ in range(c.layers)]
             self._table = torch.arange(pages, dtype=torch.int32, device=self._dev).reshape(1, -1)
+            self._q4_joins = attention._decode_q4_kernels(1, c.heads, c.kv_heads, pages * kv_page) - 1
         else:
             self.k_cache, self.v_cache = (
                 [torch.zeros((c.max_pos, c.kv_heads, hd), dtype=f32, device=self._dev) for _ in range(c.layers)]
@@ -254,7 +255,7 @@ class DecodeEngine:
         self._attn.kv_append_q4(cache, k, v, self._slot)
         self._attn.attention_decode_q4(q, cache, self._table, self._length, scale=float(np.float32(1.0 / np.sqrt(hd))),
                                        out=self.ctx.view(1, c.heads, hd))
-        self.launches_per_token += 4
+        self.launches_per_token += 3 + self._q4_joins
 
     def _token(self) -> None:
         """Enqueue one decode token (the graph body)."""
@@ -413,7 +414,9 @@ class DecodeEngine:
                 gate = torch.nn.functional.silu(project(f"{p}.mlp.gate_proj.weight", x))
                 h += project(f"{p}.mlp.down_proj.weight", gate * project(f"{p}.mlp.up_proj.weight", x))
             self.h.copy_(h[-1])
+            launches = self.launches_per_token  # a token's, which the prompt is not
             self._gemv(["lm_head.weight"], self.h, [self.logits], norm=self._norm["model.norm.weight"])
+            self.launches_per_token = launches
             _lib.check(lib.frc_argmax(self.logits.data_ptr(), c.vocab, self.tok_out.data_ptr(), self.argmax_ws.data_ptr(),
                                       self._st), lib)
             self.tok_in.copy_(self.tok_out)

@@ -89,3 +89,18 @@ def test_capture_keeps_the_last_token(bits):
         for e in (plain, eng):
             e.step()
         assert np.array_equal(eng.logits_host(), plain.logits_host()) and eng.argmax_host() == plain.argmax_host()
+
+
+def test_launches_of_a_token():
+    """The count of a token's kernels stays through a prompt; a layer whose attention needs no join has one less (2 KV heads,
+    each 3 places of 32 tokens and one: 8, which are a CTA's; with a fourth place 10)."""
+    counts = []
+    for max_pos in (96, 97):
+        eng = _engine(max_pos=max_pos, kv_bits=4, kv_page=16)
+        eng.capture()
+        counts.append(eng.launches_per_token)
+        eng.prefill(np.arange(20))
+        assert eng.launches_per_token == counts[-1]
+        eng.step()
+        assert eng.launches_per_token == counts[-1]
+    assert counts[1] - counts[0] == Q.TINY.L
