@@ -22,7 +22,8 @@ returns without waiting; positions, slots, tables and lengths are read on the
 device, so calls can be captured in a CUDA graph and replayed with new ones
 (pass ``out=`` to keep the results in place).  Arguments that do not fit raise
 ValueError before anything is launched.  Inference only: tensors that require
-gradients are refused while gradients are recorded.
+gradients, outputs among them, are refused while gradients are recorded, and so are
+tensors with forward-mode tangents.
 """
 
 from __future__ import annotations
@@ -33,6 +34,7 @@ import struct
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -89,6 +91,8 @@ def _no_grad(*tensors) -> None:
     for t in tensors:
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError("the operator has no backward pass: call it under torch.no_grad()")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError("the operator has no forward-mode derivative: its results would have no tangents")
 
 
 def _index(t: torch.Tensor, name: str, dtype: torch.dtype, shape) -> None:
@@ -219,6 +223,7 @@ def qk_norm_rope(qkv, heads: int, kv_heads: int, cos, sin, positions, *, bias=No
     if dtype not in _TYPE or (out_dtype is not None and out_dtype != dtype):
         raise ValueError("out has another type than out_dtype, or not fp32, fp16 or bf16")
     shape = (tokens, kv_heads, hd)
+    _no_grad(q, k, v)
     q_row = _packed(q, "out q", (tokens, heads, hd), dtype)
     k_row = _packed(k, "out k", shape, dtype)
     v_row = _packed(v, "out v", shape, dtype)
@@ -310,6 +315,7 @@ def kv_read_q4(cache, slots, *, dtype=None, out=None):
     if len(out) != 2 or out[0].dtype not in _TYPE or dtype not in (None, out[0].dtype):
         raise ValueError("out must be (k, v) in fp32, fp16 or bf16, of the type asked for")
     k, v = out
+    _no_grad(k, v)
     k_row, k_head = _rows(k, "out k", shape, k.dtype)
     v_row, v_head = _rows(v, "out v", shape, k.dtype)
     if tokens and (min(k_row, v_row) <= 0 < tokens - 1 or min(k_head, v_head) <= 0 < nkv - 1):
@@ -368,7 +374,7 @@ def attention_decode_q4(q, cache, block_table, lengths, *, scale: float | None =
     o_seq, o_head = _rows(out, "out", shape, q.dtype)
     if batch and (o_seq <= 0 < batch - 1 or o_head <= 0 < nh - 1):
         raise ValueError("the rows or heads of out overlap")
-    _no_grad(q)
+    _no_grad(q, out)
     device = _device(q, cache, block_table, lengths, out)
     nbytes = _decode_q4_workspace(batch, nh, nkv, hd)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
@@ -422,7 +428,7 @@ def attention_prefill(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: f
         raise ValueError("the rows or heads of out overlap")
     if at[3] in at[:3] and tokens:
         raise ValueError("out must not be q, k or v: they are read while its rows are written")
-    _no_grad(q, k, v)
+    _no_grad(q, k, v, out)
     _launch(_device(q, k, v, cu_q, cu_k, out), _PREFILL, _TYPE[dtype], at[0], q_row, q_head, at[1], k_row, k_head,
             at[2], v_row, v_head, cu_q.data_ptr(), cu_k.data_ptr(), cu_q.shape[0] - 1, tokens, tokens_k, nh, nkv, hd,
             hd ** -0.5 if scale is None else scale, 1 if causal else 0, at[3], o_row, o_head)

@@ -207,3 +207,44 @@ def test_oracle_of_the_cache_round_trips():
                 bound = np.repeat(d, 32, -1) * (0.5 + 15 * 2.0 ** -11) + np.abs(x).max() * 2.0 ** -11
                 assert np.all(np.abs(x - y) <= bound)
         assert np.isnan(kk[40, 1, 32:64]).all() and np.isfinite(kk[40, 1, :32]).all() and np.isfinite(vv[40]).all()
+
+
+def _calls():
+    """Each operator with CPU tensors: (name of each floating tensor, the call with some of them replaced)."""
+    half = torch.float16
+    cache = A.kv_cache_q4(2, 32, 2, 64, device="cpu")
+    slots, n = torch.zeros(5, dtype=torch.int64), torch.zeros(3, dtype=torch.int32)
+    rows = {"k": torch.zeros(5, 2, 64), "v": torch.zeros(5, 2, 64)}
+    rope = {"qkv": torch.zeros(3, 512), "cos": torch.zeros(9, 32), "sin": torch.zeros(9, 32), "bias": torch.zeros(512),
+            "q": torch.zeros(3, 4, 64), "k": torch.zeros(3, 2, 64), "v": torch.zeros(3, 2, 64)}
+    decode = {"q": torch.zeros(3, 4, 64), "out": torch.zeros(3, 4, 64)}
+    prefill = {"q": torch.zeros(5, 4, 64, dtype=half), "k": torch.zeros(5, 2, 64, dtype=half),
+               "v": torch.zeros(5, 2, 64, dtype=half), "out": torch.zeros(5, 4, 64, dtype=half)}
+    cu = torch.tensor([0, 5], dtype=torch.int32)
+    return [
+        (rope, lambda a: A.qk_norm_rope(a["qkv"], 4, 2, a["cos"], a["sin"], n, bias=a["bias"], out=(a["q"], a["k"], a["v"]))),
+        (rows, lambda a: A.kv_append_q4(cache, a["k"], a["v"], slots)),
+        (rows, lambda a: A.kv_read_q4(cache, slots, out=(a["k"], a["v"]))),
+        (decode, lambda a: A.attention_decode_q4(a["q"], cache, n[:, None], n, out=a["out"])),
+        (prefill, lambda a: A.attention_prefill(a["q"], a["k"], a["v"], cu, out=a["out"])),
+    ]
+
+
+@pytest.mark.parametrize("operator", range(5))
+def test_derivatives_of_either_mode_are_refused(operator):
+    """Inputs and outputs that require gradients, and inputs and outputs with tangents; without either the call gets as
+    far as the device."""
+    from torch.autograd import forward_ad
+
+    tensors, call = _calls()[operator]
+    with pytest.raises(ValueError, match="CUDA device"):
+        call(tensors)
+    for name, t in tensors.items():
+        with pytest.raises(ValueError, match="no backward"):
+            call({**tensors, name: t.clone().requires_grad_()})
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA device"):
+            call({**tensors, name: t.clone().requires_grad_()})
+        with forward_ad.dual_level(), pytest.raises(ValueError, match="forward-mode"):
+            call({**tensors, name: forward_ad.make_dual(t, torch.ones_like(t))})
+    with forward_ad.dual_level(), pytest.raises(ValueError, match="CUDA device"):
+        call(tensors)
