@@ -72,6 +72,8 @@ def _launch(device: int, op, *args) -> None:
     else:
         with torch.cuda.device(device):
             rc = lib.frc_serving_call(number, record.pack(*args), record.size, _raw_stream(device))
+    if rc == _lib.FRC_ERR_INVALID:
+        raise ValueError(_lib.last_error(lib))
     if rc:
         _lib.check(rc)
 
