@@ -181,8 +181,9 @@ def qk_norm_rope(qkv, heads: int, kv_heads: int, cos, sin, positions, *, bias=No
     are (zeros where this call makes the outputs).
 
     Returns q (tokens, heads, head_dim), k and v (tokens, kv_heads, head_dim)
-    in `out_dtype` (default: qkv's); `out` = (q, k, v) to write to, which may
-    be views of qkv itself.
+    in `out_dtype` (default: qkv's); `out` = (q, k, v) to write to: the three
+    parts of qkv itself, or tensors that share no memory with it or each
+    other.
     """
     in_type = _TYPE.get(qkv.dtype)
     if qkv.dim() != 2 or in_type is None:
@@ -355,7 +356,7 @@ def attention_decode_q4(q, cache, block_table, lengths, *, scale: float | None =
     t // page_size.  `scale` defaults to head_dim^-1/2.  Page numbers outside
     the cache hide their tokens, lengths are held to what the table covers, and
     a sequence without tokens gives zeros.  Returns (batch, heads, head_dim) in
-    q's type, into `out` where given.
+    q's type, into `out` where given (q itself, or apart from it).
     """
     pages, nkv, page, hd = _cache(cache)
     dtype = _TYPE.get(q.dtype)

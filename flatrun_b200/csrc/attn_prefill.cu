@@ -898,6 +898,12 @@ extern "C" int frc_attention_prefill(int type, const void* q, int64_t q_tok_stri
   FRC_REQUIRE(q && ((k && v) || tokens_k == 0) && cu_q && cu_k && out, "frc_attention_prefill: null pointer");
   FRC_REQUIRE(frc::aligned_to(q, 16) && frc::aligned_to(k, 16) && frc::aligned_to(v, 16) && frc::aligned_to(out, 16),
               "frc_attention_prefill: q, k, v and out must be 16-byte aligned");
+  const frc::View results(out, 2, tokens_q, out_tok_stride, nh, out_head_stride, hd);
+  FRC_REQUIRE(results.distinct(), "frc_attention_prefill: the rows or heads of out overlap");
+  FRC_REQUIRE(!frc::views_share(results, frc::View(q, 2, tokens_q, q_tok_stride, nh, q_head_stride, hd)) &&
+                  !frc::views_share(results, frc::View(k, 2, tokens_k, k_tok_stride, nkv, k_head_stride, hd)) &&
+                  !frc::views_share(results, frc::View(v, 2, tokens_k, v_tok_stride, nkv, v_head_stride, hd)),
+              "frc_attention_prefill: out shares memory with q, k or v");
   frc::PrefillParams p{};
   p.q = q;
   p.k = k;

@@ -1059,6 +1059,13 @@ int frc_attention_decode_q4(int type, const void* q, int64_t q_seq_stride, int64
   const int grid = static_cast<int>(want < frc::kAqGrid ? want : frc::kAqGrid);
   FRC_REQUIRE(most / grid < (int64_t(1) << 30), "frc_attention_decode_q4: block table too large");
   const size_t es = type == FRC_F32 ? 4 : 2;
+  const frc::View results(out, es, batch, out_seq_stride, nh, out_head_stride, hd), from(q, es, batch, q_seq_stride, nh, q_head_stride, hd);
+  const frc::View blocks_of(cache, 1, 1, 0, 1, 0, pages * (page_size / frc::kQ4Tokens) * nkv * frc::Q4Layout(hd).block_bytes());
+  FRC_REQUIRE(results.distinct(), "frc_attention_decode_q4: the rows or heads of out overlap");
+  // (a row is written after all that read it have)
+  const bool in_place = out == q && (batch == 1 || out_seq_stride == q_seq_stride) && (nh == 1 || out_head_stride == q_head_stride);
+  FRC_REQUIRE((in_place || !frc::views_share(results, from)) && !frc::views_share(results, blocks_of),
+              "frc_attention_decode_q4: out shares memory with the cache, or with q without being q");
   const int run = type == FRC_F32 ? 4 : 8;  // elements of a 16-byte load
   frc::AttnQ4Params p{};
   FRC_LAUNCHED(frc::serving_status(&p.status), "status word");

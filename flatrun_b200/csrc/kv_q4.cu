@@ -258,6 +258,14 @@ int kv_q4_call(const char* what, int type, KvQ4Params p, int hd, int page_size, 
   if (p.tokens == 0) return FRC_OK;
   FRC_REQUIRE(p.cache && p.slots && p.k && p.v, "kv_q4: null pointer");
   FRC_REQUIRE(aligned_to(p.cache, 16), "kv_q4: the cache must be 16-byte aligned");
+  const size_t es = type == FRC_F32 ? 4 : 2;
+  if (READ) {
+    const View k(p.k, es, p.tokens, p.k_tok, p.nkv, p.k_head, hd), v(p.v, es, p.tokens, p.v_tok, p.nkv, p.v_head, hd);
+    const View cache(p.cache, 1, 1, 0, 1, 0, p.pages * p.blocks_per_page * p.nkv * Q4Layout(hd).block_bytes());
+    FRC_REQUIRE(k.distinct() && v.distinct(), "kv_q4: the rows or heads of an output overlap");
+    FRC_REQUIRE(!views_share(k, v) && !views_share(k, cache) && !views_share(v, cache),
+                "kv_q4: the outputs share memory with each other or with the cache");
+  }
   const int run = type == FRC_F32 ? 4 : 8;  // elements of a 16-byte load
   const bool vec = aligned_to(p.k, 16) && aligned_to(p.v, 16) && p.k_tok % run == 0 && p.k_head % run == 0 &&
                    p.v_tok % run == 0 && p.v_head % run == 0;

@@ -173,6 +173,56 @@ inline cudaError_t allow_smem(K kernel, size_t bytes, std::atomic<uint64_t>& rea
 // (attn_q4.cu): bits of bounded waits that ran out, read by frc_device_status.
 cudaError_t serving_status(uint32_t** word);
 
+// A (rows, heads, channels) operand as a call gives it, in bytes.
+struct View {
+  uintptr_t at;
+  int64_t rows, row, heads, head, channels;
+  View(const void* p, size_t size, int64_t rows_, int64_t row_, int64_t heads_, int64_t head_, int64_t channels_)
+      : at(reinterpret_cast<uintptr_t>(p)), rows(rows_), row(row_ * static_cast<int64_t>(size)), heads(heads_),
+        head(head_ * static_cast<int64_t>(size)), channels(channels_ * static_cast<int64_t>(size)) {}
+  using Wide = __int128;  // strides times counts
+  Wide row_span() const { return Wide(rows - 1) * row; }
+  Wide head_span() const { return Wide(heads - 1) * head; }
+  Wide end() const { return Wide(at) + row_span() + head_span() + channels; }
+  bool empty() const { return rows < 1 || heads < 1 || channels < 1; }
+  // No two rows or heads lie over each other.
+  bool distinct() const {
+    if (empty()) return true;
+    const bool rows_inside = heads < 2 || (rows > 1 && row < head);
+    const int64_t inner = rows_inside ? row : head, outer = rows_inside ? head : row;
+    const int64_t n = rows_inside ? rows : heads, m = rows_inside ? heads : rows;
+    return (n < 2 || inner >= channels) && (m < 2 || outer >= Wide(n - 1) * inner + channels);
+  }
+};
+
+// Whether two operands share memory, for all that can be told from where they start
+// and end, and from what each holds of a period: of rows or of heads that are equally far
+// apart in both, or of the largest step that all of them are multiples of.
+inline bool views_share(const View& a, const View& b) {
+  if (a.empty() || b.empty() || a.end() <= View::Wide(b.at) || b.end() <= View::Wide(a.at)) return false;
+  int64_t common = 0;
+  auto with = [&](int64_t n, int64_t s) {
+    if (n < 2) return;
+    while (s) {
+      const int64_t r = common % s;
+      common = s;
+      s = r;
+    }
+  };
+  with(a.rows, a.row);
+  with(a.heads, a.head);
+  with(b.rows, b.row);
+  with(b.heads, b.head);
+  auto separate = [&](int64_t step, View::Wide a_holds, View::Wide b_holds) {  // in each period b is `off` behind a
+    if (step <= 0) return false;
+    const int64_t off = ((static_cast<int64_t>(b.at - a.at) % step) + step) % step;
+    return a_holds <= off && off + b_holds <= step;
+  };
+  return !(a.row == b.row && separate(a.row, a.head_span() + a.channels, b.head_span() + b.channels)) &&
+         !(a.head == b.head && separate(a.head, a.row_span() + a.channels, b.row_span() + b.channels)) &&
+         !separate(common, a.channels, b.channels);
+}
+
 inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 }  // namespace frc

@@ -204,6 +204,16 @@ extern "C" int frc_qk_norm_rope(int in_type, int out_type, const void* qkv, int6
   FRC_REQUIRE(qkv && pos_dev && q_out && k_out && v_out && (rot == 0 || (cos_table && sin_table)),
               "frc_qk_norm_rope: null pointer");
   const size_t is = in_type == FRC_F32 ? 4 : 2, os = out_type == FRC_F32 ? 4 : 2;
+  // outputs apart from everything, or all in the places of their inputs
+  const frc::View q_rows(q_out, os, tokens, q_stride, 1, 0, nq), k_rows(k_out, os, tokens, k_stride, 1, 0, nk),
+      v_rows(v_out, os, tokens, v_stride, 1, 0, nk), rows(qkv, is, tokens, row_stride, 1, 0, nq + 2 * nk);
+  FRC_REQUIRE(!frc::views_share(q_rows, k_rows) && !frc::views_share(q_rows, v_rows) && !frc::views_share(k_rows, v_rows),
+              "frc_qk_norm_rope: the outputs share memory");
+  const char* in = static_cast<const char*>(qkv);
+  const bool in_place = in_type == out_type && q_out == in && k_out == in + nq * is && v_out == in + (nq + nk) * is &&
+                        (tokens == 1 || (q_stride == row_stride && k_stride == row_stride && v_stride == row_stride));
+  FRC_REQUIRE(in_place || !(frc::views_share(q_rows, rows) || frc::views_share(k_rows, rows) || frc::views_share(v_rows, rows)),
+              "frc_qk_norm_rope: an output shares memory with qkv, but not all three in the places of their inputs");
   // four channels a load: every run starts at a multiple of four channels
   const bool vec = hd % 8 == 0 && rot % 8 == 0 && row_stride % 4 == 0 && q_stride % 4 == 0 && k_stride % 4 == 0 &&
                    v_stride % 4 == 0 && frc::aligned_to(qkv, 4 * is) && frc::aligned_to(q_out, 4 * os) &&

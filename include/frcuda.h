@@ -265,7 +265,8 @@ int frc_pos_advance(int* pos_dev, void* stream);
  *    writes q, k and v rows (heads contiguous) in out_type.  Rows whose
  *    position is outside [0, max_pos) are padding: their outputs stay as they
  *    are.  Computed in fp32.  The outputs may be the parts of the input rows
- *    themselves (same type and strides).  hd even, at most 256.
+ *    themselves (same type and strides); otherwise they share no memory with
+ *    them or each other.  hd even, at most 256.
  *  The 4-bit cache: (pages, nkv, page_size / 16) blocks of 20 * hd bytes
  *    (frc_kv_q4_bytes in all), hd 64 or 128, page_size a multiple of 16; a slot is
  *    page * page_size + offset.  Of each 32 channels of a token: m = fp16(min),
@@ -278,7 +279,7 @@ int frc_pos_advance(int* pos_dev, void* stream);
  *    of one call must differ: where two rows share one, it holds parts of
  *    both.
  *  frc_kv_read_q4: the values of slots_dev[i] into k[i], v[i]; rows whose slot is
- *    outside the cache stay as they are.
+ *    outside the cache stay as they are.  k and v share no memory.
  *  frc_attention_decode_q4: for each sequence one query token q[b] ([nh][hd])
  *    over its first lengths[b] cached tokens, the t-th in page
  *    block_table[b][t / page_size]: softmax(q.k * scale) . v per head, query
@@ -286,7 +287,8 @@ int frc_pos_advance(int* pos_dev, void* stream);
  *    their tokens, lengths are held within 0 and max_pages * page_size, and a
  *    sequence without tokens gives zeros.  `workspace` holds
  *    frc_attention_decode_q4_workspace bytes, in any state; calls that can
- *    overlap in time need one each.
+ *    overlap in time need one each.  out may be q; otherwise they share no
+ *    memory.  Scores that all overflow to -inf give NaN.
  *  frc_attention_prefill: packed sequences, sequence b being rows
  *    cu_q[b] .. cu_q[b + 1] of q and out and rows cu_k[b] .. cu_k[b + 1] of k
  *    and v; causal: the last query of a sequence sees all its keys, each

@@ -308,6 +308,66 @@ def test_outputs_that_share_memory():
                 rope(rows, out)
 
 
+@pytest.mark.skipif(torch.cuda.is_available(), reason="addresses of no memory: where a GPU is, the calls below must not be launched")
+def test_outputs_that_share_memory(lib):
+    """The C entry points refuse outputs over inputs, over each other or over themselves.  What they take gets as far as the
+    launch, which fails here without a device."""
+    taken, refused = (_lib.FRC_ERR_CUDA,), (_lib.FRC_ERR_INVALID,)
+    a = 1 << 20
+
+    def prefill(out, o=(256, 64), q=a, q_strides=(256, 64), k=1 << 24, k_strides=(128, 64), tokens=5, nh=4):
+        return lib.frc_attention_prefill(1, q, *q_strides, k, *k_strides, k + 8192, *k_strides, 16, 16, 1, tokens, 5, nh, 2, 64,
+                                         0.1, 1, out, *o, None)
+
+    far = 1 << 26
+    row = dict(q_strides=(768, 64), k=a + 512, k_strides=(768, 64))  # [q 4 | k 2 | ...| out 4] heads of 64, 2 bytes each
+    for rc, want in (
+            (prefill(far), taken), (prefill(a + 16), refused), (prefill(a - 16), refused), (prefill(a + 5 * 512), taken),
+            (prefill(a - 5 * 512), taken), (prefill(a), refused), (prefill((1 << 24) + 1024), refused),
+            (prefill(a + 512, o=(768, 64), q_strides=(768, 64)), taken),      # columns of one buffer
+            (prefill(a + 496, o=(768, 64), q_strides=(768, 64)), refused),
+            (prefill(a + 5 * 128, o=(64, 640), q_strides=(64, 640)), taken),  # heads before tokens, by turns
+            (prefill(a + 4 * 128, o=(64, 640), q_strides=(64, 640)), refused),
+            (prefill(a + 128, o=(512, 128), q_strides=(512, 128)), taken),    # heads by turns
+            (prefill(a + 112, o=(512, 128), q_strides=(512, 128)), refused),
+            (prefill(far, o=(128, 64)), refused), (prefill(far, o=(0, 64)), refused), (prefill(far, o=(64, 320)), taken),
+            (prefill(far, o=(64, 312)), refused), (prefill(far, o=(8, 64), tokens=1), taken),
+            (prefill(far, o=(64, 8), q_strides=(64, 8), nh=2), refused),
+            (prefill(far, **row), taken)):
+        assert rc in want
+
+    def decode(out, o=(256, 64), q=a, batch=3, cache=1 << 24):
+        return lib.frc_attention_decode_q4(0, q, 256, 64, cache, 3, 32, 16, 2, 2, 16, batch, 4, 2, 64, 0.1, 1 << 28, 1 << 30, out,
+                                           *o, None)
+
+    for rc, want in ((decode(far), taken), (decode(a), taken), (decode(a + 16), refused), (decode(a, o=(512, 64)), refused),
+                     (decode(a, o=(8, 64), batch=1), taken), (decode(a + 3 * 1024), taken), (decode(far, o=(192, 64)), refused),
+                     (decode((1 << 24) + 3 * 2 * 2 * 1280), taken), (decode((1 << 24) + 3 * 2 * 2 * 1280 - 16), refused)):
+        assert rc in want
+
+    def read(k, v, strides=(128, 64), v_strides=None):
+        return lib.frc_kv_read_q4(0, 1 << 24, 16, 5, 2, 64, 3, 32, k, *strides, v, *(v_strides or strides), None)
+
+    for rc, want in ((read(a, far), taken), (read(a, a), refused), (read(a, a + 2560), taken), (read(a, a + 2556), refused),
+                     (read(a, a + 256, (384, 192)), taken), (read(a, a + 128, (384, 192)), refused),
+                     (read(a, far, (64, 64)), refused), (read(a, far, v_strides=(0, 64)), refused),
+                     (read((1 << 24) + 1280, far), refused)):
+        assert rc in want
+
+    def rope(qkv, q, k, v, types=(0, 0), strides=(512, 512, 512, 512), tokens=3):
+        return lib.frc_qk_norm_rope(*types, qkv, strides[0], tokens, 4, 2, 64, None, None, None, 1e-6, 16, 16, 10, 64, 0, 16, q,
+                                    strides[1], k, strides[2], v, strides[3], None)
+
+    own = (a, a, a + 1024, a + 1536)
+    for rc, want in ((rope(*own), taken), (rope(*own, types=(0, 1)), refused), (rope(*own, strides=(512, 512, 520, 512)), refused),
+                     (rope(*own, strides=(512, 256, 128, 128), tokens=1), taken), (rope(a, a, a + 1536, a + 1024), refused),
+                     (rope(a, far, far + 1024, far + 1536), taken), (rope(a, far, far + 1024, far + 1024), refused),
+                     (rope(a, far, far + 1020, far + 1536), refused), (rope(a, a, far, far + 512), refused),
+                     (rope(a + 2048, a, far, far + 512, strides=(1024,) * 4), taken),
+                     (rope(a + 1020, a, far, far + 512, strides=(1024,) * 4), refused)):
+        assert rc in want
+
+
 def test_operators_raise_value_errors(monkeypatch):
     """What the library refuses raises ValueError from the Python entry points, as what they refuse themselves does."""
     monkeypatch.setattr(A, "_device", lambda first, *others: 0)

@@ -104,3 +104,32 @@ def test_launches_of_a_token():
         eng.step()
         assert eng.launches_per_token == counts[-1]
     assert counts[1] - counts[0] == Q.TINY.L
+
+
+def test_outputs_in_place_and_beside():
+    """Decode attention into its queries and into columns of their buffer gives what it gives into memory of its own; an
+    output that lies over them by a part is refused."""
+    from flatrun_b200 import attention as A
+
+    g = torch.Generator(device="cuda")
+    g.manual_seed(2)
+    lens = [700, 3, 0, 5000]
+    cache = A.kv_cache_q4(100, 64, 2, 128)
+    k, v = (torch.randn((6400, 2, 128), generator=g, device="cuda") for _ in range(2))
+    A.kv_append_q4(cache, k, v, torch.arange(6400, device="cuda"))
+    table = torch.arange(100, dtype=torch.int32, device="cuda").repeat(4, 1)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    for heads in (4, 32):
+        buffer = torch.zeros((4, 2 * heads, 128), device="cuda")
+        q, beside = buffer[:, :heads], buffer[:, heads:]
+        q.copy_(torch.randn(q.shape, generator=g, device="cuda"))
+        ref = A.attention_decode_q4(q, cache, table, n)
+        for _ in range(5):
+            again = q.clone()
+            A.attention_decode_q4(q, cache, table, n, out=beside)
+            A.attention_decode_q4(again, cache, table, n, out=again)
+            assert torch.equal(beside, ref) and torch.equal(again, ref)
+        with pytest.raises(ValueError, match="share"):
+            A.attention_decode_q4(q, cache, table, n, out=buffer[:, 1:heads + 1])
+        with pytest.raises(ValueError, match="finite"):
+            A.attention_decode_q4(q, cache, table, n, scale=float("nan"))
