@@ -250,64 +250,6 @@ def test_derivatives_of_either_mode_are_refused(operator):
         call(tensors)
 
 
-def test_outputs_that_share_memory():
-    """Outputs over inputs, over each other or over themselves are refused; the parts of a projection, columns and heads of one
-    buffer, and what the documentation allows in place get as far as the device."""
-    half = torch.float16
-    cu = torch.tensor([0, 5], dtype=torch.int32)
-    device, share, own = "CUDA device", "share", "overlap"
-
-    # prompt attention: everything in one buffer
-    base = torch.zeros(5 * 4 * 64 * 8, dtype=half)
-    q, k = base[:1280].view(5, 4, 64), torch.zeros(5, 2, 64, dtype=half)
-    row = torch.zeros(5, (4 + 2 + 2 + 4) * 64, dtype=half)
-    parts = [p.unflatten(1, (-1, 64)) for p in row.split((256, 128, 128, 256), dim=1)]
-    heads_first = torch.zeros(4, 2, 5, 64, dtype=half)
-    for out, args, msg in (
-            (base[8:1288].view(5, 4, 64), (q, k, k), "out must not be"),
-            (base[1272:2552].view(5, 4, 64), (q, k, k), "out must not be"),
-            (base[1280:2560].view(5, 4, 64), (q, k, k), device),
-            (parts[3], parts[:3], device),
-            (row[:, 128:384].unflatten(1, (4, 64)), parts[:3], "out must not be"),
-            (heads_first[:, 0].transpose(0, 1), (heads_first[:, 1].transpose(0, 1), k, k), device),
-            (torch.zeros(9, 4, 64, dtype=half).as_strided((5, 4, 64), (128, 64, 1)), (q, k, k), own),
-            (torch.zeros(64, dtype=half).expand(5, 4, 64), (q, k, k), own),
-            (torch.zeros(5, 256, dtype=half).view(5, 4, 64), (q, q[:, 1:3], q[:, :2]), device)):
-        with pytest.raises(ValueError, match=msg):
-            A.attention_prefill(*args, cu, out=out)
-
-    # decode: q itself, apart, or not at all
-    cache = A.kv_cache_q4(2, 32, 2, 64, device="cpu")
-    n = torch.zeros(3, dtype=torch.int32)
-    q = torch.zeros(4 * 4 * 64)
-    for out, msg in ((q[:768].view(3, 4, 64), device), (q[4:772].view(3, 4, 64), share), (q[256:].view(3, 4, 64), share),
-                     (torch.zeros(1, 4, 64).expand(3, 4, 64), own)):
-        with pytest.raises(ValueError, match=msg):
-            A.attention_decode_q4(q[:768].view(3, 4, 64), cache, n[:, None], n, out=out)
-
-    # cache read: keys and values in one buffer
-    slots, kv = torch.zeros(5, dtype=torch.int64), torch.zeros(5, 2, 3, 64)
-    for out, msg in (((kv[:, :, 0], kv[:, :, 1]), device), ((kv[:, :, 0], kv[:, :, 0]), share),
-                     ((kv[:, :, 0], kv.view(5, 2, 192)[..., 32:96]), share), ((kv[:, :, 0], kv[:1, :, 1].expand(5, 2, 64)), own)):
-        with pytest.raises(ValueError, match=msg):
-            A.kv_read_q4(cache, slots, out=out)
-
-    # rotation: the rows' own parts, or apart
-    def rope(qkv, out):
-        A.qk_norm_rope(qkv, 4, 2, torch.zeros(9, 32), torch.zeros(9, 32), torch.zeros(len(qkv), dtype=torch.int32), out=out)
-
-    wide = torch.zeros(3, 1024)
-    for rows in (wide[:, 256:768], wide[:1, 256:768]):
-        own_parts = [p.unflatten(1, (-1, 64)) for p in rows.split((256, 128, 128), dim=1)]
-        beside = wide[:len(rows), 768:].unflatten(1, (4, 64))
-        fresh = [torch.zeros_like(p) for p in own_parts]
-        for out, msg in ((own_parts, device), (fresh, device), ([beside, fresh[1], fresh[2]], device),
-                         ([own_parts[0], own_parts[2], own_parts[1]], share), ([fresh[0], fresh[1], fresh[1]], share),
-                         ([wide[:len(rows), 200:456].unflatten(1, (4, 64)), *fresh[1:]], share)):
-            with pytest.raises(ValueError, match=msg):
-                rope(rows, out)
-
-
 @pytest.mark.skipif(torch.cuda.is_available(), reason="addresses of no memory: where a GPU is, the calls below must not be launched")
 def test_outputs_that_share_memory(lib):
     """The C entry points refuse outputs over inputs, over each other or over themselves.  What they take gets as far as the
