@@ -290,10 +290,33 @@ class HBMStreamer:
             t.join()
 
 
-def decoder_config(reader: GGUFReader, max_pos: int | None = None):
+def file_rope_scaling(reader: GGUFReader) -> dict | None:
+    """The file's ``rope.scaling.*`` as a rope_scaling of ``DecoderConfig``, None where it has none."""
+    arch = reader.metadata.get("general.architecture", "qwen2")
+    g = lambda key: reader.metadata.get(f"{arch}.rope.scaling.{key}")  # noqa: E731
+    kind = g("type") or "none"
+    if kind == "none":
+        return None
+    if kind not in ("linear", "yarn") or g("factor") is None or (kind == "yarn" and g("original_context_length") is None):
+        raise ValueError(f"{arch}.rope.scaling of type {kind!r}: only linear (factor) and yarn (factor, "
+                         "original_context_length) are taken from a file")
+    out = {"type": kind, "factor": float(g("factor"))}
+    if kind == "yarn":
+        out["original_max_position"] = int(g("original_context_length"))
+        if g("attn_factor") is not None:
+            out["attention_factor"] = float(g("attn_factor"))
+    return out
+
+
+def decoder_config(reader: GGUFReader, max_pos: int | None = None, rope_scaling: dict | str | None = None):
     """The decoder configuration of a Qwen2 GGUF file (its ``qwen2.*``
-    metadata, the vocabulary from the embedding's rows)."""
+    metadata, the vocabulary from the embedding's rows).  `rope_scaling` is
+    ``DecoderConfig``'s, or "file" for what the file's metadata asks for
+    (None: the reference's tables, whatever the file says)."""
     from .decode import DecoderConfig
+
+    if rope_scaling == "file":
+        rope_scaling = file_rope_scaling(reader)
 
     md = reader.metadata
     arch = md.get("general.architecture", "qwen2")
@@ -304,21 +327,22 @@ def decoder_config(reader: GGUFReader, max_pos: int | None = None):
                          kv_heads=int(g("attention.head_count_kv")),
                          eps=float(g("attention.layer_norm_rms_epsilon", 1e-6)),
                          rope_theta=float(g("rope.freq_base", 1e6)),
-                         max_pos=int(max_pos or g("context_length", 4096)))
+                         max_pos=int(max_pos or g("context_length", 4096)), rope_scaling=rope_scaling)
 
 
 def load_decoder(path: str, device: int = 0, max_pos: int | None = None, streamer: HBMStreamer | None = None,
-                 **engine_kwargs):
+                 rope_scaling: dict | str | None = None, **engine_kwargs):
     """A ``DecodeEngine`` whose weights stream from a Qwen2 GGUF file into
     HBM: every tensor is submitted in layer order at once, and the engine's
-    construction takes each one as it lands (layer 0 first)."""
+    construction takes each one as it lands (layer 0 first).  `rope_scaling`
+    as in ``decoder_config``; other keywords go to the engine."""
     import torch
 
     from . import _lib
     from .decode import DecodeEngine
 
     reader = GGUFReader(path)
-    cfg = decoder_config(reader, max_pos)
+    cfg = decoder_config(reader, max_pos, rope_scaling)
     own = streamer is None
     st = streamer or HBMStreamer(device)
     order = sorted(reader.tensors, key=_layer_order)

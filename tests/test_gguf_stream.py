@@ -78,6 +78,55 @@ def test_reader_round_trip(tmp_path):
             (Q.TINY.H, Q.TINY.F, Q.TINY.V, Q.TINY.L, Q.TINY.NH, Q.TINY.NKV)
 
 
+@pytest.mark.parametrize("meta,want", [
+    ({}, None),
+    ({"type": (W.STR, "none")}, None),
+    ({"type": (W.STR, "linear"), "factor": (W.F32, 4.0)}, {"type": "linear", "factor": 4.0}),
+    ({"type": (W.STR, "yarn"), "factor": (W.F32, 2.0), "original_context_length": (W.U32, 32768)},
+     {"type": "yarn", "factor": 2.0, "original_max_position": 32768}),
+    ({"type": (W.STR, "yarn"), "factor": (W.F32, 2.0)}, ValueError),
+    ({"type": (W.STR, "longrope"), "factor": (W.F32, 2.0)}, ValueError),
+])
+def test_rope_scaling_of_a_file(tmp_path, meta, want):
+    """Taken from the file where that is asked for, from the caller, or not at all."""
+    path = str(tmp_path / "t.gguf")
+    emb = np.zeros((8, 64), np.float32)
+    md = {"general.architecture": (W.STR, "qwen2"), "qwen2.block_count": (W.U32, 1), "qwen2.embedding_length": (W.U32, 64),
+          "qwen2.feed_forward_length": (W.U32, 64), "qwen2.attention.head_count": (W.U32, 1),
+          "qwen2.attention.head_count_kv": (W.U32, 1), **{f"qwen2.rope.scaling.{k}": v for k, v in meta.items()}}
+    W.write_gguf(path, md, [("token_embd.weight", 0, emb.shape, emb)])
+    reader = G.GGUFReader(path)
+    assert G.decoder_config(reader).rope_scaling is None
+    own = {"type": "ntk", "factor": 3.0}
+    assert G.decoder_config(reader, rope_scaling=own).rope_scaling == own
+    if want is ValueError:
+        with pytest.raises(ValueError, match="rope.scaling"):
+            G.decoder_config(reader, rope_scaling="file")
+    else:
+        assert G.decoder_config(reader, rope_scaling="file").rope_scaling == want
+    reader.close()
+
+
+@pytest.mark.gpu
+def test_load_decoder_stretches_the_rotation(tmp_path, cuda_backend):
+    path = str(tmp_path / "tiny.gguf")
+    _tiny_gguf(path)
+    import torch
+
+    from flatrun_b200 import attention as A
+
+    scaling = {"type": "linear", "factor": 4.0}
+    eng, plain = G.load_decoder(path, rope_scaling=scaling), G.load_decoder(path, rope_scaling="file")
+    assert eng.cfg.rope_scaling == scaling and plain.cfg.rope_scaling is None
+    cos, sin = A.rope_tables_scaled(eng.cfg.head_dim, eng.cfg.rope_theta, eng.cfg.max_pos, scaling)
+    assert np.array_equal(eng._cos.cpu().numpy(), cos) and np.array_equal(eng._sin.cpu().numpy(), sin)
+    for e in (eng, plain):
+        e.step(3)
+        e.step(5)
+    eng.logits_host(), plain.logits_host()  # (waits; this model's attention takes one key alone, so these can be equal)
+    assert torch.equal(eng.k_cache[0][0], plain.k_cache[0][0]) and not torch.equal(eng.k_cache[0][1], plain.k_cache[0][1])
+
+
 def test_reader_rejects_bad_files(tmp_path):
     bad = tmp_path / "bad.gguf"
     bad.write_bytes(b"GGML" + b"\0" * 40)
