@@ -133,3 +133,79 @@ def test_outputs_in_place_and_beside():
             A.attention_decode_q4(q, cache, table, n, out=buffer[:, 1:heads + 1])
         with pytest.raises(ValueError, match="finite"):
             A.attention_decode_q4(q, cache, table, n, scale=float("nan"))
+
+
+@pytest.mark.parametrize("bits", [32, 4])
+@pytest.mark.parametrize("parts", [(33,), (1, 5), (20, 17), (16, 40, 9)])
+def test_prefill_attention_of_every_layer(bits, parts, monkeypatch):
+    """What each layer's prompt attention is given and gives.  Keys and values are the cache's of the past and behind them
+    the prompt's own, which are the ones that the cache takes; the result is that of the 64-bit restatement."""
+    import test_attention_gpu as T
+    from flatrun_b200 import attention as A
+
+    calls = []
+    real = A.attention_prefill
+
+    def recorded(q, k, v, cu_q, cu_k, **kw):
+        out = real(q, k, v, cu_q, cu_k, **kw)
+        calls.append((q.clone(), k.clone(), v.clone(), cu_q.tolist(), cu_k.tolist(), out.clone()))
+        return out
+
+    monkeypatch.setattr(A, "attention_prefill", recorded)
+    rng = np.random.default_rng(sum(parts))
+    eng = _engine(kv_bits=bits, kv_page=16)
+
+    def cached(layer, n):
+        if bits == 32:
+            return eng.k_cache[layer][:n].clone(), eng.v_cache[layer][:n].clone()
+        return A.kv_read_q4(eng.q4_cache[layer], torch.arange(n, device="cuda"))
+
+    start = 0
+    for n in parts:
+        eng.stream.synchronize()
+        past = [cached(i, start) for i in range(Q.TINY.L)]
+        calls.clear()
+        eng.prefill(rng.integers(0, 320, n))
+        eng.stream.synchronize()
+        assert len(calls) == Q.TINY.L
+        for i, (q, k, v, cu_q, cu_k, out) in enumerate(calls):
+            assert cu_q == [0, n] and cu_k == [0, start + n]
+            for x, before, after in zip((k, v), past[i], cached(i, start + n)):
+                assert torch.equal(x[:start], before.half())
+                if bits == 32:
+                    assert torch.equal(x[start:], after[start:].half())
+                else:  # fp16's rounding and the cache's: half a step, and the roundings of d and m
+                    own = T._np(after[start:])
+                    _, d, _ = T.R.quantise(T._np(x[start:]))
+                    bound = np.repeat(d, 32, -1) * (0.5 + 16 * 2.0 ** -11) + np.abs(T._np(x[start:])).max() * 2.0 ** -10
+                    T._close(x[start:], own, bound)
+            ref, bound = T._prefill_ref(T._np(q), T._np(k), T._np(v), cu_q, cu_k, True, float(np.float32(0.125)), "fp16")
+            T._close(out, ref, bound)
+        start += n
+    assert int(eng.pos.item()) == start
+    if bits == 4:
+        assert int(eng._slot.item()) == start and int(eng._length.item()) == start + 1
+        # the next token lies behind the prompts and attends over all of them
+        eng.step(7)
+        eng.stream.synchronize()
+        q = eng.qkv[:eng.cfg.hidden].view(1, -1, 64)
+        o, bound = T._decode_ref(eng.q4_cache[-1], eng._table, torch.tensor([start + 1]), T._np(q), 0.125, "fp32", 16)
+        T._close(eng.ctx.view(1, -1, 64), o, bound)
+
+
+def test_prefill_behind_a_4_bit_past_equals_one_behind_the_same_in_fp32():
+    """An fp32 engine that starts from what a 4-bit one holds gives the same logits for the next prompt, bit for bit."""
+    from flatrun_b200 import attention as A
+
+    rng = np.random.default_rng(9)
+    first, second = rng.integers(0, 320, 21), rng.integers(0, 320, 18)
+    four = _engine(kv_bits=4, kv_page=16)
+    four.prefill(first)
+    four.stream.synchronize()
+    at = torch.arange(21, device="cuda")
+    past = {i: tuple(x.cpu().numpy() for x in A.kv_read_q4(c, at)) for i, c in enumerate(four.q4_cache)}
+    full = _engine(kv_prefill=past)
+    for e in (four, full):
+        e.prefill(second)
+    assert np.array_equal(four.logits_host(), full.logits_host())
+    assert four.argmax_host() == full.argmax_host()
