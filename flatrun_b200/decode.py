@@ -329,9 +329,12 @@ class DecodeEngine:
     def step(self, token: int | None = None) -> None:
         """One token: feed `token` (None: the previous step's argmax) and
         advance the position.  Asynchronous on the engine's stream.  Raises
-        ValueError where max_pos tokens are there already."""
+        ValueError where max_pos tokens are there already, or for a token that
+        the vocabulary does not have."""
         torch = self.torch
         self._room(1)
+        if token is not None and not 0 <= int(token) < self.cfg.vocab:
+            raise ValueError(f"token ids must lie in 0 .. {self.cfg.vocab - 1}, not {token}")
         with torch.cuda.stream(self.stream):
             if token is not None:
                 self.tok_in.fill_(int(token))

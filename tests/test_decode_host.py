@@ -85,3 +85,15 @@ def test_prefill_refuses_a_head_dim_before_anything_is_written():
     eng.cfg = DecoderConfig(80, 64, 16, 1, 1, 1, 1e-6, 1e4, 5)
     with pytest.raises(ValueError, match="head_dim"):
         eng.prefill([1, 2])
+
+
+def test_step_refuses_tokens_that_the_vocabulary_does_not_have():
+    """The embedding's row is read without a check on the device."""
+    eng = _stand_in(max_pos=9, filled=0)  # a vocabulary of 16
+    for bad in (-1, 16, 1 << 20):
+        with pytest.raises(ValueError, match="token ids"):
+            eng.step(bad)
+    assert eng.launched == 0
+    eng.step(15)
+    eng.step(0)
+    assert eng.launched == 2
