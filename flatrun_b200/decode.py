@@ -203,6 +203,8 @@ class DecodeEngine:
         self.argmax_ws = torch.zeros(int(ws.value), dtype=torch.uint8, device=self._dev)
         self._graph = None
         self.launches_per_token = 0
+        # what was filled and stored above ran on the caller's stream, tokens run on the engine's
+        torch.cuda.current_stream(self._dev).synchronize()
 
     def _store(self, layer: int, start: int, k, v) -> None:
         """Keys and values (tokens, kv_heads, head_dim) into the layer's cache from position `start` on."""

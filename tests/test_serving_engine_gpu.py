@@ -209,3 +209,14 @@ def test_prefill_behind_a_4_bit_past_equals_one_behind_the_same_in_fp32():
         e.prefill(second)
     assert np.array_equal(four.logits_host(), full.logits_host())
     assert four.argmax_host() == full.argmax_host()
+
+
+@pytest.mark.parametrize("bits", [32, 4])
+def test_construction_is_over_when_it_returns(bits):
+    """Weights, zeroed buffers and a stored past are there before the engine's own stream can touch them."""
+    kv = {i: (np.ones((40, Q.TINY.NKV, 64), np.float32),) * 2 for i in range(Q.TINY.L)}
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            _engine(kv_bits=bits, kv_prefill=kv)
+            assert side.query()
