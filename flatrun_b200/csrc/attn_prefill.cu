@@ -884,6 +884,8 @@ extern "C" int frc_attention_prefill(int type, const void* q, int64_t q_tok_stri
   FRC_REQUIRE(nh > 0 && nkv > 0 && nh <= 65535 && nh % nkv == 0, "frc_attention_prefill: needs nh a multiple of nkv");
   FRC_REQUIRE(batch >= 0 && tokens_q >= 0 && tokens_k >= 0 && tokens_q <= (1 << 30) && tokens_k <= (1 << 30),
               "frc_attention_prefill: bad batch or tokens");
+  // (an item's sequence is found 32 at a time, while the other warps' waits run: some 15 ms for as many)
+  FRC_REQUIRE(batch <= (1 << 20), "frc_attention_prefill: more than 2^20 sequences");
   const int64_t strides[] = {q_tok_stride, q_head_stride, k_tok_stride, k_head_stride,
                              v_tok_stride, v_head_stride, out_tok_stride, out_head_stride};
   for (const int64_t s : strides)

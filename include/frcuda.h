@@ -293,7 +293,7 @@ int frc_pos_advance(int* pos_dev, void* stream);
  *    cu_q[b] .. cu_q[b + 1] of q and out and rows cu_k[b] .. cu_k[b + 1] of k
  *    and v; causal: the last query of a sequence sees all its keys, each
  *    earlier one a key less.  A query that sees no key gives zeros; rows of no
- *    sequence stay as they are.  A value that is not finite reaches the rows that
+ *    sequence stay as they are.  At most 2^20 sequences.  A value that is not finite reaches the rows that
  *    see it, in its channel; masked ones reach none.  type FRC_F16 or
  *    FRC_BF16, hd 64 or 128; pointers 16-byte aligned and strides multiples of
  *    8; out apart from q, k and v (they are read while rows are written). */

@@ -318,3 +318,12 @@ def test_operators_raise_value_errors(monkeypatch):
     q, k = torch.zeros(5, 4, 64, dtype=torch.float16), torch.zeros(5, 2, 64, dtype=torch.float16)
     with pytest.raises(ValueError, match="scale must be finite"):
         A.attention_prefill(q, k, k, torch.tensor([0, 5], dtype=torch.int32), scale=math.inf)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="addresses of no memory: where a GPU is, the calls below must not be launched")
+def test_numbers_of_sequences(lib):
+    def prefill(batch):
+        return lib.frc_attention_prefill(1, 1 << 20, 256, 64, 1 << 24, 128, 64, 1 << 25, 128, 64, 16, 16, batch, 5, 5, 4, 2, 64, 0.1,
+                                         1, 1 << 26, 256, 64, None)
+
+    assert prefill(1 << 20) == _lib.FRC_ERR_CUDA and prefill((1 << 20) + 1) == _lib.FRC_ERR_INVALID
