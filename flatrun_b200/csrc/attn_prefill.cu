@@ -43,8 +43,8 @@
 // (pf_add_seen), so that an element that is not finite costs the rows beside it
 // nothing and no row is computed twice.
 //
-// Measured: 8192 tokens, causal, 64 / 8 heads of 128, bf16: 0.98 ms, 1124 TFLOP/s (0.68
-// of cuBLAS's burst rate, 0.81 of its sustained one; the card is at its power
+// Measured: 8192 tokens, causal, 64 / 8 heads of 128, bf16: 0.96 ms, 1145 TFLOP/s (0.69
+// of cuBLAS's burst rate, 0.82 of its sustained one; the card is at its power
 // limit).  A key tile's chain of scores, softmax and products takes a query tile
 // 3000 cycles (1800 in the softmax); the two tiles in turn keep the tensor pipe two
 // thirds busy.  Scores of the next 64 keys formed early, in the half of S's columns

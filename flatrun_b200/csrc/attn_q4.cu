@@ -65,14 +65,17 @@
 // places are looked up at once, a block a lane, a batch ahead) and writes the
 // units that lie wholly in its range.  (Whole CTAs on one unit with their warps
 // taking blocks in turn spent 3 us on each short sequence's head: 404 us for a
-// batch of 128 that takes 67 now.)  A unit that a boundary cuts is joined from its
+// batch of 128 that takes 68 now.)  A unit that a boundary cuts is joined from its
 // pieces, by the CTA where the CTA has all of them, otherwise from pieces that
 // the CTAs leave in the workspace, by a second kernel.
 //
-// Measured: 128 sequences of 1 to 8192 tokens, 64 / 8 heads of 128, bf16: 67 us
-// (190 MB of cache: 2.9 TB/s, 0.44 of a plain copy); 131071 tokens, 32 / 8 heads,
-// fp16: 57 us.  About 440 warp instructions a block of 16 tokens and KV head
-// keep the issue slots 68 % busy in the main loop, which is what binds.
+// Measured: 128 sequences of 1 to 8192 tokens, 64 / 8 heads of 128, bf16: 68 us
+// (190 MB of cache: 2.8 TB/s, 0.43 of a plain copy); 131071 tokens, 32 / 8 heads,
+// fp16: 59 us.  36 million warp instructions (490 a block of 16 tokens and KV head,
+// with all around the loop) would take 32 us at full issue; the slots are 60 % busy.  What
+// binds is latency at 16 warps an SM (128 registers a thread; for head_dim 128 some spill:
+// 64 bytes stored and 136 loaded for 16-bit types, 104 and 188 for fp32) and the work
+// outside the loop: opening 7 us, joining 3, the second kernel 5, waiting for the last CTAs.
 #include <cuda_runtime.h>
 
 #include <atomic>

@@ -11,13 +11,13 @@
 // found exactly, so the cache's bits follow from the definition alone.
 //
 // Bound by HBM: 2 or 4 bytes a value in, 5/8 of a byte out (append), and the
-// reverse (read), if a value takes few instructions: 7 to 10 here.  A warp takes
+// reverse (read), if a value takes few instructions.  A warp takes
 // eight tokens of one head, four lanes a token and eight channels a lane, one
 // group at a time: a group's minimum and maximum are two shuffles, a lane's eight
 // nibbles are one word, a token's K words one 4 NG byte store, and the V words of
 // eight consecutive tokens a full 32-byte sector.  65536 tokens of 8 heads of 128 in
-// bf16: 117 us appended (750 warp instructions for eight tokens of a head: the
-// issue slots bind at 3.0 TB/s), 64 us read (5.5 TB/s).  Two lanes a token
+// bf16: 117 us appended (750 warp instructions for eight tokens of a head, 23 a
+// value and lane: the issue slots bind at 3.0 TB/s), 64 us read (5.5 TB/s).  Two lanes a token
 // with twice the channels took 163 us where this took 121: fewer instructions, but
 // more code than the instruction cache holds.
 #include <cuda_runtime.h>
